@@ -336,15 +336,121 @@ int mat_pattern_rowset(const mat_pattern_spec *spec, int64_t S_kv, int64_t i,
 /* Number of (query, key) pairs over query rows [0, S_q): the pattern's nnz. */
 int mat_pattern_nnz(const mat_pattern_spec *spec, int64_t S_q, int64_t S_kv, int64_t *nnz_out);
 
+/*
+ * Paged key-value cache: pages of page_size tokens (a power of two, 8 to 1024), each token H_kv heads of D columns.
+ * Element (page, slot, head, column) of k lies at page * k_page_stride + slot * k_token_stride + head *
+ * k_head_stride + column, in ELEMENTS, so both [pages, slots, heads, D] and [pages, heads, slots, D] storage are
+ * served; the same for v.  Bases and strides are multiples of 16 bytes, D is a multiple of 8 up to 256.
+ * key_bounds holds, for every page and head, the smallest and the largest key column by column over the page's filled
+ * slots, packed [n_pages, 2, H_kv, D] in the cache's type; NULL when pages are never selected by score.
+ *
+ * A page table [B, table_width] (rows table_stride apart) of int32 names the physical page of every logical page of a
+ * sequence.  Entries of pages that a call does not touch may hold anything.  A touched entry outside [0, n_pages) is
+ * never followed: its tokens count as absent, and bit 1 (value 2) of mat_device_status is set.  The reference keeps
+ * no cache: it recomputes whole sequences (src/model.py:55-87).
+ */
+typedef struct mat_paged_cache {
+    void *k;
+    void *v;
+    void *key_bounds;
+    int64_t n_pages, page_size, H_kv, D;
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    int32_t dtype;
+    int32_t reserved;
+} mat_paged_cache;
+
+/*
+ * Writes N new tokens into the cache: sequence b owns rows [cu_seqlens[b], cu_seqlens[b+1]) of k_new and v_new and
+ * its first new token has position start[b].  cu_seqlens NULL: one token per sequence (N == B).  Rows behind
+ * cu_seqlens[B] are padding: nothing is read from or written for them.
+ *   k_new, v_new: [N, H_kv, D], heads packed, tokens *_token_stride elements apart.
+ *   q, q_out: optional queries of the same tokens, [N, H, D] with H a multiple of H_kv; q_out is packed and gets
+ *   the rotated queries (q_out may be q when that is packed).
+ *   inv_freq: rot / 2 frequencies on the device, or NULL for no rotation.  Column pair r of the first rot columns of
+ *   every key and query is turned by position * inv_freq[r]; the pair is (2r, 2r+1) when interleaved is set and
+ *   (r, r + rot/2) otherwise.  The angle is reduced in 64 bits, so far positions lose nothing.
+ * When the cache has key_bounds, those of every touched page are set from all its filled slots, whatever they were.
+ * No two sequences of a call may share a page that the call writes.
+ */
+int mat_paged_append(const mat_paged_cache *cache, const void *k_new, const void *v_new, int64_t k_token_stride,
+                     int64_t v_token_stride, int64_t N, const int32_t *cu_seqlens, const int32_t *start,
+                     const int32_t *page_table, int64_t table_width, int64_t table_stride, int64_t B,
+                     const void *q, void *q_out, int64_t H, int64_t q_token_stride, const double *inv_freq,
+                     int64_t rot, int interleaved, void *stream);
+
+/*
+ * Attention of one new token per sequence over the cache.  q: [B, H, D], heads packed, sequences q_stride elements
+ * apart; o: packed [B, H, D]; query head h reads key head h / (H / H_kv).  lengths[b] counts the cached tokens of
+ * sequence b, the new one included (its position is lengths[b] - 1); 0 gives a zero row.
+ *   left < 0: every cached token; otherwise the new token's key set under a MAT_WINDOW of `left` taps before it at
+ *   `dilation`.
+ *   pages: [B, H_kv, n_sel] logical pages to read instead (ascending and distinct, as mat_paged_select leaves them;
+ *   negative entries and entries past the length are skipped), or NULL.
+ *   scale <= 0 selects 1/sqrt(D).  A row that sees no token is zero.
+ */
+int mat_paged_decode(const mat_paged_cache *cache, const void *q, int64_t q_stride, void *o, int64_t B, int64_t H,
+                     const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,
+                     int64_t left, int64_t dilation, const int32_t *pages, int64_t n_sel, float scale,
+                     void *workspace, size_t workspace_bytes, void *stream);
+size_t mat_paged_decode_workspace_bytes(const mat_paged_cache *cache, int64_t B, int64_t H, int64_t table_width,
+                                        int64_t left, int64_t n_sel);
+
+/*
+ * The topk pages each new token reads: the page that holds the token itself and the topk - 1 best others by
+ *     score(page) = sum over the query heads of a key head and the columns d of max(q_d * lo_d, q_d * hi_d),
+ * an upper bound of the summed q . k of every key in the page.  Scores are compared in 64 bits, equal ones go to the
+ * lower page, one that is not a number ranks last.  pages: [B, H_kv, topk] int32, ascending, -1 behind the last.
+ * Needs cache->key_bounds.
+ */
+int mat_paged_select(const mat_paged_cache *cache, const void *q, int64_t q_stride, int64_t B, int64_t H,
+                     const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,
+                     int64_t topk, int32_t *pages, void *workspace, size_t workspace_bytes, void *stream);
+size_t mat_paged_select_workspace_bytes(const mat_paged_cache *cache, int64_t B, int64_t H, int64_t table_width,
+                                        int64_t topk);
+
+/*
+ * Block selection over whole sequences, the form for prompts and training: the same score with blocks of `block` keys
+ * (a multiple of 16, up to 128; the last block may be short) of k: [B, S, H_kv, D] in the place of pages and every row
+ * of q: [B, S, H, D] in the place of the new token.  causal: blocks behind the query's own are not eligible.
+ * blocks: [B, S, H_kv, topk] int32, ascending, -1 behind the last; the query's own block is always among them.
+ */
+int mat_select_blocks(const void *q, const void *k, int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype,
+                      int64_t block, int64_t topk, int causal, int32_t *blocks, void *workspace,
+                      size_t workspace_bytes, void *stream);
+size_t mat_select_blocks_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype,
+                                         int64_t block, int64_t topk);
+
+/*
+ * Attention of every query over the keys of its listed blocks, and its gradients.  q, o, dout, dq: [B, S, H, D];
+ * k, v, dk, dv: [B, S, H_kv, D]; lse: [B, S, H] fp32, the natural logarithm of each row's sum of exp(scale * q . k).
+ * D is a multiple of 8 up to 128.  An entry of blocks counts when it is a block of the sequence, is above every entry
+ * before it in its row and, with causal, not behind the query's own block.  causal also hides the keys behind the
+ * query.  A row without keys gives zeros, lse = -inf and no gradient.  The backward is deterministic (no atomics).
+ */
+int mat_selected_attn_fwd(const void *q, const void *k, const void *v, void *o, float *lse, int64_t B, int64_t S,
+                          int64_t H, int64_t H_kv, int64_t D, int dtype, const int32_t *blocks, int64_t block,
+                          int64_t topk, int causal, float scale, void *workspace, size_t workspace_bytes, void *stream);
+size_t mat_selected_attn_fwd_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype,
+                                             int64_t block, int64_t topk);
+int mat_selected_attn_bwd(const void *q, const void *k, const void *v, const void *o, const float *lse,
+                          const void *dout, void *dq, void *dk, void *dv, int64_t B, int64_t S, int64_t H, int64_t H_kv,
+                          int64_t D, int dtype, const int32_t *blocks, int64_t block, int64_t topk, int causal,
+                          float scale, void *workspace, size_t workspace_bytes, void *stream);
+size_t mat_selected_attn_bwd_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype,
+                                             int64_t block, int64_t topk);
+
 /* Name of the kernel family the last mat_sparse_attn_fwd call on this thread
  * selected ("rowwarp", "mma_window", ...): lets tests assert which path ran. */
 const char *mat_last_kernel(void);
 
 /*
  * Reads and clears the device status word of the current device (synchronises
- * with it).  0 = every kernel ran to completion; 1 = a kernel gave up on a
- * bounded wait for a staged tile and left its outputs incomplete.  No
- * counterpart in the reference, whose kernel never waits.
+ * with it).  0 = every kernel ran to completion; bit 0 = a kernel gave up on a
+ * bounded wait for a staged tile and left its outputs incomplete; bit 1 = a
+ * paged-cache call met a page table entry (or a start position) outside the
+ * cache and skipped it.  No counterpart in the reference, whose kernel never
+ * waits.
  */
 int mat_device_status(int *status_out);
 

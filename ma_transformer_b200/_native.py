@@ -23,6 +23,10 @@ EXPORTS = (
     "mat_ipc_export", "mat_ipc_open", "mat_ipc_close", "mat_sparse_attn_fwd_longformer_noalloc",
     "mat_sparse_attn_bwd", "mat_sparse_attn_bwd_workspace_bytes", "mat_sparse_attn_bwd_general", "mat_sparse_attn_bwd_general_workspace_bytes",
     "mat_longformer_shard_fwd", "mat_global_rows_partial_layout", "mat_global_rows_partial", "mat_global_rows_merge",
+    "mat_paged_append", "mat_paged_decode", "mat_paged_decode_workspace_bytes", "mat_paged_select",
+    "mat_paged_select_workspace_bytes", "mat_select_blocks", "mat_select_blocks_workspace_bytes",
+    "mat_selected_attn_fwd", "mat_selected_attn_fwd_workspace_bytes", "mat_selected_attn_bwd",
+    "mat_selected_attn_bwd_workspace_bytes",
 )
 
 
@@ -35,6 +39,17 @@ class MatPatternSpec(C.Structure):
         ("blk_rowptr", C.c_void_p), ("blk_colidx", C.c_void_p),
         ("n_global", C.c_int64), ("global_idx", C.c_void_p),
         ("q_offset", C.c_int64),
+    ]
+
+
+class MatPagedCache(C.Structure):
+    """struct mat_paged_cache"""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("key_bounds", C.c_void_p),
+        ("n_pages", C.c_int64), ("page_size", C.c_int64), ("H_kv", C.c_int64), ("D", C.c_int64),
+        ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
     ]
 
 
@@ -90,6 +105,27 @@ def _load() -> C.CDLL:
     lib.mat_global_rows_merge.restype = C.c_int
     lib.mat_global_rows_merge.argtypes = [vp, i64, i64, vp, vp, i64, i64, i64, i64, i64, C.c_int32, C.c_int32,
                                           C.c_int, C.c_float, vp]
+    cache_p = C.POINTER(MatPagedCache)
+    lib.mat_paged_append.restype = C.c_int
+    lib.mat_paged_append.argtypes = [cache_p, vp, vp, i64, i64, i64, vp, vp, vp, i64, i64, i64, vp, vp, i64, i64, vp, i64,
+                                     C.c_int, vp]
+    lib.mat_paged_decode.restype = C.c_int
+    lib.mat_paged_decode.argtypes = [cache_p, vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, C.c_float, vp, sz, vp]
+    lib.mat_paged_decode_workspace_bytes.restype = sz
+    lib.mat_paged_decode_workspace_bytes.argtypes = [cache_p, i64, i64, i64, i64, i64]
+    lib.mat_paged_select.restype = C.c_int
+    lib.mat_paged_select.argtypes = [cache_p, vp, i64, i64, i64, vp, i64, i64, vp, i64, vp, vp, sz, vp]
+    lib.mat_paged_select_workspace_bytes.restype = sz
+    lib.mat_paged_select_workspace_bytes.argtypes = [cache_p, i64, i64, i64, i64]
+    lib.mat_select_blocks.restype = C.c_int
+    lib.mat_select_blocks.argtypes = [vp, vp, i64, i64, i64, i64, i64, C.c_int, i64, i64, C.c_int, vp, vp, sz, vp]
+    lib.mat_selected_attn_fwd.restype = C.c_int
+    lib.mat_selected_attn_fwd.argtypes = [vp] * 5 + [i64] * 5 + [C.c_int, vp, i64, i64, C.c_int, C.c_float, vp, sz, vp]
+    lib.mat_selected_attn_bwd.restype = C.c_int
+    lib.mat_selected_attn_bwd.argtypes = [vp] * 9 + [i64] * 5 + [C.c_int, vp, i64, i64, C.c_int, C.c_float, vp, sz, vp]
+    for name in ("mat_select_blocks", "mat_selected_attn_fwd", "mat_selected_attn_bwd"):
+        getattr(lib, name + "_workspace_bytes").restype = sz
+        getattr(lib, name + "_workspace_bytes").argtypes = [i64] * 5 + [C.c_int, i64, i64]
     lib.mat_enable_peer_access.restype = C.c_int
     lib.mat_enable_peer_access.argtypes = [C.c_int, C.c_int]
     lib.mat_ipc_export.restype = C.c_int

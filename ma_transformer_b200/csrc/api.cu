@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "mat_common.cuh"
+#include "paged.cuh"
 
 namespace mat {
 
@@ -195,6 +196,9 @@ int mat_device_status(int *status_out) {
     int e = 0;
     if (int rc = tiled_status_read_and_clear(&e)) return rc;
     d |= e;
+    int f = 0;
+    if (int rc = paged_status_read_and_clear(&f)) return rc;
+    d |= f;
     *status_out = a | b | c | d;
     return MAT_OK;
 }

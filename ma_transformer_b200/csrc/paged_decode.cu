@@ -1,0 +1,339 @@
+// Attention of one new token per sequence over a paged cache: split over the cache's length, then joined.
+//
+// A row is (sequence, key head) with the G query heads that read it, so every key and value leaves HBM once for all of
+// them.  What a row sees is a list of n virtual tokens: the whole cache (t -> position t), a window of the framework's
+// kind (t -> first + t * dilation) or a list of pages (t -> slot t mod page of page entry t / page).  The list is cut
+// into chunks of c tokens, one CTA each; a CTA keeps the running maximum and sum of its softmax and one output row per
+// query head, and rows of several chunks leave (maximum, sum, unnormalised output) in the workspace in fp32 for
+// join_kernel, which adds them up in chunk order: the result depends on the lengths alone, not on timing.
+#include <limits.h>
+
+#include <cmath>
+
+#include "paged.cuh"
+
+namespace mat {
+namespace {
+
+constexpr int kSms = 148;
+
+struct DecodeArgs {
+    PagedView c;
+    const void *q;
+    void *o;
+    int64_t q_stride, B, H, Hkv, D;
+    const int32_t *lengths;
+    int64_t left, dilation;
+    const int32_t *pages;
+    int64_t n_sel;
+    float scale_log2;
+    int nsplit, min_chunk, tiles;   // tiles: groups of query heads per key head
+    float2 *stats;                  // [B, H, nsplit] (maximum, sum)
+    float *part;                    // [B, H, nsplit, D]
+    int *status;
+};
+
+// The virtual tokens of one row.
+struct RowTokens {
+    int64_t len, first, dil;
+    const int32_t *list;
+    int64_t n;
+    __device__ __forceinline__ RowTokens(const DecodeArgs &a, int64_t b, int64_t h) {
+        len = a.lengths[b];
+        first = 0; dil = 1; list = nullptr;
+        if (len <= 0) {
+            n = 0;
+        } else if (a.pages) {
+            list = a.pages + (b * a.Hkv + h) * a.n_sel;
+            n = a.n_sel << a.c.page_shift;
+        } else if (a.left < 0) {
+            n = len;
+        } else {
+            dil = a.dilation;
+            const int64_t back = (len - 1) / dil;
+            n = (a.left < back ? a.left : back) + 1;
+            first = len - 1 - (n - 1) * dil;
+        }
+    }
+    // tokens per chunk; rows of up to c tokens are one chunk
+    __device__ __forceinline__ int64_t chunk(const DecodeArgs &a) const {
+        const int64_t c = ((n + a.nsplit - 1) / a.nsplit + 63) / 64 * 64;
+        return c > a.min_chunk ? c : a.min_chunk;
+    }
+    // position of virtual token t, or -1
+    __device__ __forceinline__ int64_t position(const DecodeArgs &a, int64_t t) const {
+        if (!list) return first + t * dil;
+        const int64_t p = list[t >> a.c.page_shift];
+        const int64_t pos = (p << a.c.page_shift) + (t & ((1 << a.c.page_shift) - 1));
+        return p >= 0 && pos < len ? pos : -1;
+    }
+};
+
+// ---- one warp per few keys, fp32 arithmetic: any type ---------------------------------------------------------------
+// LPK lanes hold one key's columns, NV 16-byte vectors each (lanes past D idle); a warp scores 32 / LPK keys at a time,
+// U times unrolled so that their loads are in flight together.  GT query heads per CTA.
+template <typename T, int LPK, int NV, int GT, int U>
+__global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
+    constexpr int W = Vec16<T>::N, KPW = 32 / LPK, C = NV * W;
+    const int64_t b = blockIdx.z, h = blockIdx.y / a.tiles, g0 = (int64_t)(blockIdx.y % a.tiles) * GT;
+    const int64_t G = a.H / a.Hkv;
+    const int D = (int)a.D;
+    const RowTokens row(a, b, h);
+    const int64_t chunk = row.chunk(a), t0 = blockIdx.x * chunk;
+    const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
+    if (t0 >= row.n && blockIdx.x > 0) return;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, part = lane % LPK, key = lane / LPK;
+
+    float q[GT][C], acc[GT][C], m[GT], l[GT];
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+        m[g] = -INFINITY; l[g] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * LPK + part) * W;
+            if (g0 + g < G && col < D) {
+                Vec16<T>::unpack(*reinterpret_cast<const uint4 *>((const T *)a.q + b * a.q_stride + (h * G + g0 + g) * D + col), &q[g][i * W]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) q[g][i * W + j] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j) { q[g][j] *= a.scale_log2; acc[g][j] = 0.f; }
+    }
+
+    for (int64_t base = t0 + warp * (KPW * U); base < t1; base += 4 * KPW * U) {
+        uint4 kv[U][NV], vv[U][NV];
+        bool ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = base + u * KPW + key;
+            const int64_t pos = t < t1 ? row.position(a, t) : -1;
+            const int64_t phys = pos >= 0 ? physical_page(a.c, b, pos >> a.c.page_shift, a.status) : -1;
+            ok[u] = phys >= 0;
+            const int64_t slot = pos & ((1 << a.c.page_shift) - 1);
+            const T *kr = (const T *)a.c.k + phys * a.c.k_page + slot * a.c.k_tok + h * a.c.k_head;
+            const T *vr = (const T *)a.c.v + phys * a.c.v_page + slot * a.c.v_tok + h * a.c.v_head;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int col = (i * LPK + part) * W;
+                const bool in = ok[u] && col < D;
+                kv[u][i] = in ? __ldg(reinterpret_cast<const uint4 *>(kr + col)) : make_uint4(0, 0, 0, 0);
+                vv[u][i] = in ? __ldg(reinterpret_cast<const uint4 *>(vr + col)) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        float s[U][GT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float k[C];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) Vec16<T>::unpack(kv[u][i], k + i * W);
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                float d = 0.f;
+#pragma unroll
+                for (int j = 0; j < C; ++j) d = fmaf(q[g][j], k[j], d);
+#pragma unroll
+                for (int o = LPK / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+                s[u][g] = ok[u] ? d : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            float top = m[g];
+#pragma unroll
+            for (int u = 0; u < U; ++u) top = fmaxf(top, s[u][g]);
+            const float ref = top == -INFINITY ? 0.f : top;   // nothing seen yet: every weight below is 2^-inf = 0
+            const float keep = exp2f(m[g] - ref);
+            m[g] = top;
+            l[g] *= keep;
+#pragma unroll
+            for (int j = 0; j < C; ++j) acc[g][j] *= keep;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s[u][g] = exp2f(s[u][g] - ref);
+                l[g] += s[u][g];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float v[C];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) Vec16<T>::unpack(vv[u][i], v + i * W);
+#pragma unroll
+            for (int g = 0; g < GT; ++g)
+#pragma unroll
+                for (int j = 0; j < C; ++j) acc[g][j] = fmaf(s[u][g], v[j], acc[g][j]);
+        }
+    }
+    // join the key lanes of a warp, then the warps
+    extern __shared__ float sm[];        // [4][GT][D + 2]
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+#pragma unroll
+        for (int o = LPK; o < 32; o <<= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m[g], o), l2 = __shfl_xor_sync(0xffffffffu, l[g], o);
+            const float top = fmaxf(m[g], m2), ref = top == -INFINITY ? 0.f : top;
+            const float e1 = exp2f(m[g] - ref), e2 = exp2f(m2 - ref);
+            l[g] = l[g] * e1 + l2 * e2;
+            m[g] = top;
+#pragma unroll
+            for (int j = 0; j < C; ++j) acc[g][j] = acc[g][j] * e1 + __shfl_xor_sync(0xffffffffu, acc[g][j], o) * e2;
+        }
+        float *w = sm + (warp * GT + g) * (D + 2);
+        if (key == 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if ((i * LPK + part) * W < D) w[2 + (i * LPK + part) * W + j] = acc[g][i * W + j];
+            if (part == 0) { w[0] = m[g]; w[1] = l[g]; }
+        }
+    }
+    __syncthreads();
+    const bool whole = chunk >= row.n;
+    for (int g = 0; g < GT && g0 + g < G; ++g) {
+        const float *w = sm + g * (D + 2);
+        const int stride = GT * (D + 2);
+        float top = -INFINITY, sum = 0.f, e[4];
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, w[i * stride]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        for (int i = 0; i < 4; ++i) { e[i] = exp2f(w[i * stride] - ref); sum += w[i * stride + 1] * e[i]; }
+        const int64_t head = b * a.H + h * G + g0 + g;
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        for (int d = threadIdx.x; d < D; d += 128) {
+            float x = 0.f;
+            for (int i = 0; i < 4; ++i) x += w[i * stride + 2 + d] * e[i];
+            if (whole) ((T *)a.o)[head * D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x * inv);
+            else a.part[(head * a.nsplit + blockIdx.x) * D + d] = x;
+        }
+        if (!whole && threadIdx.x == 0) a.stats[head * a.nsplit + blockIdx.x] = make_float2(top, sum);
+    }
+}
+
+// ---- joining the chunks of a row -------------------------------------------------------------------------------------
+template <typename T> __global__ void __launch_bounds__(128) join_kernel(const DecodeArgs a) {
+    const int64_t b = blockIdx.y, head = b * a.H + blockIdx.x, h = blockIdx.x / (a.H / a.Hkv);
+    const RowTokens row(a, b, h);
+    const int64_t chunk = row.chunk(a);
+    if (chunk >= row.n) return;                      // written by its only chunk
+    const int n = (int)((row.n + chunk - 1) / chunk);
+    const float2 *st = a.stats + head * a.nsplit;
+    float top = -INFINITY;
+    for (int i = 0; i < n; ++i) top = fmaxf(top, st[i].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int i = 0; i < n; ++i) sum += st[i].y * exp2f(st[i].x - ref);
+    for (int d = threadIdx.x; d < a.D; d += 128) {
+        float x = 0.f;
+        for (int i = 0; i < n; ++i) x += a.part[(head * a.nsplit + i) * a.D + d] * exp2f(st[i].x - ref);
+        ((T *)a.o)[head * a.D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x / sum);
+    }
+}
+
+template <typename T, int LPK, int NV, int GT> int launch_simt(const DecodeArgs &a, cudaStream_t s) {
+    constexpr int U = NV == 1 ? 4 : 2;
+    dim3 grid((unsigned)a.nsplit, (unsigned)(a.Hkv * a.tiles), (unsigned)a.B);
+    const size_t smem = 4 * GT * (a.D + 2) * sizeof(float);
+    decode_simt_kernel<T, LPK, NV, GT, U><<<grid, 128, smem, s>>>(a);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode");
+}
+
+template <typename T, int LPK, int NV> int launch_simt_heads(const DecodeArgs &a, int gt, cudaStream_t s) {
+    switch (gt) {
+        case 1: return launch_simt<T, LPK, NV, 1>(a, s);
+        case 2: return launch_simt<T, LPK, NV, 2>(a, s);
+        default: return launch_simt<T, LPK, NV, 4>(a, s);
+    }
+}
+
+template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
+    const int64_t G = a.H / a.Hkv;
+    const int gt = G >= 4 ? 4 : (G >= 2 ? 2 : 1);
+    a.tiles = (int)((G + gt - 1) / gt);
+    const int vecs = (int)(a.D * sizeof(T) / 16);
+    int rc = vecs <= 8 ? launch_simt_heads<T, 8, 1>(a, gt, s)
+           : vecs <= 16 ? launch_simt_heads<T, 16, 1>(a, gt, s)
+           : vecs <= 32 ? launch_simt_heads<T, 32, 1>(a, gt, s) : launch_simt_heads<T, 32, 2>(a, gt, s);
+    if (rc || a.nsplit == 1) return rc;
+    join_kernel<T><<<dim3((unsigned)a.H, (unsigned)a.B), 128, 0, s>>>(a);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode's join");
+}
+
+// How many chunks a row may have, and their least size.  The lengths are on the device, so both come from the page
+// table's width; the kernels shorten the chunks' number, not their size, for shorter rows.
+void plan(const mat_paged_cache *c, int64_t B, int64_t H, int64_t width, int64_t left, int64_t n_sel, bool list,
+          int &nsplit, int &min_chunk) {
+    int64_t most = width * c->page_size;
+    if (list) most = n_sel * c->page_size;
+    else if (left >= 0 && left + 1 < most) most = left + 1;
+    const int64_t rows = B * c->H_kv;
+    min_chunk = rows >= 8 * kSms ? 1024 : rows >= 2 * kSms ? 512 : 128;
+    int64_t cap = 16 * kSms / rows;
+    if (cap < 8) cap = 8;
+    int64_t n = (most + min_chunk - 1) / min_chunk;
+    nsplit = (int)(n < 1 ? 1 : n > cap ? cap : n);
+    (void)H;
+}
+
+int check_decode(const mat_paged_cache *c, int64_t B, int64_t H, int64_t left, int64_t n_sel) {
+    if (H < c->H_kv || H % c->H_kv) return fail(MAT_ERR_INVALID, "H = %lld query heads do not divide over H_kv = %lld key heads", (long long)H, (long long)c->H_kv);
+    if (H > 65535) return fail(MAT_ERR_UNSUPPORTED, "at most 65535 query heads");
+    if (n_sel < 0 || n_sel * c->page_size > INT_MAX) return fail(MAT_ERR_INVALID, "the list of pages is too long");
+    (void)B; (void)left;
+    return MAT_OK;
+}
+
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace mat
+
+using namespace mat;
+
+extern "C" size_t mat_paged_decode_workspace_bytes(const mat_paged_cache *cache, int64_t B, int64_t H, int64_t table_width,
+                                                   int64_t left, int64_t n_sel) {
+    if (check_paged_cache(cache) || B < 1 || H < 1 || table_width < 1 || check_decode(cache, B, H, left, n_sel)) return 0;
+    int nsplit, min_chunk;
+    plan(cache, B, H, table_width, left, n_sel, n_sel > 0, nsplit, min_chunk);
+    if (nsplit == 1) return 0;
+    return align256((size_t)B * H * nsplit * sizeof(float2)) + (size_t)B * H * nsplit * cache->D * sizeof(float);
+}
+
+extern "C" int mat_paged_decode(const mat_paged_cache *cache, const void *q, int64_t q_stride, void *o, int64_t B, int64_t H,
+                                const int32_t *page_table, int64_t table_width, int64_t table_stride,
+                                const int32_t *lengths, int64_t left, int64_t dilation, const int32_t *pages,
+                                int64_t n_sel, float scale, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_paged_cache(cache)) return rc;
+    if (int rc = check_page_table(page_table, table_width, table_stride, B)) return rc;
+    if (int rc = check_decode(cache, B, H, left, n_sel)) return rc;
+    if (!q || !o || !lengths) return fail(MAT_ERR_INVALID, "q, o and lengths must be non-NULL");
+    if (((uintptr_t)q | (uintptr_t)o) % 16 || q_stride < 0 || q_stride * (int64_t)dtype_size(cache->dtype) % 16)
+        return fail(MAT_ERR_INVALID, "q and o must be 16-byte aligned and q's stride a multiple of 16 bytes");
+    if (left >= 0 && dilation < 1) return fail(MAT_ERR_INVALID, "dilation must be >= 1");
+    if (pages && n_sel < 1) return fail(MAT_ERR_INVALID, "a list of pages needs at least one entry per row");
+    if (pages && left >= 0) return fail(MAT_ERR_INVALID, "a list of pages and a window cannot be combined");
+    const size_t need = mat_paged_decode_workspace_bytes(cache, B, H, table_width, left, pages ? n_sel : 0);
+    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
+        return fail(MAT_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+    DecodeArgs a;
+    a.c = paged_view(cache, page_table, table_width, table_stride);
+    a.q = q; a.o = o; a.q_stride = q_stride;
+    a.B = B; a.H = H; a.Hkv = cache->H_kv; a.D = cache->D;
+    a.lengths = lengths; a.left = left; a.dilation = dilation;
+    a.pages = pages; a.n_sel = n_sel;
+    a.scale_log2 = (scale > 0.f ? scale : 1.0f / std::sqrt((float)cache->D)) * 1.4426950408889634f;
+    plan(cache, B, H, table_width, left, n_sel, pages != nullptr, a.nsplit, a.min_chunk);
+    a.stats = (float2 *)workspace;
+    a.part = (float *)((char *)workspace + align256((size_t)B * H * a.nsplit * sizeof(float2)));
+    if (!(a.status = paged_status_word())) return fail(MAT_ERR_CUDA, "no device status word");
+    note_kernel("paged_decode");
+    cudaStream_t s = (cudaStream_t)stream;
+    switch (cache->dtype) {
+        case MAT_F32: return launch_decode<float>(a, s);
+        case MAT_BF16: return launch_decode<__nv_bfloat16>(a, s);
+        default: return launch_decode<__half>(a, s);
+    }
+}

@@ -1,0 +1,47 @@
+// Block-selected attention: what its translation units share.
+#pragma once
+
+#include "mat_common.cuh"
+
+namespace mat {
+
+struct SelProblem {
+    const void *q, *k, *v, *o, *dout;
+    void *out, *dq, *dk, *dv;
+    const float *lse_in;
+    float *lse;
+    int64_t B, S, H, Hkv, D;
+    int dtype;
+    const int32_t *blocks;
+    int64_t block, topk, nb;
+    int causal;
+    float scale;
+    cudaStream_t stream;
+};
+
+// Which queries chose a block, the selection turned round: for (batch, key head) bh and block n the entries
+// [base[bh * (nb + 1) + n], base[bh * (nb + 1) + n + 1]) of query[bh * S * topk + ...] (ascending) and slot[...], the
+// place of the block in the query's list.
+struct SelLists {
+    int32_t *counts;   // [bh][nb][tiles] queries of a tile that chose a block, then their offset within the block's list
+    int32_t *totals;   // [bh][nb]
+    int32_t *base;     // [bh][nb + 1]
+    int32_t *query;    // [bh][S * topk]
+    uint16_t *slot;
+    int64_t tiles;
+};
+size_t sel_lists_bytes(int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk);
+SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk);
+int launch_sel_lists(const SelProblem &p, const SelLists &l);
+
+// An entry of a query's list counts when it names a block of the sequence, is above every entry before it and, with
+// causal, not behind the query's own block.  `prev` carries the largest entry so far (start at -1).
+__device__ __forceinline__ bool sel_entry_counts(int n, int &prev, int limit) {
+    if (n <= prev) return false;
+    prev = n;
+    return n < limit;
+}
+
+static inline size_t sel_align(size_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace mat
