@@ -85,23 +85,48 @@ __global__ void __launch_bounds__(128) lists_offsets_kernel(SelLists l, int64_t 
     if (lane == 0) l.totals[r] = total;
 }
 
-// totals of the blocks -> where each list starts, one warp per bh
-__global__ void __launch_bounds__(32) lists_base_kernel(SelLists l, int64_t nb) {
-    const int64_t bh = blockIdx.x;
-    const int lane = threadIdx.x;
-    int total = 0;
-    for (int64_t n0 = 0; n0 < nb; n0 += 32) {
-        const int x = n0 + lane < nb ? l.totals[bh * nb + n0 + lane] : 0;
-        int sum = x;
+// inclusive sum over the CTA's 1024 threads
+__device__ __forceinline__ int block_scan(int x, int *of_warp) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += y;
-        }
-        if (n0 + lane < nb) l.base[bh * (nb + 1) + n0 + lane] = total + sum - x;
-        total += __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
     }
-    if (lane == 0) l.base[bh * (nb + 1) + nb] = total;
+    __syncthreads();                 // of_warp may still be read from the scan before
+    if (lane == 31) of_warp[warp] = x;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += of_warp[w];
+    return x + before;
+}
+
+// totals of the blocks -> where each list starts, and the items of its rows: one CTA per bh
+__global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb, int G, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item) {
+    __shared__ int of_warp[32], carry[2];
+    const int64_t bh = blockIdx.x;
+    int entries = 0, before = 0;
+    for (int64_t n0 = 0; n0 < nb; n0 += 1024) {
+        const int64_t n = n0 + threadIdx.x;
+        const int x = n < nb ? l.totals[bh * nb + n] : 0;
+        const int sum = block_scan(x, of_warp);
+        if (n < nb) l.base[bh * (nb + 1) + n] = entries + sum - x;
+        const int mine = (int)(((int64_t)x * G + rows_per_item - 1) / rows_per_item);
+        const int isum = block_scan(mine, of_warp);
+        if (items && n < nb) {
+            const int at = before + isum - mine;
+            item_base[bh * (nb + 1) + n] = at;
+            for (int i = 0; i < mine; ++i) items[bh * max_items + at + i] = make_int2((int)n, i * rows_per_item);
+        }
+        if (threadIdx.x == 1023) { carry[0] = sum; carry[1] = isum; }
+        __syncthreads();
+        entries += carry[0];
+        before += carry[1];
+    }
+    if (threadIdx.x == 0) {
+        l.base[bh * (nb + 1) + nb] = entries;
+        if (items) item_base[bh * (nb + 1) + nb] = before;
+    }
 }
 
 // ---- one warp per row -----------------------------------------------------------------------------------------------
@@ -252,7 +277,7 @@ template <typename T> int run_fwd(const SelProblem &p) {
 }
 
 template <typename T> int run_bwd(const SelProblem &p, const SelLists &l, float *delta) {
-    if (int rc = launch_sel_lists(p, l)) return rc;
+    if (int rc = launch_sel_lists(p, l, nullptr, nullptr, 0, 1)) return rc;
     sel_rows_kernel<T, true><<<(unsigned)((p.B * p.S * p.H + 3) / 4), 128, 0, p.stream>>>(p, delta);
     if (int rc = launched("launching the selected attention's query gradient")) return rc;
     sel_keys_kernel<T><<<(unsigned)((p.B * p.S * p.Hkv + 3) / 4), 128, 0, p.stream>>>(p, l, delta);
@@ -292,13 +317,13 @@ SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, i
     return l;
 }
 
-int launch_sel_lists(const SelProblem &p, const SelLists &l) {
+int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item) {
     const unsigned bh = (unsigned)(p.B * p.Hkv);
     const dim3 grid((unsigned)l.tiles, (unsigned)((p.nb + kRange - 1) / kRange), bh);
     lists_kernel<false><<<grid, kTile, 0, p.stream>>>(p, l);
     const int64_t rows = (int64_t)bh * p.nb;
     lists_offsets_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, p.stream>>>(l, rows);
-    lists_base_kernel<<<bh, 32, 0, p.stream>>>(l, p.nb);
+    lists_base_kernel<<<bh, 1024, 0, p.stream>>>(l, p.nb, (int)(p.H / p.Hkv), items, item_base, max_items, rows_per_item);
     lists_kernel<true><<<grid, kTile, 0, p.stream>>>(p, l);
     return launched("launching the lists of a block selection");
 }
@@ -308,7 +333,8 @@ int launch_sel_lists(const SelProblem &p, const SelLists &l) {
 using namespace mat;
 
 extern "C" size_t mat_selected_attn_fwd_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype, int64_t block, int64_t topk) {
-    return 0;
+    if (check_selected(B, S, H, H_kv, D, dtype, block, topk) || dtype == MAT_F32) return 0;
+    return sel_mma_workspace_bytes(B, S, H, H_kv, D, block, topk, false);
 }
 
 extern "C" int mat_selected_attn_fwd(const void *q, const void *k, const void *v, void *o, float *lse, int64_t B, int64_t S, int64_t H,
@@ -323,16 +349,16 @@ extern "C" int mat_selected_attn_fwd(const void *q, const void *k, const void *v
     p.blocks = blocks; p.block = block; p.topk = topk; p.nb = (S + block - 1) / block; p.causal = causal != 0;
     p.scale = scale > 0.f ? scale : 1.0f / std::sqrt((float)D);
     p.stream = (cudaStream_t)stream;
-    note_kernel("selected_rows");
-    switch (dtype) {
-        case MAT_F32: return run_fwd<float>(p);
-        case MAT_BF16: return run_fwd<__nv_bfloat16>(p);
-        default: return run_fwd<__half>(p);
-    }
+    const size_t need = mat_selected_attn_fwd_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk);
+    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
+        return fail(MAT_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+    note_kernel(dtype == MAT_F32 ? "selected_rows" : "selected_mma");
+    return dtype == MAT_F32 ? run_fwd<float>(p) : launch_sel_mma(p, workspace, false);
 }
 
 extern "C" size_t mat_selected_attn_bwd_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype, int64_t block, int64_t topk) {
     if (check_selected(B, S, H, H_kv, D, dtype, block, topk)) return 0;
+    if (dtype != MAT_F32) return sel_mma_workspace_bytes(B, S, H, H_kv, D, block, topk, true);
     return sel_align((size_t)B * S * H * 4) + sel_lists_bytes(B, S, H_kv, (S + block - 1) / block, topk);
 }
 
@@ -353,11 +379,7 @@ extern "C" int mat_selected_attn_bwd(const void *q, const void *k, const void *v
     p.blocks = blocks; p.block = block; p.topk = topk; p.nb = (S + block - 1) / block; p.causal = causal != 0;
     p.scale = scale > 0.f ? scale : 1.0f / std::sqrt((float)D);
     p.stream = (cudaStream_t)stream;
-    const SelLists l = sel_lists_at((char *)workspace + sel_align((size_t)B * S * H * 4), B, S, H_kv, p.nb, topk);
-    note_kernel("selected_bwd_rows");
-    switch (dtype) {
-        case MAT_F32: return run_bwd<float>(p, l, (float *)workspace);
-        case MAT_BF16: return run_bwd<__nv_bfloat16>(p, l, (float *)workspace);
-        default: return run_bwd<__half>(p, l, (float *)workspace);
-    }
+    note_kernel(dtype == MAT_F32 ? "selected_bwd_rows" : "selected_bwd_mma");
+    if (dtype != MAT_F32) return launch_sel_mma(p, workspace, true);
+    return run_bwd<float>(p, sel_lists_at((char *)workspace + sel_align((size_t)B * S * H * 4), B, S, H_kv, p.nb, topk), (float *)workspace);
 }

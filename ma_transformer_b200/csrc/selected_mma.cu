@@ -1,0 +1,618 @@
+// Block-selected attention for 16-bit types on the warp-level tensor-core instructions.
+//
+// Queries of one sequence choose different blocks, so a tile of neighbouring queries shares no keys.  The selection is
+// turned round instead: per block the list of the rows (query, head) that chose it, gathered 16 or 64 at a time into
+// dense tiles against the block's keys, which stay in shared memory.  A row meets its blocks in different CTAs, so each
+// leaves a partial result in fp32 (forward: maximum, sum, unnormalised output; backward: its share of dq), and a second
+// kernel joins a row's partials in the order of its list.  dk and dv of a block are summed over its rows by one CTA per
+// `rows per item` rows and then over the items in order: nothing depends on timing, there are no atomics.
+//
+// The partials are the traffic: 4 D bytes written and read per (row, block) against 2 D for the gathered query, so the
+// (batch, key head) pairs are worked off in groups whose partials take about kPartBudget bytes.
+#include <cmath>
+
+#include "selected_attn.cuh"
+#include "ptx.cuh"
+
+namespace mat {
+namespace {
+
+constexpr int kFwdRows = 512;        // rows per forward item (a multiple of 64)
+constexpr int kBwdRows = 512;        // rows per backward item
+constexpr size_t kPartBudget = 64ull << 20;
+
+struct SelTile {                     // what the kernels need beside SelProblem
+    SelLists l;
+    const int2 *items;               // [bh][max_items] (block, first row)
+    const int32_t *item_base;        // [bh][nb + 1]
+    int64_t max_items;
+    float2 *stats;                   // [group rows][slots]
+    float *part;                     // [group rows][slots][D]
+    float *kv_part;                  // [group bh][max_items][nsub][2][64][D]
+    const float *delta;
+    int64_t bh0;                     // first (batch, key head) of the group
+    int G, nsub;
+    float scale_log2;
+};
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// rows [0, n) of `rows` into shared memory, the rest zeros; columns [D, cols) zeros
+template <typename T, int PITCH>
+__device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_stride, int n, int rows, int D, int cols) {
+    const int chunks = cols / 8;
+    for (int i = threadIdx.x; i < rows * chunks; i += blockDim.x) {
+        const int r = i / chunks, c = (i % chunks) * 8;
+        const bool in = r < n && c < D;
+        cp_async16(dst + r * PITCH + c, in ? src + r * row_stride + c : src, in);
+    }
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------------
+// One warp per 16 rows, NKP keys at a time; keys and values of the block are shared by the CTA's warps, each warp's
+// queries have two buffers of their own.
+template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) sel_fwd_mma_kernel(const SelProblem p, const SelTile t) {
+    constexpr int PITCH = DP + 8, NF = NKP / 8;
+    const int64_t bh = t.bh0 + blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
+    if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
+    const int2 item = t.items[bh * t.max_items + blockIdx.x];
+    const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n];
+    const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
+    const int r_end = min(item.y + kFwdRows, rows_all);
+    const int D = (int)p.D, d16 = (D + 15) / 16, block = (int)p.block, T_ = (int)p.topk;
+    const int64_t j0 = (int64_t)n * block;
+    const int held = (int)min((int64_t)block, p.S - j0);
+    extern __shared__ __align__(16) char smem[];
+    const int key_rows = (block + NKP - 1) / NKP * NKP;
+    T *ks = (T *)smem, *vs = ks + key_rows * PITCH;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    T *qs = vs + key_rows * PITCH + warp * 2 * 16 * PITCH;
+    const int64_t krow = p.Hkv * D;
+    const T *kg = (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, *vg = (const T *)p.v + ((b * p.S + j0) * p.Hkv + h) * D;
+    stage_keys<T, PITCH>(ks, kg, krow, held, key_rows, D, d16 * 16);
+    stage_keys<T, PITCH>(vs, vg, krow, held, key_rows, D, d16 * 16);
+    cp_async_commit();
+    const int32_t *queries = t.l.query + bh * p.S * T_ + e0;
+    const uint16_t *slots = t.l.slot + bh * p.S * T_ + e0;
+
+    // lane r (and r + 16) knows row r of a tile: its query, and where its partial goes
+    auto row_of = [&](int first, int &i, int64_t &at) {
+        const int r = first + lane % 16;
+        i = -1; at = 0;
+        if (r < r_end) {
+            const int e = r / t.G, g = r - e * t.G;
+            i = queries[e];
+            at = (((int64_t)blockIdx.y * p.S + i) * t.G + g) * T_ + slots[e];
+        }
+    };
+    auto stage_rows = [&](T *dst, int first, int i) {
+        const int chunks = d16 * 2;
+        for (int c = lane; c < 16 * chunks; c += 32) {
+            const int r = c / chunks, col = (c % chunks) * 8;
+            const int ir = __shfl_sync(0xffffffffu, i, r);
+            const int g = (first + r) % t.G;
+            const bool in = ir >= 0 && col < D;
+            cp_async16(dst + r * PITCH + col, in ? (const T *)p.q + ((b * p.S + ir) * p.H + h * t.G + g) * D + col : (const T *)p.q, in);
+        }
+    };
+    int first = item.y + warp * 16, cur = 0, i;
+    int64_t at;
+    row_of(first, i, at);
+    if (first < r_end) stage_rows(qs, first, i);
+    cp_async_commit();
+    cp_async_wait<1>();          // the block's keys and values
+    __shared__ uint32_t odd_keys[4];
+    if (threadIdx.x < 4) odd_keys[threadIdx.x] = 0;
+    __syncthreads();
+    // A weight of zero does not silence a value that is infinite or NaN (a padded token behind the query, say), so such
+    // values go into the product as zeros and are added to the rows that see them.
+    for (int x = threadIdx.x; x < held * d16 * 2; x += 128) {
+        T *at = vs + x / (d16 * 2) * PITCH + x % (d16 * 2) * 8;
+        for (int y = 0; y < 8; ++y) {
+            const float f = Elem<T>::to_f(at[y]);
+            if (f - f != 0.f) {
+                at[y] = Elem<T>::from_f(0.f);
+                atomicOr(&odd_keys[x / (d16 * 2) / 32], 1u << (x / (d16 * 2) % 32));
+            }
+        }
+    }
+    __syncthreads();
+    const bool odd = (odd_keys[0] | odd_keys[1] | odd_keys[2] | odd_keys[3]) != 0;
+    for (; first < r_end; first += 64) {
+        int i_next = -1;
+        int64_t at_next = 0;
+        if (first + 64 < r_end) {
+            row_of(first + 64, i_next, at_next);
+            stage_rows(qs + (cur ^ 1) * 16 * PITCH, first + 64, i_next);
+        }
+        cp_async_commit();
+        cp_async_wait<1>();
+        __syncwarp();
+        const T *q = qs + cur * 16 * PITCH;
+        uint32_t qf[DP / 16][4];
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+            if (kk < d16) ptx::ldmatrix_x4(qf[kk], ptx::smem_u32(q + (lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+        // keys of the block that a row sees: the first `vis`
+        const int mine = i < 0 ? 0 : p.causal ? min(held, (int)(i + 1 - j0)) : held;
+        const int vis0 = __shfl_sync(0xffffffffu, mine, lane / 4), vis1 = __shfl_sync(0xffffffffu, mine, lane / 4 + 8);
+        const bool full = __all_sync(0xffffffffu, mine == block);
+        float o[DP / 8][4];
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        for (int base = 0; base < held; base += NKP) {
+            const int n16 = min(NKP, block - base) / 16;
+            float s[NF][4];
+#pragma unroll
+            for (int c = 0; c < NF; ++c) s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk)
+                if (kk < d16)
+#pragma unroll
+                    for (int c = 0; c < NF / 2; ++c)
+                        if (c < n16) {
+                            uint32_t r[4];
+                            ptx::ldmatrix_x4(r, ptx::smem_u32(ks + (base + c * 16 + lane % 8 + (lane / 16) * 8) * PITCH + kk * 16 + (lane / 8 % 2) * 8));
+                            ptx::Mma<T>::run(s[2 * c], qf[kk], r[0], r[1]);
+                            ptx::Mma<T>::run(s[2 * c + 1], qf[kk], r[2], r[3]);
+                        }
+            float t0 = m0, t1 = m1;
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
+                if (!full) {
+                    const int col = base + c * 8 + (lane % 4) * 2;
+                    if (col >= vis0) s[c][0] = -INFINITY;
+                    if (col + 1 >= vis0) s[c][1] = -INFINITY;
+                    if (col >= vis1) s[c][2] = -INFINITY;
+                    if (col + 1 >= vis1) s[c][3] = -INFINITY;
+                } else if (c / 2 >= n16) {
+                    s[c][0] = s[c][1] = s[c][2] = s[c][3] = -INFINITY;
+                }
+                t0 = fmaxf(t0, fmaxf(s[c][0], s[c][1]) * t.scale_log2);
+                t1 = fmaxf(t1, fmaxf(s[c][2], s[c][3]) * t.scale_log2);
+            }
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, x));
+                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, x));
+            }
+            const float ref0 = t0 == -INFINITY ? 0.f : t0, ref1 = t1 == -INFINITY ? 0.f : t1;
+            const float keep0 = ptx::ex2(m0 - ref0), keep1 = ptx::ex2(m1 - ref1);
+            m0 = t0; m1 = t1;
+            l0 *= keep0; l1 *= keep1;
+            if (base > 0)
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c) { o[c][0] *= keep0; o[c][1] *= keep0; o[c][2] *= keep1; o[c][3] *= keep1; }
+            uint32_t pf[NF / 2][4];
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
+                const float a = ptx::ex2(fmaf(s[c][0], t.scale_log2, -ref0)), bb = ptx::ex2(fmaf(s[c][1], t.scale_log2, -ref0));
+                const float cc = ptx::ex2(fmaf(s[c][2], t.scale_log2, -ref1)), d = ptx::ex2(fmaf(s[c][3], t.scale_log2, -ref1));
+                l0 += a + bb;
+                l1 += cc + d;
+                // the weights are rounded to the inputs' type for the tensor cores: one more rounding of the kind the
+                // output has; their sum is kept in fp32
+                pf[c / 2][(c % 2) * 2] = ptx::Mma<T>::pack(a, bb);
+                pf[c / 2][(c % 2) * 2 + 1] = ptx::Mma<T>::pack(cc, d);
+            }
+#pragma unroll
+            for (int kk = 0; kk < NF / 2; ++kk)
+                if (kk < n16)
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c)
+                        if (c < d16) {
+                            uint32_t r[4];
+                            ptx::ldmatrix_x4_trans(r, ptx::smem_u32(vs + (base + kk * 16 + lane % 16) * PITCH + c * 16 + (lane / 16) * 8));
+                            ptx::Mma<T>::run(o[2 * c], pf[kk], r[0], r[1]);
+                            ptx::Mma<T>::run(o[2 * c + 1], pf[kk], r[2], r[3]);
+                        }
+        }
+        if (odd)
+            for (int j = 0; j < held; ++j) {
+                if (!(odd_keys[j / 32] >> (j % 32) & 1)) continue;
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int col = c * 8 + (lane % 4) * 2 + y % 2;
+                        if (col >= D || j >= (y < 2 ? vis0 : vis1)) continue;
+                        const float f = Elem<T>::to_f(vg[j * krow + col]);
+                        if (f - f != 0.f) o[c][y] += f;
+                    }
+            }
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+        }
+        const int64_t at0 = __shfl_sync(0xffffffffu, at, lane / 4), at1 = __shfl_sync(0xffffffffu, at, lane / 4 + 8);
+        const bool in0 = vis0 > 0, in1 = vis1 > 0;
+        if (lane % 4 == 0) {
+            if (in0) t.stats[at0] = make_float2(m0, l0);
+            if (in1) t.stats[at1] = make_float2(m1, l1);
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+            const int col = c * 8 + (lane % 4) * 2;
+            if (c * 8 < D) {
+                if (in0) *reinterpret_cast<float2 *>(t.part + at0 * D + col) = make_float2(o[c][0], o[c][1]);
+                if (in1) *reinterpret_cast<float2 *>(t.part + at1 * D + col) = make_float2(o[c][2], o[c][3]);
+            }
+        }
+        __syncwarp();
+        cur ^= 1;
+        i = i_next; at = at_next;
+    }
+    cp_async_wait<0>();
+}
+
+// Joins a row's partials in the order of its list: LPR lanes of 4 columns per row.  BWD: the sum of its shares of dq.
+template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t, int64_t rows) {
+    const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;     // (bh of the group, i, g)
+    const int col = (threadIdx.x % LPR) * 4, D = (int)p.D;
+    if (r >= rows) return;
+    const int g = (int)(r % t.G);
+    const int64_t i = r / t.G % p.S, bh = t.bh0 + r / t.G / p.S, b = bh / p.Hkv, h = bh % p.Hkv;
+    const int32_t *list = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
+    const int limit = p.causal ? (int)(i / p.block) + 1 : (int)p.nb;
+    const int64_t out = ((b * p.S + i) * p.H + h * t.G + g);
+    const bool in = col < D;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    int prev = -1;
+    if (BWD) {
+        for (int s = 0; s < p.topk; ++s) {
+            if (!sel_entry_counts(list[s], prev, limit)) continue;
+            const int subs = min(t.nsub, (int)((p.S - (int64_t)prev * p.block + 63) / 64));
+            for (int u = 0; u < subs; ++u)
+                if (in) {
+                    const float4 x = *reinterpret_cast<const float4 *>(t.part + ((r * p.topk + s) * t.nsub + u) * D + col);
+                    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+                }
+        }
+        acc.x *= p.scale; acc.y *= p.scale; acc.z *= p.scale; acc.w *= p.scale;
+    } else {
+        float m = -INFINITY, l = 0.f;
+        for (int s = 0; s < p.topk; ++s) {
+            if (!sel_entry_counts(list[s], prev, limit)) continue;
+            const float2 st = t.stats[r * p.topk + s];
+            const float4 x = in ? *reinterpret_cast<const float4 *>(t.part + (r * p.topk + s) * D + col) : acc;
+            const float top = fmaxf(m, st.x), ref = top == -INFINITY ? 0.f : top, a = ptx::ex2(m - ref), c = ptx::ex2(st.x - ref);
+            m = top;
+            l = l * a + st.y * c;
+            acc.x = acc.x * a + x.x * c; acc.y = acc.y * a + x.y * c; acc.z = acc.z * a + x.z * c; acc.w = acc.w * a + x.w * c;
+        }
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+        if (col == 0) p.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    }
+    if (!in) return;
+    T y[4] = {Elem<T>::from_f(acc.x), Elem<T>::from_f(acc.y), Elem<T>::from_f(acc.z), Elem<T>::from_f(acc.w)};
+    *reinterpret_cast<uint2 *>((T *)(BWD ? p.dq : p.out) + out * D + col) = *reinterpret_cast<uint2 *>(y);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// A tile is 64 rows against up to NKP keys of one (sub-)block.  Warp w scores rows 16 w .. 16 w + 15 and writes their
+// share of dq; for dk and dv the weights and dS go through shared memory and warp w owns 16 keys (NKP = 64), or 16 keys
+// and half of the columns (NKP = 32).
+template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
+    constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW;
+    const int64_t bhl = blockIdx.z, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
+    if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
+    const int2 item = t.items[bh * t.max_items + blockIdx.x];
+    const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n], sub = blockIdx.y;
+    const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
+    const int r_end = min(item.y + kBwdRows, rows_all);
+    const int D = (int)p.D, d16 = (D + 15) / 16, T_ = (int)p.topk;
+    const int64_t j0 = (int64_t)n * p.block + sub * 64;
+    const int keys = min((int)p.block - sub * 64, 64);                       // of the sub-block
+    const int held = (int)max((int64_t)0, min((int64_t)keys, p.S - j0)), n16 = (keys + 15) / 16;
+    if (held == 0) return;                                                    // the sequence ends before this half
+    extern __shared__ __align__(16) char smem[];
+    T *ks = (T *)smem, *vs = ks + NKP * PITCH, *qs = vs + NKP * PITCH, *os = qs + 64 * PITCH;
+    T *ps = os + 64 * PITCH, *ds = ps + 64 * WP;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t krow = p.Hkv * D;
+    stage_keys<T, PITCH>(ks, (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D, d16 * 16);
+    stage_keys<T, PITCH>(vs, (const T *)p.v + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D, d16 * 16);
+    cp_async_commit();
+    const int32_t *queries = t.l.query + bh * p.S * T_ + e0;
+    const uint16_t *slots = t.l.slot + bh * p.S * T_ + e0;
+    float dk[CF][2][4], dv[CF][2][4];
+#pragma unroll
+    for (int c = 0; c < CF; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) dk[c][x][y] = dv[c][x][y] = 0.f;
+    const int kg = warp % KW, cg = warp / KW;          // this warp's keys and column half in the key pass
+
+    for (int first = item.y; first < r_end; first += 64) {
+        // warp w gathers and owns rows 16 w .. 16 w + 15; lane r knows row r
+        const int r = first + warp * 16 + lane % 16;
+        int i = -1;
+        int64_t at = 0;
+        float lse = 0.f, delta = 0.f;
+        if (r < r_end) {
+            const int e = r / t.G, g = r - e * t.G;
+            i = queries[e];
+            at = ((((int64_t)bhl * p.S + i) * t.G + g) * T_ + slots[e]) * t.nsub + sub;
+            const int64_t row = (b * p.S + i) * p.H + h * t.G + g;
+            lse = p.lse_in[row] * 1.4426950408889634f;
+            delta = t.delta[row];
+        }
+        const int chunks = d16 * 2;
+        for (int c = lane; c < 16 * chunks; c += 32) {
+            const int rr = c / chunks, col = (c % chunks) * 8;
+            const int ir = __shfl_sync(0xffffffffu, i, rr);
+            const int64_t off = ((b * p.S + (ir < 0 ? 0 : ir)) * p.H + h * t.G + (first + warp * 16 + rr) % t.G) * D + col;
+            const bool in = ir >= 0 && col < D;
+            cp_async16(qs + (warp * 16 + rr) * PITCH + col, in ? (const T *)p.q + off : (const T *)p.q, in);
+            cp_async16(os + (warp * 16 + rr) * PITCH + col, in ? (const T *)p.dout + off : (const T *)p.dout, in);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncthreads();
+        const int mine = i < 0 ? 0 : p.causal ? max(0, (int)min((int64_t)held, i + 1 - j0)) : held;
+        const int vis0 = __shfl_sync(0xffffffffu, mine, lane / 4), vis1 = __shfl_sync(0xffffffffu, mine, lane / 4 + 8);
+        const float lse0 = __shfl_sync(0xffffffffu, lse, lane / 4), lse1 = __shfl_sync(0xffffffffu, lse, lane / 4 + 8);
+        const float del0 = __shfl_sync(0xffffffffu, delta, lane / 4), del1 = __shfl_sync(0xffffffffu, delta, lane / 4 + 8);
+        float s[NF][4], dp[NF][4];
+#pragma unroll
+        for (int c = 0; c < NF; ++c)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) s[c][y] = dp[c][y] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+            if (kk < d16) {
+                uint32_t qf[4], of[4];
+                ptx::ldmatrix_x4(qf, ptx::smem_u32(qs + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+                ptx::ldmatrix_x4(of, ptx::smem_u32(os + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+#pragma unroll
+                for (int c = 0; c < NF / 2; ++c)
+                    if (c < n16) {
+                        uint32_t x[4];
+                        const int row = c * 16 + lane % 8 + (lane / 16) * 8, col = kk * 16 + (lane / 8 % 2) * 8;
+                        ptx::ldmatrix_x4(x, ptx::smem_u32(ks + row * PITCH + col));
+                        ptx::Mma<T>::run(s[2 * c], qf, x[0], x[1]);
+                        ptx::Mma<T>::run(s[2 * c + 1], qf, x[2], x[3]);
+                        ptx::ldmatrix_x4(x, ptx::smem_u32(vs + row * PITCH + col));
+                        ptx::Mma<T>::run(dp[2 * c], of, x[0], x[1]);
+                        ptx::Mma<T>::run(dp[2 * c + 1], of, x[2], x[3]);
+                    }
+            }
+        uint32_t df[NF / 2][4];
+#pragma unroll
+        for (int c = 0; c < NF; ++c) {
+            const int col = c * 8 + (lane % 4) * 2;
+            const float a = col < vis0 ? ptx::ex2(fmaf(s[c][0], t.scale_log2, -lse0)) : 0.f;
+            const float bb = col + 1 < vis0 ? ptx::ex2(fmaf(s[c][1], t.scale_log2, -lse0)) : 0.f;
+            const float cc = col < vis1 ? ptx::ex2(fmaf(s[c][2], t.scale_log2, -lse1)) : 0.f;
+            const float d = col + 1 < vis1 ? ptx::ex2(fmaf(s[c][3], t.scale_log2, -lse1)) : 0.f;
+            // weights and dS are rounded to the inputs' type for the tensor cores, once each
+            const uint32_t p0 = ptx::Mma<T>::pack(a, bb), p1 = ptx::Mma<T>::pack(cc, d);
+            const uint32_t d0 = ptx::Mma<T>::pack(col < vis0 ? a * (dp[c][0] - del0) : 0.f, col + 1 < vis0 ? bb * (dp[c][1] - del0) : 0.f);
+            const uint32_t d1 = ptx::Mma<T>::pack(col < vis1 ? cc * (dp[c][2] - del1) : 0.f, col + 1 < vis1 ? d * (dp[c][3] - del1) : 0.f);
+            df[c / 2][(c % 2) * 2] = d0;
+            df[c / 2][(c % 2) * 2 + 1] = d1;
+            const int row = warp * 16 + lane / 4;
+            *reinterpret_cast<uint32_t *>(ps + row * WP + col) = p0;
+            *reinterpret_cast<uint32_t *>(ps + (row + 8) * WP + col) = p1;
+            *reinterpret_cast<uint32_t *>(ds + row * WP + col) = d0;
+            *reinterpret_cast<uint32_t *>(ds + (row + 8) * WP + col) = d1;
+        }
+        __syncthreads();
+        // dq share of this warp's rows, 16 columns at a time
+        const int64_t at0 = __shfl_sync(0xffffffffu, at, lane / 4), at1 = __shfl_sync(0xffffffffu, at, lane / 4 + 8);
+        const int i0 = __shfl_sync(0xffffffffu, i, lane / 4), i1 = __shfl_sync(0xffffffffu, i, lane / 4 + 8);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+            if (c < d16) {
+                float q0[4] = {0.f, 0.f, 0.f, 0.f}, q1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < NF / 2; ++kk)
+                    if (kk < n16) {
+                        uint32_t x[4];
+                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(ks + (kk * 16 + lane % 16) * PITCH + c * 16 + (lane / 16) * 8));
+                        ptx::Mma<T>::run(q0, df[kk], x[0], x[1]);
+                        ptx::Mma<T>::run(q1, df[kk], x[2], x[3]);
+                    }
+                const int col = c * 16 + (lane % 4) * 2;
+                if (i0 >= 0) {
+                    *reinterpret_cast<float2 *>(t.part + at0 * D + col) = make_float2(q0[0], q0[1]);
+                    if (c * 16 + 8 < D) *reinterpret_cast<float2 *>(t.part + at0 * D + col + 8) = make_float2(q1[0], q1[1]);
+                }
+                if (i1 >= 0) {
+                    *reinterpret_cast<float2 *>(t.part + at1 * D + col) = make_float2(q0[2], q0[3]);
+                    if (c * 16 + 8 < D) *reinterpret_cast<float2 *>(t.part + at1 * D + col + 8) = make_float2(q1[2], q1[3]);
+                }
+            }
+        // dv += P^T dO, dk += dS^T Q for this warp's keys and columns
+        if (kg < n16)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                uint32_t pa[4], da[4];
+                const int row = kk * 16 + (lane / 16) * 8 + lane % 8, col = kg * 16 + (lane / 8 % 2) * 8;
+                ptx::ldmatrix_x4_trans(pa, ptx::smem_u32(ps + row * WP + col));
+                ptx::ldmatrix_x4_trans(da, ptx::smem_u32(ds + row * WP + col));
+#pragma unroll
+                for (int c = 0; c < CF; ++c)
+                    if (cg * CF + c < d16) {
+                        uint32_t x[4];
+                        const int dc = (cg * CF + c) * 16 + (lane / 16) * 8;
+                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(os + (kk * 16 + lane % 16) * PITCH + dc));
+                        ptx::Mma<T>::run(dv[c][0], pa, x[0], x[1]);
+                        ptx::Mma<T>::run(dv[c][1], pa, x[2], x[3]);
+                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(qs + (kk * 16 + lane % 16) * PITCH + dc));
+                        ptx::Mma<T>::run(dk[c][0], da, x[0], x[1]);
+                        ptx::Mma<T>::run(dk[c][1], da, x[2], x[3]);
+                    }
+            }
+        __syncthreads();
+    }
+    float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
+    if (kg < n16)
+#pragma unroll
+        for (int c = 0; c < CF; ++c)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int col = (cg * CF + c) * 16 + x * 8 + (lane % 4) * 2, row = kg * 16 + lane / 4;
+                if ((cg * CF + c) * 16 + x * 8 < D) {
+                    *reinterpret_cast<float2 *>(out + row * D + col) = make_float2(dk[c][x][0], dk[c][x][1]);
+                    *reinterpret_cast<float2 *>(out + (row + 8) * D + col) = make_float2(dk[c][x][2], dk[c][x][3]);
+                    *reinterpret_cast<float2 *>(out + (64 + row) * D + col) = make_float2(dv[c][x][0], dv[c][x][1]);
+                    *reinterpret_cast<float2 *>(out + (64 + row + 8) * D + col) = make_float2(dv[c][x][2], dv[c][x][3]);
+                }
+            }
+}
+
+// dk and dv of a (sub-)block: the sum of its items' shares in order; zeros for a block that nobody chose
+template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(const SelProblem p, const SelTile t) {
+    const int64_t bhl = blockIdx.y, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
+    const int n = blockIdx.x / t.nsub, sub = blockIdx.x % t.nsub, D = (int)p.D;
+    const int64_t j0 = (int64_t)n * p.block + sub * 64;
+    const int held = (int)min((int64_t)min((int)p.block - sub * 64, 64), p.S - j0);
+    const int i0 = t.item_base[bh * (p.nb + 1) + n], i1 = t.item_base[bh * (p.nb + 1) + n + 1];
+    for (int x = threadIdx.x; x < held * D / 4; x += 128) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
+        for (int i = i0; i < i1; ++i) {
+            const float *src = t.kv_part + (((bhl * t.max_items + i) * t.nsub + sub) * 2) * 64 * D;
+            const float4 u = *reinterpret_cast<const float4 *>(src + x * 4), w = *reinterpret_cast<const float4 *>(src + 64 * D + x * 4);
+            a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+            c.x += w.x; c.y += w.y; c.z += w.z; c.w += w.w;
+        }
+        const int64_t at = ((b * p.S + j0 + x * 4 / D) * p.Hkv + h) * D + x * 4 % D;
+        T ya[4] = {Elem<T>::from_f(a.x * p.scale), Elem<T>::from_f(a.y * p.scale), Elem<T>::from_f(a.z * p.scale), Elem<T>::from_f(a.w * p.scale)};
+        T yc[4] = {Elem<T>::from_f(c.x), Elem<T>::from_f(c.y), Elem<T>::from_f(c.z), Elem<T>::from_f(c.w)};
+        *reinterpret_cast<uint2 *>((T *)p.dk + at) = *reinterpret_cast<uint2 *>(ya);
+        *reinterpret_cast<uint2 *>((T *)p.dv + at) = *reinterpret_cast<uint2 *>(yc);
+    }
+}
+
+// delta = dO . O of every row: D / 8 lanes of 16 bytes, padded to a power of two
+template <typename T, int LPR> __global__ void __launch_bounds__(128) sel_delta_kernel(const T *o, const T *dout, float *delta, int64_t rows, int D) {
+    const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;
+    const int col = (threadIdx.x % LPR) * 8;
+    float s = 0.f;
+    if (r < rows && col < D) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(o + r * D + col)), b = __ldg(reinterpret_cast<const uint4 *>(dout + r * D + col));
+        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s = fmaf(ptx::Mma<T>::lo(x[j]), ptx::Mma<T>::lo(y[j]), s);
+            s = fmaf(ptx::Mma<T>::hi(x[j]), ptx::Mma<T>::hi(y[j]), s);
+        }
+    }
+#pragma unroll
+    for (int x = 1; x < LPR; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (r < rows && col == 0) delta[r] = s;
+}
+
+int launched(const char *what) {
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, what);
+}
+
+// What lies where in the workspace.
+struct Plan {
+    int64_t max_items, group;       // items per (batch, key head); pairs worked off together
+    int nsub;
+    size_t lists, items, base, stats, part, kv, delta, total;
+};
+
+Plan plan(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk, bool bwd) {
+    Plan w;
+    const int64_t nb = (S + block - 1) / block, G = H / Hkv, bh = B * Hkv;
+    w.nsub = bwd ? (int)((block + 63) / 64) : 1;
+    const int64_t rows = bwd ? kBwdRows : kFwdRows;
+    w.max_items = S * topk * G / rows + nb;
+    const size_t per = (size_t)S * G * topk * w.nsub * D * 4;
+    w.group = per >= kPartBudget ? 1 : (int64_t)(kPartBudget / per);
+    if (w.group > bh) w.group = bh;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t x = at; at += sel_align(n); return x; };
+    w.lists = take(sel_lists_bytes(B, S, Hkv, nb, topk));
+    w.items = take((size_t)bh * w.max_items * sizeof(int2));
+    w.base = take((size_t)bh * (nb + 1) * 4);
+    w.stats = take(bwd ? 0 : (size_t)w.group * S * G * topk * sizeof(float2));
+    w.part = take((size_t)w.group * per);
+    w.kv = take(bwd ? (size_t)w.group * w.max_items * w.nsub * 2 * 64 * D * 4 : 0);
+    w.delta = take(bwd ? (size_t)B * S * H * 4 : 0);
+    w.total = at;
+    return w;
+}
+
+int prepare(const SelProblem &p, const Plan &w, void *ws, bool bwd, SelTile &t) {
+    char *at = (char *)ws;
+    t.l = sel_lists_at(at + w.lists, p.B, p.S, p.Hkv, p.nb, p.topk);
+    t.items = (const int2 *)(at + w.items);
+    t.item_base = (const int32_t *)(at + w.base);
+    t.max_items = w.max_items;
+    t.stats = (float2 *)(at + w.stats);
+    t.part = (float *)(at + w.part);
+    t.kv_part = (float *)(at + w.kv);
+    t.delta = (const float *)(at + w.delta);
+    t.G = (int)(p.H / p.Hkv);
+    t.nsub = w.nsub;
+    t.scale_log2 = p.scale * 1.4426950408889634f;
+    return launch_sel_lists(p, t.l, (int2 *)(at + w.items), (int32_t *)(at + w.base), t.max_items, bwd ? kBwdRows : kFwdRows);
+}
+
+template <typename T, int DP, int NKP> int fwd(const SelProblem &p, const Plan &w, SelTile t) {
+    const int64_t bh = p.B * p.Hkv;
+    const size_t smem = ((p.block + NKP - 1) / NKP * NKP * 2 + 4 * 2 * 16) * (DP + 8) * sizeof(T);
+    if (int rc = ensure_dynamic_smem((const void *)sel_fwd_mma_kernel<T, DP, NKP>, smem, "shared memory of the selected attention")) return rc;
+    for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
+        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
+        sel_fwd_mma_kernel<T, DP, NKP><<<dim3((unsigned)w.max_items, (unsigned)n), 128, smem, p.stream>>>(p, t);
+        if (p.D <= 64) sel_join_kernel<T, 16, false><<<(unsigned)((rows * 16 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
+        else sel_join_kernel<T, 32, false><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
+    }
+    return launched("launching the selected attention");
+}
+
+template <typename T, int DP, int NKP> int bwd(const SelProblem &p, const Plan &w, SelTile t) {
+    const int64_t bh = p.B * p.Hkv, all = p.B * p.S * p.H;
+    const size_t smem = ((2 * NKP + 2 * 64) * (DP + 8) + 2 * 64 * (NKP + 8)) * sizeof(T);
+    if (int rc = ensure_dynamic_smem((const void *)sel_bwd_mma_kernel<T, DP, NKP>, smem, "shared memory of the selected attention's backward")) return rc;
+    float *delta = const_cast<float *>(t.delta);
+    if (p.D <= 64) sel_delta_kernel<T, 8><<<(unsigned)((all * 8 + 127) / 128), 128, 0, p.stream>>>((const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
+    else sel_delta_kernel<T, 16><<<(unsigned)((all * 16 + 127) / 128), 128, 0, p.stream>>>((const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
+    for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
+        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
+        sel_bwd_mma_kernel<T, DP, NKP><<<dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), 128, smem, p.stream>>>(p, t);
+        if (p.D <= 64) sel_join_kernel<T, 16, true><<<(unsigned)((rows * 16 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
+        else sel_join_kernel<T, 32, true><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
+        sel_kv_join_kernel<T><<<dim3((unsigned)(p.nb * w.nsub), (unsigned)n), 128, 0, p.stream>>>(p, t);
+    }
+    return launched("launching the selected attention's backward");
+}
+
+template <typename T> int run(const SelProblem &p, void *ws, bool back) {
+    const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.block, p.topk, back);
+    SelTile t{};
+    if (int rc = prepare(p, w, ws, back, t)) return rc;
+    const bool narrow = p.block <= 32;
+    if (back) {
+        if (p.D <= 64) return narrow ? bwd<T, 64, 32>(p, w, t) : bwd<T, 64, 64>(p, w, t);
+        return narrow ? bwd<T, 128, 32>(p, w, t) : bwd<T, 128, 64>(p, w, t);
+    }
+    if (p.D <= 64) return narrow ? fwd<T, 64, 32>(p, w, t) : fwd<T, 64, 64>(p, w, t);
+    return narrow ? fwd<T, 128, 32>(p, w, t) : fwd<T, 128, 64>(p, w, t);
+}
+
+}  // namespace
+
+size_t sel_mma_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk, bool bwd) {
+    return plan(B, S, H, Hkv, D, block, topk, bwd).total;
+}
+
+int launch_sel_mma(const SelProblem &p, void *workspace, bool bwd) {
+    return p.dtype == MAT_BF16 ? run<__nv_bfloat16>(p, workspace, bwd) : run<__half>(p, workspace, bwd);
+}
+
+}  // namespace mat

@@ -248,6 +248,24 @@ def test_large_scores_stay_finite():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_keys_behind_the_query_may_hold_anything(dtype):
+    """Padded tokens behind a row, infinite or not a number, change nothing for it, in the row's own block or later ones;
+    rows that see them get what the formula gives."""
+    B, S, H, Hkv, D, block = 1, 180, 4, 2, 72, 64
+    q, k, v, do = inputs(B, S, H, Hkv, D, dtype, seed=10)
+    blocks = plain_select(q, k, block, 2, True)
+    want, tol = reference(q, k, v, do, blocks, block, True)
+    k[:, 150:], v[:, 151], v[:, 152, :, 5], v[:, 160:] = float("nan"), float("nan"), float("inf"), -float("inf")
+    out, lse = sel.forward_selected(*(t.cuda() for t in (q, k, v, blocks)), block)
+    check([out[:, :150], lse[:, :150]], [w[:, :150] for w in want[:2]], [t[:, :150] for t in tol[:2]], ("out", "lse"))
+    assert torch.isnan(out[:, 150:]).all()
+    k = inputs(B, S, H, Hkv, D, dtype, seed=10)[1]
+    out, _ = sel.forward_selected(*(t.cuda() for t in (q, k, v, blocks)), block)
+    assert torch.isfinite(out[:, :151]).all() and torch.isnan(out[:, 151:153]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("case", [CASES[2], CASES[4]], ids=str)
 def test_the_same_every_time_in_graphs_and_on_another_stream(case):
     B, S, H, Hkv, D, block, topk, causal, dtype = case
