@@ -30,7 +30,7 @@ template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const
     const int64_t tile = blockIdx.x, bh = blockIdx.z, b = bh / p.Hkv, h = bh % p.Hkv;
     const int n0 = blockIdx.y * kRange, n1 = min(n0 + kRange, (int)p.nb);
     const int tid = threadIdx.x;
-    for (int i = tid; i < kRange * (kTile / 32); i += kTile) (&mask[0][0])[i] = 0;
+    for (int i = tid; i < (n1 - n0) * (kTile / 32); i += kTile) (&mask[0][0])[i] = 0;
     __syncthreads();
     const int64_t i = tile * kTile + tid;
     const int32_t *row = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
@@ -57,9 +57,7 @@ template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const
             if (!sel_entry_counts(n, prev, limit) || n < n0 || n >= n1) continue;
             int rank = __popc(mask[n - n0][tid / 32] & ((1u << (tid % 32)) - 1));
             for (int w = 0; w < tid / 32; ++w) rank += __popc(mask[n - n0][w]);
-            const int64_t at = bh * p.S * p.topk + l.base[bh * (p.nb + 1) + n] + l.counts[(bh * p.nb + n) * l.tiles + tile] + rank;
-            l.query[at] = (int32_t)i;
-            l.slot[at] = (uint16_t)s;
+            l.entry[bh * p.S * p.topk + l.base[bh * (p.nb + 1) + n] + l.counts[(bh * p.nb + n) * l.tiles + tile] + rank] = (int32_t)(i * p.topk + s);
         }
     }
 }
@@ -236,9 +234,9 @@ template <typename T> __global__ void __launch_bounds__(128) sel_keys_kernel(con
         k[c] = in ? Elem<T>::to_f(((const T *)p.k)[r * D + c * 32 + lane]) : 0.f;
         v[c] = in ? Elem<T>::to_f(((const T *)p.v)[r * D + c * 32 + lane]) : 0.f;
     }
-    const int32_t *list = l.query + bh * p.S * p.topk;
+    const int32_t *list = l.entry + bh * p.S * p.topk;
     for (int e = l.base[bh * (p.nb + 1) + n]; e < l.base[bh * (p.nb + 1) + n + 1]; ++e) {
-        const int64_t i = list[e];
+        const int64_t i = list[e] / p.topk;
         if (p.causal && i < j) continue;
         for (int g = 0; g < G; ++g) {
             const int64_t row = (b * p.S + i) * p.H + h * G + g;
@@ -292,7 +290,7 @@ int check_selected(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int 
     if (block < 16 || block > 128 || block % 16) return fail(MAT_ERR_UNSUPPORTED, "block must be a multiple of 16 from 16 to 128, got %lld", (long long)block);
     if (topk < 1 || topk > 1024) return fail(MAT_ERR_UNSUPPORTED, "topk must be in [1, 1024], got %lld", (long long)topk);
     if (B * Hkv > 65535) return fail(MAT_ERR_UNSUPPORTED, "B * H_kv must be at most 65535");
-    if (S * topk > INT_MAX || B * S * H > (int64_t)INT_MAX * 2) return fail(MAT_ERR_UNSUPPORTED, "the sequence is too long for its topk");
+    if (S * topk > INT_MAX / (H / Hkv) || S * H > INT_MAX || B * S * H > (int64_t)INT_MAX * 2) return fail(MAT_ERR_UNSUPPORTED, "the sequence is too long for its topk");
     return MAT_OK;
 }
 
@@ -301,7 +299,7 @@ int check_selected(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int 
 size_t sel_lists_bytes(int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk) {
     const int64_t tiles = (S + kTile - 1) / kTile, bh = B * Hkv;
     return sel_align((size_t)bh * nb * tiles * 4) + sel_align((size_t)bh * nb * 4) + sel_align((size_t)bh * (nb + 1) * 4) +
-           sel_align((size_t)bh * S * topk * 4) + sel_align((size_t)bh * S * topk * 2);
+           sel_align((size_t)bh * S * topk * 4);
 }
 
 SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk) {
@@ -312,8 +310,7 @@ SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, i
     l.counts = (int32_t *)at; at += sel_align((size_t)bh * nb * l.tiles * 4);
     l.totals = (int32_t *)at; at += sel_align((size_t)bh * nb * 4);
     l.base = (int32_t *)at;   at += sel_align((size_t)bh * (nb + 1) * 4);
-    l.query = (int32_t *)at;  at += sel_align((size_t)bh * S * topk * 4);
-    l.slot = (uint16_t *)at;
+    l.entry = (int32_t *)at;
     return l;
 }
 

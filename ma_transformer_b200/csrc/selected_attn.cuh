@@ -20,14 +20,13 @@ struct SelProblem {
 };
 
 // Which queries chose a block, the selection turned round: for (batch, key head) bh and block n the entries
-// [base[bh * (nb + 1) + n], base[bh * (nb + 1) + n + 1]) of query[bh * S * topk + ...] (ascending) and slot[...], the
-// place of the block in the query's list.
+// [base[bh * (nb + 1) + n], base[bh * (nb + 1) + n + 1]) of entry[bh * S * topk + ...], ascending, each
+// query * topk + the place of the block in the query's list.
 struct SelLists {
     int32_t *counts;   // [bh][nb][tiles] queries of a tile that chose a block, then their offset within the block's list
     int32_t *totals;   // [bh][nb]
     int32_t *base;     // [bh][nb + 1]
-    int32_t *query;    // [bh][S * topk]
-    uint16_t *slot;
+    int32_t *entry;    // [bh][S * topk]
     int64_t tiles;
 };
 size_t sel_lists_bytes(int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk);

@@ -8,7 +8,9 @@
 // `rows per item` rows and then over the items in order: nothing depends on timing, there are no atomics.
 //
 // The partials are the traffic: 4 D bytes written and read per (row, block) against 2 D for the gathered query, so the
-// (batch, key head) pairs are worked off in groups whose partials take about kPartBudget bytes.
+// (batch, key head) pairs are worked off in groups whose partials take about kPartBudget bytes.  Groups small enough for
+// L2 (64 MB) were slower than all pairs at once, for the tails of their launches: 281 + 446 against 247 + 377 us forward
+// and backward at 8192 tokens x 8 heads of 64 x 16 blocks, so the budget only bounds the workspace.
 #include <cmath>
 
 #include "selected_attn.cuh"
@@ -17,9 +19,9 @@
 namespace mat {
 namespace {
 
-constexpr int kFwdRows = 512;        // rows per forward item (a multiple of 64)
+constexpr int kFwdRows = 256;        // rows per forward item (a multiple of 64)
 constexpr int kBwdRows = 512;        // rows per backward item
-constexpr size_t kPartBudget = 64ull << 20;
+constexpr size_t kPartBudget = 1024ull << 20;
 
 struct SelTile {                     // what the kernels need beside SelProblem
     SelLists l;
@@ -41,21 +43,21 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// rows [0, n) of `rows` into shared memory, the rest zeros; columns [D, cols) zeros
-template <typename T, int PITCH>
-__device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_stride, int n, int rows, int D, int cols) {
-    const int chunks = cols / 8;
-    for (int i = threadIdx.x; i < rows * chunks; i += blockDim.x) {
-        const int r = i / chunks, c = (i % chunks) * 8;
+// rows [0, n) of `rows` into shared memory, the rest zeros; columns from D on are zeros
+template <typename T, int DP>
+__device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_stride, int n, int rows, int D) {
+    for (int i = threadIdx.x; i < rows * (DP / 8); i += 128) {
+        const int r = i / (DP / 8), c = i % (DP / 8) * 8;
         const bool in = r < n && c < D;
-        cp_async16(dst + r * PITCH + c, in ? src + r * row_stride + c : src, in);
+        cp_async16(dst + r * (DP + 8) + c, in ? src + r * row_stride + c : src, in);
     }
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // One warp per 16 rows, NKP keys at a time; keys and values of the block are shared by the CTA's warps, each warp's
 // queries have two buffers of their own.
-template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) sel_fwd_mma_kernel(const SelProblem p, const SelTile t) {
+// EXACT: D == DP and a block is a whole number of NKP keys, known to the compiler.
+template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, DP == 64 ? 4 : 3) sel_fwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8;
     const int64_t bh = t.bh0 + blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
     if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
@@ -63,7 +65,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
     const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n];
     const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
     const int r_end = min(item.y + kFwdRows, rows_all);
-    const int D = (int)p.D, d16 = (D + 15) / 16, block = (int)p.block, T_ = (int)p.topk;
+    const int D = EXACT ? DP : (int)p.D, d16 = EXACT ? DP / 16 : (D + 15) / 16, block = (int)p.block, T_ = (int)p.topk;
     const int64_t j0 = (int64_t)n * block;
     const int held = (int)min((int64_t)block, p.S - j0);
     extern __shared__ __align__(16) char smem[];
@@ -73,62 +75,62 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
     T *qs = vs + key_rows * PITCH + warp * 2 * 16 * PITCH;
     const int64_t krow = p.Hkv * D;
     const T *kg = (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, *vg = (const T *)p.v + ((b * p.S + j0) * p.Hkv + h) * D;
-    stage_keys<T, PITCH>(ks, kg, krow, held, key_rows, D, d16 * 16);
-    stage_keys<T, PITCH>(vs, vg, krow, held, key_rows, D, d16 * 16);
+    stage_keys<T, DP>(ks, kg, krow, held, key_rows, D);
+    stage_keys<T, DP>(vs, vg, krow, held, key_rows, D);
     cp_async_commit();
-    const int32_t *queries = t.l.query + bh * p.S * T_ + e0;
-    const uint16_t *slots = t.l.slot + bh * p.S * T_ + e0;
-
-    // lane r (and r + 16) knows row r of a tile: its query, and where its partial goes
-    auto row_of = [&](int first, int &i, int64_t &at) {
-        const int r = first + lane % 16;
-        i = -1; at = 0;
+    // the item's rows: query (-1 past the end), row of q within the batch item, place of the partial within the pair
+    __shared__ int row_q[kFwdRows], row_src[kFwdRows], row_at[kFwdRows];
+    for (int x = threadIdx.x; x < kFwdRows; x += 128) {
+        const int r = item.y + x;
+        int i = -1, src = 0, at = 0;
         if (r < r_end) {
-            const int e = r / t.G, g = r - e * t.G;
-            i = queries[e];
-            at = (((int64_t)blockIdx.y * p.S + i) * t.G + g) * T_ + slots[e];
+            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bh * p.S * T_ + e0 + e];
+            i = entry / T_;
+            src = i * (int)p.H + g;
+            at = (i * t.G + g) * T_ + entry - i * T_;
+        }
+        row_q[x] = i; row_src[x] = src; row_at[x] = at;
+    }
+    const int64_t part0 = (int64_t)blockIdx.y * p.S * t.G * T_;
+    const T *q0 = (const T *)p.q + (b * p.S * p.H + h * t.G) * D;
+    auto stage_rows = [&](T *dst, int x) {
+#pragma unroll
+        for (int c = lane; c < 16 * (DP / 8); c += 32) {
+            const int r = c / (DP / 8), col = c % (DP / 8) * 8;
+            const bool in = row_q[x + r] >= 0 && (EXACT || col < D);
+            cp_async16(dst + r * PITCH + col, q0 + (int64_t)row_src[x + r] * D + (in ? col : 0), in);
         }
     };
-    auto stage_rows = [&](T *dst, int first, int i) {
-        const int chunks = d16 * 2;
-        for (int c = lane; c < 16 * chunks; c += 32) {
-            const int r = c / chunks, col = (c % chunks) * 8;
-            const int ir = __shfl_sync(0xffffffffu, i, r);
-            const int g = (first + r) % t.G;
-            const bool in = ir >= 0 && col < D;
-            cp_async16(dst + r * PITCH + col, in ? (const T *)p.q + ((b * p.S + ir) * p.H + h * t.G + g) * D + col : (const T *)p.q, in);
-        }
-    };
-    int first = item.y + warp * 16, cur = 0, i;
-    int64_t at;
-    row_of(first, i, at);
-    if (first < r_end) stage_rows(qs, first, i);
-    cp_async_commit();
-    cp_async_wait<1>();          // the block's keys and values
     __shared__ uint32_t odd_keys[4];
     if (threadIdx.x < 4) odd_keys[threadIdx.x] = 0;
     __syncthreads();
+    int first = item.y + warp * 16, cur = 0;
+    if (first < r_end) stage_rows(qs, first - item.y);
+    cp_async_commit();
+    cp_async_wait<1>();          // the block's keys and values
+    __syncthreads();
     // A weight of zero does not silence a value that is infinite or NaN (a padded token behind the query, say), so such
     // values go into the product as zeros and are added to the rows that see them.
-    for (int x = threadIdx.x; x < held * d16 * 2; x += 128) {
-        T *at = vs + x / (d16 * 2) * PITCH + x % (d16 * 2) * 8;
-        for (int y = 0; y < 8; ++y) {
-            const float f = Elem<T>::to_f(at[y]);
-            if (f - f != 0.f) {
-                at[y] = Elem<T>::from_f(0.f);
-                atomicOr(&odd_keys[x / (d16 * 2) / 32], 1u << (x / (d16 * 2) % 32));
+    constexpr uint32_t kExp = sizeof(T) == 2 && ptx::Mma<T>::kOnes == 0x3F803F80u ? 0x7f80u : 0x7c00u;
+    for (int x = threadIdx.x; x < held * (DP / 8); x += 128) {
+        T *at = vs + x / (DP / 8) * PITCH + x % (DP / 8) * 8;
+        const uint4 u = *reinterpret_cast<const uint4 *>(at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        bool any = false;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) any |= (w[y] & kExp) == kExp || (w[y] >> 16 & kExp) == kExp;
+        if (any) {
+            for (int y = 0; y < 8; ++y) {
+                const float f = Elem<T>::to_f(at[y]);
+                if (f - f != 0.f) at[y] = Elem<T>::from_f(0.f);
             }
+            atomicOr(&odd_keys[x / (DP / 8) / 32], 1u << (x / (DP / 8) % 32));
         }
     }
     __syncthreads();
     const bool odd = (odd_keys[0] | odd_keys[1] | odd_keys[2] | odd_keys[3]) != 0;
     for (; first < r_end; first += 64) {
-        int i_next = -1;
-        int64_t at_next = 0;
-        if (first + 64 < r_end) {
-            row_of(first + 64, i_next, at_next);
-            stage_rows(qs + (cur ^ 1) * 16 * PITCH, first + 64, i_next);
-        }
+        if (first + 64 < r_end) stage_rows(qs + (cur ^ 1) * 16 * PITCH, first + 64 - item.y);
         cp_async_commit();
         cp_async_wait<1>();
         __syncwarp();
@@ -138,6 +140,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
         for (int kk = 0; kk < DP / 16; ++kk)
             if (kk < d16) ptx::ldmatrix_x4(qf[kk], ptx::smem_u32(q + (lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
         // keys of the block that a row sees: the first `vis`
+        const int i = row_q[first - item.y + lane % 16];
         const int mine = i < 0 ? 0 : p.causal ? min(held, (int)(i + 1 - j0)) : held;
         const int vis0 = __shfl_sync(0xffffffffu, mine, lane / 4), vis1 = __shfl_sync(0xffffffffu, mine, lane / 4 + 8);
         const bool full = __all_sync(0xffffffffu, mine == block);
@@ -146,7 +149,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
         for (int c = 0; c < DP / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
         for (int base = 0; base < held; base += NKP) {
-            const int n16 = min(NKP, block - base) / 16;
+            const int n16 = EXACT ? NKP / 16 : min(NKP, block - base) / 16;
             float s[NF][4];
 #pragma unroll
             for (int c = 0; c < NF; ++c) s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.f;
@@ -161,7 +164,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
                             ptx::Mma<T>::run(s[2 * c], qf[kk], r[0], r[1]);
                             ptx::Mma<T>::run(s[2 * c + 1], qf[kk], r[2], r[3]);
                         }
-            float t0 = m0, t1 = m1;
+            float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
             for (int c = 0; c < NF; ++c) {
                 if (!full) {
@@ -170,17 +173,19 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
                     if (col + 1 >= vis0) s[c][1] = -INFINITY;
                     if (col >= vis1) s[c][2] = -INFINITY;
                     if (col + 1 >= vis1) s[c][3] = -INFINITY;
-                } else if (c / 2 >= n16) {
+                } else if (!EXACT && c / 2 >= n16) {
                     s[c][0] = s[c][1] = s[c][2] = s[c][3] = -INFINITY;
                 }
-                t0 = fmaxf(t0, fmaxf(s[c][0], s[c][1]) * t.scale_log2);
-                t1 = fmaxf(t1, fmaxf(s[c][2], s[c][3]) * t.scale_log2);
+                t0 = fmaxf(t0, fmaxf(s[c][0], s[c][1]));
+                t1 = fmaxf(t1, fmaxf(s[c][2], s[c][3]));
             }
 #pragma unroll
             for (int x = 1; x < 4; x <<= 1) {
                 t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, x));
                 t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, x));
             }
+            t0 = fmaxf(m0, t0 * t.scale_log2);
+            t1 = fmaxf(m1, t1 * t.scale_log2);
             const float ref0 = t0 == -INFINITY ? 0.f : t0, ref1 = t1 == -INFINITY ? 0.f : t1;
             const float keep0 = ptx::ex2(m0 - ref0), keep1 = ptx::ex2(m1 - ref1);
             m0 = t0; m1 = t1;
@@ -230,7 +235,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
             l0 += __shfl_xor_sync(0xffffffffu, l0, x);
             l1 += __shfl_xor_sync(0xffffffffu, l1, x);
         }
-        const int64_t at0 = __shfl_sync(0xffffffffu, at, lane / 4), at1 = __shfl_sync(0xffffffffu, at, lane / 4 + 8);
+        const int64_t at0 = part0 + row_at[first - item.y + lane / 4], at1 = part0 + row_at[first - item.y + lane / 4 + 8];
         const bool in0 = vis0 > 0, in1 = vis1 > 0;
         if (lane % 4 == 0) {
             if (in0) t.stats[at0] = make_float2(m0, l0);
@@ -246,52 +251,79 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
         }
         __syncwarp();
         cur ^= 1;
-        i = i_next; at = at_next;
     }
     cp_async_wait<0>();
 }
 
-// Joins a row's partials in the order of its list: LPR lanes of 4 columns per row.  BWD: the sum of its shares of dq.
+// Joins a row's partials in the order of its list: LPR lanes of 4 columns per row.  The lanes first look at LPR entries
+// of the list together (which count, and with what weight), then read the partials of those that do, four at a time.
+// BWD: the sum of a row's shares of dq.
 template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t, int64_t rows) {
     const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;     // (bh of the group, i, g)
-    const int col = (threadIdx.x % LPR) * 4, D = (int)p.D;
-    if (r >= rows) return;
-    const int g = (int)(r % t.G);
-    const int64_t i = r / t.G % p.S, bh = t.bh0 + r / t.G / p.S, b = bh / p.Hkv, h = bh % p.Hkv;
+    const int lane = threadIdx.x % LPR, col = lane * 4, D = (int)p.D, T_ = (int)p.topk;
+    const bool live = r < rows, in = live && col < D;
+    const int64_t rr = live ? r : 0;
+    const int g = (int)(rr % t.G);
+    const int64_t i = rr / t.G % p.S, bh = t.bh0 + rr / t.G / p.S, b = bh / p.Hkv, h = bh % p.Hkv;
     const int32_t *list = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
     const int limit = p.causal ? (int)(i / p.block) + 1 : (int)p.nb;
     const int64_t out = ((b * p.S + i) * p.H + h * t.G + g);
-    const bool in = col < D;
+    const float *part = t.part + rr * T_ * t.nsub * D + col;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
     int prev = -1;
-    if (BWD) {
-        for (int s = 0; s < p.topk; ++s) {
-            if (!sel_entry_counts(list[s], prev, limit)) continue;
-            const int subs = min(t.nsub, (int)((p.S - (int64_t)prev * p.block + 63) / 64));
-            for (int u = 0; u < subs; ++u)
-                if (in) {
-                    const float4 x = *reinterpret_cast<const float4 *>(t.part + ((r * p.topk + s) * t.nsub + u) * D + col);
+    for (int s0 = 0; s0 < T_; s0 += LPR) {
+        const int s = s0 + lane;
+        const int n = s < T_ ? list[s] : -1;
+        int top = n;                                   // largest entry up to this lane's
+#pragma unroll
+        for (int x = 1; x < LPR; x <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, top, x, LPR);
+            if (lane >= x) top = max(top, y);
+        }
+        int before = __shfl_up_sync(0xffffffffu, top, 1, LPR);
+        before = lane == 0 ? prev : max(prev, before);
+        const bool counts = n > before && n < limit;
+        prev = max(prev, __shfl_sync(0xffffffffu, top, LPR - 1, LPR));
+        // BWD: how many sub-blocks of the block hold keys
+        int uses = counts ? 1 : 0;
+        float w = counts ? 1.f : 0.f;
+        if (BWD) {
+            if (counts) uses = min(t.nsub, (int)((p.S - (int64_t)n * p.block + 63) / 64));
+        } else {
+            const float2 st = counts && live ? t.stats[rr * T_ + s] : make_float2(-INFINITY, 0.f);
+            float mx = st.x;
+#pragma unroll
+            for (int x = LPR / 2; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x, LPR));
+            const float now = fmaxf(m, mx), ref = now == -INFINITY ? 0.f : now, keep = ptx::ex2(m - ref);
+            m = now;
+            w = ptx::ex2(st.x - ref);
+            float sum = st.y * w;
+#pragma unroll
+            for (int x = LPR / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x, LPR);
+            l = l * keep + sum;
+            acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+        }
+        const int cnt = min(LPR, T_ - s0);
+#pragma unroll 4
+        for (int y = 0; y < cnt; ++y) {
+            const int use = __shfl_sync(0xffffffffu, uses, y, LPR);
+            const float f = __shfl_sync(0xffffffffu, w, y, LPR);
+            if (BWD) {
+                for (int u = 0; u < t.nsub; ++u) {
+                    const float4 x = in && u < use ? *reinterpret_cast<const float4 *>(part + ((s0 + y) * t.nsub + u) * (int64_t)D) : make_float4(0.f, 0.f, 0.f, 0.f);
                     acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
                 }
+            } else {
+                const float4 x = in && use ? *reinterpret_cast<const float4 *>(part + (s0 + y) * (int64_t)D) : make_float4(0.f, 0.f, 0.f, 0.f);
+                acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+            }
         }
-        acc.x *= p.scale; acc.y *= p.scale; acc.z *= p.scale; acc.w *= p.scale;
-    } else {
-        float m = -INFINITY, l = 0.f;
-        for (int s = 0; s < p.topk; ++s) {
-            if (!sel_entry_counts(list[s], prev, limit)) continue;
-            const float2 st = t.stats[r * p.topk + s];
-            const float4 x = in ? *reinterpret_cast<const float4 *>(t.part + (r * p.topk + s) * D + col) : acc;
-            const float top = fmaxf(m, st.x), ref = top == -INFINITY ? 0.f : top, a = ptx::ex2(m - ref), c = ptx::ex2(st.x - ref);
-            m = top;
-            l = l * a + st.y * c;
-            acc.x = acc.x * a + x.x * c; acc.y = acc.y * a + x.y * c; acc.z = acc.z * a + x.z * c; acc.w = acc.w * a + x.w * c;
-        }
-        const float f = l == 0.f ? 0.f : 1.f / l;
-        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-        if (col == 0) p.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
     if (!in) return;
-    T y[4] = {Elem<T>::from_f(acc.x), Elem<T>::from_f(acc.y), Elem<T>::from_f(acc.z), Elem<T>::from_f(acc.w)};
+    const float f = BWD ? p.scale : l == 0.f ? 0.f : 1.f / l;
+    if (!BWD && lane == 0) p.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    T y[4] = {Elem<T>::from_f(acc.x * f), Elem<T>::from_f(acc.y * f), Elem<T>::from_f(acc.z * f), Elem<T>::from_f(acc.w * f)};
     *reinterpret_cast<uint2 *>((T *)(BWD ? p.dq : p.out) + out * D + col) = *reinterpret_cast<uint2 *>(y);
 }
 
@@ -299,29 +331,60 @@ template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) 
 // A tile is 64 rows against up to NKP keys of one (sub-)block.  Warp w scores rows 16 w .. 16 w + 15 and writes their
 // share of dq; for dk and dv the weights and dS go through shared memory and warp w owns 16 keys (NKP = 64), or 16 keys
 // and half of the columns (NKP = 32).
-template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
-    constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW;
+template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, 2) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
+    constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW, NBUF = DP == 64 ? 2 : 1;
     const int64_t bhl = blockIdx.z, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
     if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
     const int2 item = t.items[bh * t.max_items + blockIdx.x];
     const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n], sub = blockIdx.y;
     const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
     const int r_end = min(item.y + kBwdRows, rows_all);
-    const int D = (int)p.D, d16 = (D + 15) / 16, T_ = (int)p.topk;
+    const int D = EXACT ? DP : (int)p.D, d16 = EXACT ? DP / 16 : (D + 15) / 16, T_ = (int)p.topk;
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
     const int keys = min((int)p.block - sub * 64, 64);                       // of the sub-block
-    const int held = (int)max((int64_t)0, min((int64_t)keys, p.S - j0)), n16 = (keys + 15) / 16;
+    const int held = (int)max((int64_t)0, min((int64_t)keys, p.S - j0)), n16 = EXACT ? NKP / 16 : (keys + 15) / 16;
     if (held == 0) return;                                                    // the sequence ends before this half
     extern __shared__ __align__(16) char smem[];
-    T *ks = (T *)smem, *vs = ks + NKP * PITCH, *qs = vs + NKP * PITCH, *os = qs + 64 * PITCH;
-    T *ps = os + 64 * PITCH, *ds = ps + 64 * WP;
+    T *ks = (T *)smem, *vs = ks + NKP * PITCH, *qs = vs + NKP * PITCH, *ps = qs + NBUF * 128 * PITCH, *ds = ps + 64 * WP;
+    int *row_q = (int *)(ds + 64 * WP), *row_at = row_q + kBwdRows;
+    int *row_src = row_at + kBwdRows;
+    float *row_lse = (float *)(row_src + kBwdRows), *row_delta = row_lse + kBwdRows;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t krow = p.Hkv * D;
-    stage_keys<T, PITCH>(ks, (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D, d16 * 16);
-    stage_keys<T, PITCH>(vs, (const T *)p.v + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D, d16 * 16);
+    stage_keys<T, DP>(ks, (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D);
+    stage_keys<T, DP>(vs, (const T *)p.v + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D);
     cp_async_commit();
-    const int32_t *queries = t.l.query + bh * p.S * T_ + e0;
-    const uint16_t *slots = t.l.slot + bh * p.S * T_ + e0;
+    for (int x = threadIdx.x; x < kBwdRows; x += 128) {
+        const int r = item.y + x;
+        int i = -1, at = 0, src = 0;
+        float lse = 0.f, delta = 0.f;
+        if (r < r_end) {
+            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bh * p.S * T_ + e0 + e];
+            i = entry / T_;
+            at = (i * t.G + g) * T_ + entry - i * T_;
+            src = i * (int)p.H + g;
+            const int64_t row = b * p.S * p.H + h * t.G + src;
+            lse = p.lse_in[row] * 1.4426950408889634f;
+            delta = t.delta[row];
+        }
+        row_q[x] = i; row_at[x] = at; row_src[x] = src; row_lse[x] = lse; row_delta[x] = delta;
+    }
+    const int64_t part0 = (int64_t)bhl * p.S * t.G * T_;
+    // queries and output gradients of 64 rows: warp w gathers (and scores) rows 16 w .. 16 w + 15
+    const int64_t src0 = (b * p.S * p.H + h * t.G) * D;
+    auto stage_rows = [&](T *dst, int x) {
+#pragma unroll
+        for (int c = lane; c < 16 * (DP / 8); c += 32) {
+            const int r = warp * 16 + c / (DP / 8), col = c % (DP / 8) * 8;
+            const bool in = row_q[x + r] >= 0 && (EXACT || col < D);
+            const int64_t off = src0 + (int64_t)row_src[x + r] * D + (in ? col : 0);
+            cp_async16(dst + r * PITCH + col, (const T *)p.q + off, in);
+            cp_async16(dst + (64 + r) * PITCH + col, (const T *)p.dout + off, in);
+        }
+        cp_async_commit();
+    };
+    __syncthreads();
+    stage_rows(qs, 0);
     float dk[CF][2][4], dv[CF][2][4];
 #pragma unroll
     for (int c = 0; c < CF; ++c)
@@ -331,36 +394,16 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
             for (int y = 0; y < 4; ++y) dk[c][x][y] = dv[c][x][y] = 0.f;
     const int kg = warp % KW, cg = warp / KW;          // this warp's keys and column half in the key pass
 
-    for (int first = item.y; first < r_end; first += 64) {
-        // warp w gathers and owns rows 16 w .. 16 w + 15; lane r knows row r
-        const int r = first + warp * 16 + lane % 16;
-        int i = -1;
-        int64_t at = 0;
-        float lse = 0.f, delta = 0.f;
-        if (r < r_end) {
-            const int e = r / t.G, g = r - e * t.G;
-            i = queries[e];
-            at = ((((int64_t)bhl * p.S + i) * t.G + g) * T_ + slots[e]) * t.nsub + sub;
-            const int64_t row = (b * p.S + i) * p.H + h * t.G + g;
-            lse = p.lse_in[row] * 1.4426950408889634f;
-            delta = t.delta[row];
-        }
-        const int chunks = d16 * 2;
-        for (int c = lane; c < 16 * chunks; c += 32) {
-            const int rr = c / chunks, col = (c % chunks) * 8;
-            const int ir = __shfl_sync(0xffffffffu, i, rr);
-            const int64_t off = ((b * p.S + (ir < 0 ? 0 : ir)) * p.H + h * t.G + (first + warp * 16 + rr) % t.G) * D + col;
-            const bool in = ir >= 0 && col < D;
-            cp_async16(qs + (warp * 16 + rr) * PITCH + col, in ? (const T *)p.q + off : (const T *)p.q, in);
-            cp_async16(os + (warp * 16 + rr) * PITCH + col, in ? (const T *)p.dout + off : (const T *)p.dout, in);
-        }
-        cp_async_commit();
+    int cur = 0;
+    for (int first = item.y; first < r_end; first += 64, cur ^= NBUF - 1) {
+        const T *qt = qs + cur * 128 * PITCH, *ot = qt + 64 * PITCH;
         cp_async_wait<0>();
-        __syncthreads();
-        const int mine = i < 0 ? 0 : p.causal ? max(0, (int)min((int64_t)held, i + 1 - j0)) : held;
-        const int vis0 = __shfl_sync(0xffffffffu, mine, lane / 4), vis1 = __shfl_sync(0xffffffffu, mine, lane / 4 + 8);
-        const float lse0 = __shfl_sync(0xffffffffu, lse, lane / 4), lse1 = __shfl_sync(0xffffffffu, lse, lane / 4 + 8);
-        const float del0 = __shfl_sync(0xffffffffu, delta, lane / 4), del1 = __shfl_sync(0xffffffffu, delta, lane / 4 + 8);
+        __syncthreads();                 // this tile is in; the other buffer, ps and ds are free again
+        if (NBUF == 2 && first + 64 < r_end) stage_rows(qs + (cur ^ 1) * 128 * PITCH, first + 64 - item.y);
+        const int x0 = first - item.y + warp * 16 + lane / 4, x1 = x0 + 8, i0 = row_q[x0], i1 = row_q[x1];
+        const int vis0 = i0 < 0 ? 0 : p.causal ? max(0, (int)min((int64_t)held, i0 + 1 - j0)) : held;
+        const int vis1 = i1 < 0 ? 0 : p.causal ? max(0, (int)min((int64_t)held, i1 + 1 - j0)) : held;
+        const float lse0 = row_lse[x0], lse1 = row_lse[x1], del0 = row_delta[x0], del1 = row_delta[x1];
         float s[NF][4], dp[NF][4];
 #pragma unroll
         for (int c = 0; c < NF; ++c)
@@ -370,8 +413,8 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
         for (int kk = 0; kk < DP / 16; ++kk)
             if (kk < d16) {
                 uint32_t qf[4], of[4];
-                ptx::ldmatrix_x4(qf, ptx::smem_u32(qs + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
-                ptx::ldmatrix_x4(of, ptx::smem_u32(os + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+                ptx::ldmatrix_x4(qf, ptx::smem_u32(qt + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+                ptx::ldmatrix_x4(of, ptx::smem_u32(ot + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
 #pragma unroll
                 for (int c = 0; c < NF / 2; ++c)
                     if (c < n16) {
@@ -385,7 +428,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
                         ptx::Mma<T>::run(dp[2 * c + 1], of, x[2], x[3]);
                     }
             }
-        uint32_t df[NF / 2][4];
+        uint32_t df[NF / 2][4], dl[NF / 2][4];
 #pragma unroll
         for (int c = 0; c < NF; ++c) {
             const int col = c * 8 + (lane % 4) * 2;
@@ -393,12 +436,17 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
             const float bb = col + 1 < vis0 ? ptx::ex2(fmaf(s[c][1], t.scale_log2, -lse0)) : 0.f;
             const float cc = col < vis1 ? ptx::ex2(fmaf(s[c][2], t.scale_log2, -lse1)) : 0.f;
             const float d = col + 1 < vis1 ? ptx::ex2(fmaf(s[c][3], t.scale_log2, -lse1)) : 0.f;
-            // weights and dS are rounded to the inputs' type for the tensor cores, once each
+            // Weights and dS are rounded to the inputs' type for the products over the rows (dv, dk: one rounding of the
+            // kind the result has).  dq has the rounded output's error in delta beside its own rounding, so dS goes into
+            // it as two halves, rounded value and rest: 1.9e-3 off instead of 2.6e-3 for bf16.
+            const float ea = col < vis0 ? a * (dp[c][0] - del0) : 0.f, eb = col + 1 < vis0 ? bb * (dp[c][1] - del0) : 0.f;
+            const float ec = col < vis1 ? cc * (dp[c][2] - del1) : 0.f, ed = col + 1 < vis1 ? d * (dp[c][3] - del1) : 0.f;
             const uint32_t p0 = ptx::Mma<T>::pack(a, bb), p1 = ptx::Mma<T>::pack(cc, d);
-            const uint32_t d0 = ptx::Mma<T>::pack(col < vis0 ? a * (dp[c][0] - del0) : 0.f, col + 1 < vis0 ? bb * (dp[c][1] - del0) : 0.f);
-            const uint32_t d1 = ptx::Mma<T>::pack(col < vis1 ? cc * (dp[c][2] - del1) : 0.f, col + 1 < vis1 ? d * (dp[c][3] - del1) : 0.f);
+            const uint32_t d0 = ptx::Mma<T>::pack(ea, eb), d1 = ptx::Mma<T>::pack(ec, ed);
             df[c / 2][(c % 2) * 2] = d0;
             df[c / 2][(c % 2) * 2 + 1] = d1;
+            dl[c / 2][(c % 2) * 2] = ptx::Mma<T>::pack(ea - ptx::Mma<T>::lo(d0), eb - ptx::Mma<T>::hi(d0));
+            dl[c / 2][(c % 2) * 2 + 1] = ptx::Mma<T>::pack(ec - ptx::Mma<T>::lo(d1), ed - ptx::Mma<T>::hi(d1));
             const int row = warp * 16 + lane / 4;
             *reinterpret_cast<uint32_t *>(ps + row * WP + col) = p0;
             *reinterpret_cast<uint32_t *>(ps + (row + 8) * WP + col) = p1;
@@ -407,8 +455,7 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
         }
         __syncthreads();
         // dq share of this warp's rows, 16 columns at a time
-        const int64_t at0 = __shfl_sync(0xffffffffu, at, lane / 4), at1 = __shfl_sync(0xffffffffu, at, lane / 4 + 8);
-        const int i0 = __shfl_sync(0xffffffffu, i, lane / 4), i1 = __shfl_sync(0xffffffffu, i, lane / 4 + 8);
+        const int64_t at0 = (part0 + row_at[x0]) * t.nsub + sub, at1 = (part0 + row_at[x1]) * t.nsub + sub;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
             if (c < d16) {
@@ -420,6 +467,8 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
                         ptx::ldmatrix_x4_trans(x, ptx::smem_u32(ks + (kk * 16 + lane % 16) * PITCH + c * 16 + (lane / 16) * 8));
                         ptx::Mma<T>::run(q0, df[kk], x[0], x[1]);
                         ptx::Mma<T>::run(q1, df[kk], x[2], x[3]);
+                        ptx::Mma<T>::run(q0, dl[kk], x[0], x[1]);
+                        ptx::Mma<T>::run(q1, dl[kk], x[2], x[3]);
                     }
                 const int col = c * 16 + (lane % 4) * 2;
                 if (i0 >= 0) {
@@ -444,15 +493,18 @@ template <typename T, int DP, int NKP> __global__ void __launch_bounds__(128) se
                     if (cg * CF + c < d16) {
                         uint32_t x[4];
                         const int dc = (cg * CF + c) * 16 + (lane / 16) * 8;
-                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(os + (kk * 16 + lane % 16) * PITCH + dc));
+                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(ot + (kk * 16 + lane % 16) * PITCH + dc));
                         ptx::Mma<T>::run(dv[c][0], pa, x[0], x[1]);
                         ptx::Mma<T>::run(dv[c][1], pa, x[2], x[3]);
-                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(qs + (kk * 16 + lane % 16) * PITCH + dc));
+                        ptx::ldmatrix_x4_trans(x, ptx::smem_u32(qt + (kk * 16 + lane % 16) * PITCH + dc));
                         ptx::Mma<T>::run(dk[c][0], da, x[0], x[1]);
                         ptx::Mma<T>::run(dk[c][1], da, x[2], x[3]);
                     }
             }
-        __syncthreads();
+        if (NBUF == 1) {
+            __syncthreads();             // every warp is done with the tile
+            if (first + 64 < r_end) stage_rows(qs, first + 64 - item.y);
+        }
     }
     float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
     if (kg < n16)
@@ -477,8 +529,10 @@ template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
     const int held = (int)min((int64_t)min((int)p.block - sub * 64, 64), p.S - j0);
     const int i0 = t.item_base[bh * (p.nb + 1) + n], i1 = t.item_base[bh * (p.nb + 1) + n + 1];
-    for (int x = threadIdx.x; x < held * D / 4; x += 128) {
+    const int x = blockIdx.z * 128 + threadIdx.x;
+    if (x < held * D / 4) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
+#pragma unroll 4
         for (int i = i0; i < i1; ++i) {
             const float *src = t.kv_part + (((bhl * t.max_items + i) * t.nsub + sub) * 2) * 64 * D;
             const float4 u = *reinterpret_cast<const float4 *>(src + x * 4), w = *reinterpret_cast<const float4 *>(src + 64 * D + x * 4);
@@ -562,32 +616,32 @@ int prepare(const SelProblem &p, const Plan &w, void *ws, bool bwd, SelTile &t) 
     return launch_sel_lists(p, t.l, (int2 *)(at + w.items), (int32_t *)(at + w.base), t.max_items, bwd ? kBwdRows : kFwdRows);
 }
 
-template <typename T, int DP, int NKP> int fwd(const SelProblem &p, const Plan &w, SelTile t) {
+template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, const Plan &w, SelTile t) {
     const int64_t bh = p.B * p.Hkv;
     const size_t smem = ((p.block + NKP - 1) / NKP * NKP * 2 + 4 * 2 * 16) * (DP + 8) * sizeof(T);
-    if (int rc = ensure_dynamic_smem((const void *)sel_fwd_mma_kernel<T, DP, NKP>, smem, "shared memory of the selected attention")) return rc;
+    if (int rc = ensure_dynamic_smem((const void *)sel_fwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention")) return rc;
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
         const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
-        sel_fwd_mma_kernel<T, DP, NKP><<<dim3((unsigned)w.max_items, (unsigned)n), 128, smem, p.stream>>>(p, t);
+        sel_fwd_mma_kernel<T, DP, NKP, EXACT><<<dim3((unsigned)w.max_items, (unsigned)n), 128, smem, p.stream>>>(p, t);
         if (p.D <= 64) sel_join_kernel<T, 16, false><<<(unsigned)((rows * 16 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
         else sel_join_kernel<T, 32, false><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
     }
     return launched("launching the selected attention");
 }
 
-template <typename T, int DP, int NKP> int bwd(const SelProblem &p, const Plan &w, SelTile t) {
+template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, const Plan &w, SelTile t) {
     const int64_t bh = p.B * p.Hkv, all = p.B * p.S * p.H;
-    const size_t smem = ((2 * NKP + 2 * 64) * (DP + 8) + 2 * 64 * (NKP + 8)) * sizeof(T);
-    if (int rc = ensure_dynamic_smem((const void *)sel_bwd_mma_kernel<T, DP, NKP>, smem, "shared memory of the selected attention's backward")) return rc;
+    const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 2 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20;
+    if (int rc = ensure_dynamic_smem((const void *)sel_bwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention's backward")) return rc;
     float *delta = const_cast<float *>(t.delta);
     if (p.D <= 64) sel_delta_kernel<T, 8><<<(unsigned)((all * 8 + 127) / 128), 128, 0, p.stream>>>((const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
     else sel_delta_kernel<T, 16><<<(unsigned)((all * 16 + 127) / 128), 128, 0, p.stream>>>((const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
         const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
-        sel_bwd_mma_kernel<T, DP, NKP><<<dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), 128, smem, p.stream>>>(p, t);
+        sel_bwd_mma_kernel<T, DP, NKP, EXACT><<<dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), 128, smem, p.stream>>>(p, t);
         if (p.D <= 64) sel_join_kernel<T, 16, true><<<(unsigned)((rows * 16 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
         else sel_join_kernel<T, 32, true><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
-        sel_kv_join_kernel<T><<<dim3((unsigned)(p.nb * w.nsub), (unsigned)n), 128, 0, p.stream>>>(p, t);
+        sel_kv_join_kernel<T><<<dim3((unsigned)(p.nb * w.nsub), (unsigned)n, (unsigned)((64 * p.D / 4 + 127) / 128)), 128, 0, p.stream>>>(p, t);
     }
     return launched("launching the selected attention's backward");
 }
@@ -596,13 +650,18 @@ template <typename T> int run(const SelProblem &p, void *ws, bool back) {
     const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.block, p.topk, back);
     SelTile t{};
     if (int rc = prepare(p, w, ws, back, t)) return rc;
-    const bool narrow = p.block <= 32;
-    if (back) {
-        if (p.D <= 64) return narrow ? bwd<T, 64, 32>(p, w, t) : bwd<T, 64, 64>(p, w, t);
-        return narrow ? bwd<T, 128, 32>(p, w, t) : bwd<T, 128, 64>(p, w, t);
-    }
-    if (p.D <= 64) return narrow ? fwd<T, 64, 32>(p, w, t) : fwd<T, 64, 64>(p, w, t);
-    return narrow ? fwd<T, 128, 32>(p, w, t) : fwd<T, 128, 64>(p, w, t);
+    const int dp = p.D <= 64 ? 64 : 128, nkp = p.block <= 32 ? 32 : 64;
+    const bool exact = p.D == dp && p.block % nkp == 0;
+#define SEL_CASE(DP, NKP)                                                                        \
+    if (dp == DP && nkp == NKP)                                                                  \
+        return back ? (exact ? bwd<T, DP, NKP, true>(p, w, t) : bwd<T, DP, NKP, false>(p, w, t)) \
+                    : (exact ? fwd<T, DP, NKP, true>(p, w, t) : fwd<T, DP, NKP, false>(p, w, t))
+    SEL_CASE(64, 32);
+    SEL_CASE(64, 64);
+    SEL_CASE(128, 32);
+    SEL_CASE(128, 64);
+#undef SEL_CASE
+    return fail(MAT_ERR_UNSUPPORTED, "no kernel for this width");
 }
 
 }  // namespace
