@@ -11,6 +11,7 @@
 #include <cmath>
 
 #include "paged.cuh"
+#include "ptx.cuh"
 
 namespace mat {
 namespace {
@@ -28,6 +29,7 @@ struct DecodeArgs {
     int64_t n_sel;
     float scale_log2;
     int nsplit, min_chunk, tiles;   // tiles: groups of query heads per key head
+    int aligned;                    // the kernel reads 16 neighbouring positions at a time: first is a multiple of 16
     float2 *stats;                  // [B, H, nsplit] (maximum, sum)
     float *part;                    // [B, H, nsplit, D]
     int *status;
@@ -35,12 +37,12 @@ struct DecodeArgs {
 
 // The virtual tokens of one row.
 struct RowTokens {
-    int64_t len, first, dil;
+    int64_t len, first, lo, dil;   // positions below lo belong to the alignment, not to the row
     const int32_t *list;
     int64_t n;
     __device__ __forceinline__ RowTokens(const DecodeArgs &a, int64_t b, int64_t h) {
         len = a.lengths[b];
-        first = 0; dil = 1; list = nullptr;
+        first = lo = 0; dil = 1; list = nullptr;
         if (len <= 0) {
             n = 0;
         } else if (a.pages) {
@@ -52,7 +54,11 @@ struct RowTokens {
             dil = a.dilation;
             const int64_t back = (len - 1) / dil;
             n = (a.left < back ? a.left : back) + 1;
-            first = len - 1 - (n - 1) * dil;
+            first = lo = len - 1 - (n - 1) * dil;
+            if (a.aligned) {
+                first = lo / 16 * 16;
+                n += lo - first;
+            }
         }
     }
     // tokens per chunk; rows of up to c tokens are one chunk
@@ -211,24 +217,250 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     }
 }
 
+// ---- 16-bit types on the tensor cores ---------------------------------------------------------------------------------
+// One warp per 16 neighbouring tokens against up to 16 query heads of a key head: S = Q K^T and O += P V are m16n8k16
+// products whose rows are the heads, so a group of 1 to 16 heads costs the same and the kernel stays bound by memory
+// (at D = 128 a warp spends about 170 instructions on the 8 KB of 16 tokens; the SM's share of HBM brings 8 KB in 350
+// clocks, 1400 issue slots).  What it needs is bytes in flight: every warp has a ring of NS tiles of its own, filled by
+// cp.async NS - 1 tiles ahead and waited for without a CTA barrier.  A tile never crosses a page (pages of 16 tokens and
+// more), so its 16 rows share one table lookup; a warp looks up 32 tiles at a time.
+__device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) decode_mma_kernel(const DecodeArgs a) {
+    constexpr int PITCH = DP + 8, TILE = 16 * PITCH, CH = DP / 8;
+    const int64_t b = blockIdx.z, h = blockIdx.y / a.tiles, G = a.H / a.Hkv;
+    const int g0 = (blockIdx.y % a.tiles) * 16, heads = min(16, (int)G - g0);
+    const int D = (int)a.D;
+    const RowTokens row(a, b, h);
+    const int64_t chunk = row.chunk(a), t0 = blockIdx.x * chunk;
+    const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
+    if (t0 >= row.n && blockIdx.x > 0) return;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    extern __shared__ __align__(16) char smem[];
+    T *ring = (T *)smem + warp * NS * 2 * TILE;          // NS x (16 keys, 16 values)
+    const int tiles = t1 > t0 ? (int)((t1 - t0 + 15) / 16) : 0, mine = (tiles - warp + 3) / 4;   // tiles warp, warp + 4, ...
+
+    // queries: through this warp's ring into registers
+    uint32_t qf[DP / 16][4];
+    for (int c = lane; c < 16 * CH; c += 32) {
+        const int r = c / CH, col = c % CH * 8;
+        const bool in = r < heads && col < D;
+        const T *src = (const T *)a.q + b * a.q_stride + (h * G + g0 + (in ? r : 0)) * D + (in ? col : 0);
+        *reinterpret_cast<uint4 *>(ring + r * PITCH + col) = in ? __ldg(reinterpret_cast<const uint4 *>(src)) : make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+        ptx::ldmatrix_x4(qf[kk], ptx::smem_u32(ring + (lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+    __syncwarp();
+
+    // lane x of a batch of 32 tiles: physical page (-1: none) and first position of this warp's tile 32 * batch + x
+    int phys_of = -1, pos_of = 0;
+    auto look_up = [&](int batch) {
+        const int x = batch * 32 + lane;
+        phys_of = -1;
+        if (x < mine) {
+            const int64_t t = t0 + (int64_t)(warp + 4 * x) * 16;
+            const int64_t pos = row.position(a, t);     // -1: a list entry that counts for nothing
+            if (pos >= 0) {
+                phys_of = (int)physical_page(a.c, b, pos >> a.c.page_shift, a.status);
+                pos_of = (int)pos;
+            }
+        }
+    };
+    auto load = [&](int x) {                             // tile x into its place of the ring
+        const int phys = __shfl_sync(0xffffffffu, phys_of, x % 32), pos = __shfl_sync(0xffffffffu, pos_of, x % 32);
+        if (x < mine) {
+            T *dst = ring + x % NS * 2 * TILE;
+            const int64_t slot = pos & ((1 << a.c.page_shift) - 1);
+            const T *k = (const T *)a.c.k + (phys < 0 ? 0 : phys * a.c.k_page + slot * a.c.k_tok + h * a.c.k_head);
+            const T *v = (const T *)a.c.v + (phys < 0 ? 0 : phys * a.c.v_page + slot * a.c.v_tok + h * a.c.v_head);
+            const int lo = (int)(row.lo - pos), hi = phys < 0 ? 0 : (int)(row.len - pos < 16 ? row.len - pos : 16);
+#pragma unroll
+            for (int c = lane; c < 16 * CH; c += 32) {
+                const int r = c / CH, col = c % CH * 8;
+                // rows outside the sequence and columns past D arrive as zeros: a weight of zero would not silence what
+                // such a row holds
+                const bool in = r >= lo && r < hi && col < D;
+                cp_async16(dst + r * PITCH + col, in ? k + r * a.c.k_tok + col : (const T *)a.c.k, in);
+                cp_async16(dst + TILE + r * PITCH + col, in ? v + r * a.c.v_tok + col : (const T *)a.c.v, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    float o[DP / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    look_up(0);
+    int phys_now = phys_of, pos_now = pos_of;            // of the batch being computed; loads may be a batch ahead
+#pragma unroll
+    for (int x = 0; x < NS - 1; ++x) load(x);
+    for (int x = 0; x < mine; ++x) {
+        if (x % 32 == 0) { phys_now = phys_of; pos_now = pos_of; }
+        if ((x + NS - 1) % 32 == 0) look_up((x + NS - 1) / 32);
+        load(x + NS - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
+        __syncwarp();
+        const T *k = ring + x % NS * 2 * TILE, *v = k + TILE;
+        const int phys = __shfl_sync(0xffffffffu, phys_now, x % 32), pos = __shfl_sync(0xffffffffu, pos_now, x % 32);
+        if (phys >= 0) {
+            float s[2][4] = {};
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                uint32_t r[4];
+                ptx::ldmatrix_x4(r, ptx::smem_u32(k + (lane % 8 + (lane / 16) * 8) * PITCH + kk * 16 + (lane / 8 % 2) * 8));
+                ptx::Mma<T>::run(s[0], qf[kk], r[0], r[1]);
+                ptx::Mma<T>::run(s[1], qf[kk], r[2], r[3]);
+            }
+            const int lo = (int)(row.lo - pos), hi = (int)(row.len - pos < 16 ? row.len - pos : 16);
+            if (lo > 0 || hi < 16)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int col = c * 8 + (lane % 4) * 2 + y % 2;
+                        if (col < lo || col >= hi) s[c][y] = -INFINITY;
+                    }
+            float t0m = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+            float t1m = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+#pragma unroll
+            for (int y = 1; y < 4; y <<= 1) {
+                t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, y));
+                t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, y));
+            }
+            t0m = fmaxf(m0, t0m * a.scale_log2);
+            t1m = fmaxf(m1, t1m * a.scale_log2);
+            if (__any_sync(0xffffffffu, t0m != m0 || t1m != m1)) {       // a new maximum somewhere: rescale
+                const float e0 = ptx::ex2(m0 - (t0m == -INFINITY ? 0.f : t0m)), e1 = ptx::ex2(m1 - (t1m == -INFINITY ? 0.f : t1m));
+                m0 = t0m; m1 = t1m;
+                l0 *= e0; l1 *= e1;
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c) { o[c][0] *= e0; o[c][1] *= e0; o[c][2] *= e1; o[c][3] *= e1; }
+            }
+            const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+            // the weights are rounded to the cache's type for the tensor cores, one rounding of the kind the output has;
+            // their sum stays in fp32
+            uint32_t pf[4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float w = ptx::ex2(fmaf(s[c][0], a.scale_log2, -r0)), x1 = ptx::ex2(fmaf(s[c][1], a.scale_log2, -r0));
+                const float y = ptx::ex2(fmaf(s[c][2], a.scale_log2, -r1)), z = ptx::ex2(fmaf(s[c][3], a.scale_log2, -r1));
+                l0 += w + x1;
+                l1 += y + z;
+                pf[2 * c] = ptx::Mma<T>::pack(w, x1);
+                pf[2 * c + 1] = ptx::Mma<T>::pack(y, z);
+            }
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                uint32_t r[4];
+                ptx::ldmatrix_x4_trans(r, ptx::smem_u32(v + (lane % 16) * PITCH + c * 16 + (lane / 16) * 8));
+                ptx::Mma<T>::run(o[2 * c], pf, r[0], r[1]);
+                ptx::Mma<T>::run(o[2 * c + 1], pf, r[2], r[3]);
+            }
+        }
+        __syncwarp();                                    // the tile's place may be filled again
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int y = 1; y < 4; y <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, y);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, y);
+    }
+    __syncthreads();                                     // the rings become the warps' results
+    float *sm = (float *)smem;                           // [4][16][DP + 4], then [4][16] maxima and sums
+    float *ms = sm + 4 * 16 * (DP + 4), *ls = ms + 64;
+    const int gr = lane / 4;
+    if (lane % 4 == 0) {
+        ms[warp * 16 + gr] = m0; ms[warp * 16 + gr + 8] = m1;
+        ls[warp * 16 + gr] = l0; ls[warp * 16 + gr + 8] = l1;
+    }
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+        float *w = sm + (warp * 16 + gr) * (DP + 4) + c * 8 + (lane % 4) * 2;
+        *reinterpret_cast<float2 *>(w) = make_float2(o[c][0], o[c][1]);
+        *reinterpret_cast<float2 *>(w + 8 * (DP + 4)) = make_float2(o[c][2], o[c][3]);
+    }
+    __syncthreads();
+    const bool whole = chunk >= row.n;
+    const int vecs = D / 4;
+    for (int x = threadIdx.x; x < heads * vecs; x += 128) {
+        const int g = x / vecs, col = x % vecs * 4;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ms[i * 16 + g]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e = ptx::ex2(ms[i * 16 + g] - ref);
+            sum += ls[i * 16 + g] * e;
+            const float4 u = *reinterpret_cast<const float4 *>(sm + (i * 16 + g) * (DP + 4) + col);
+            y.x = fmaf(u.x, e, y.x); y.y = fmaf(u.y, e, y.y); y.z = fmaf(u.z, e, y.z); y.w = fmaf(u.w, e, y.w);
+        }
+        const int64_t head = b * a.H + h * G + g0 + g;
+        if (whole) {
+            const float f = sum == 0.f ? 0.f : 1.f / sum;
+            T z[4] = {Elem<T>::from_f(y.x * f), Elem<T>::from_f(y.y * f), Elem<T>::from_f(y.z * f), Elem<T>::from_f(y.w * f)};
+            *reinterpret_cast<uint2 *>((T *)a.o + head * D + col) = *reinterpret_cast<uint2 *>(z);
+        } else {
+            *reinterpret_cast<float4 *>(a.part + (head * a.nsplit + blockIdx.x) * D + col) = y;
+            if (col == 0) a.stats[head * a.nsplit + blockIdx.x] = make_float2(top, sum);
+        }
+    }
+}
+
 // ---- joining the chunks of a row -------------------------------------------------------------------------------------
-template <typename T> __global__ void __launch_bounds__(128) join_kernel(const DecodeArgs a) {
+// One CTA per (sequence, query head).  The chunks' weights first, then the sum: D / 4 lanes of four columns, the other
+// threads take every k-th chunk, and their sums are added in a fixed order.
+template <typename T> __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a) {
+    __shared__ float4 acc[256];
+    __shared__ float red[8], weight[256];
     const int64_t b = blockIdx.y, head = b * a.H + blockIdx.x, h = blockIdx.x / (a.H / a.Hkv);
+    const int tid = threadIdx.x, D = (int)a.D, vecs = D / 4, lanes = 256 / vecs, v = tid % vecs, k = tid / vecs;
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a);
     if (chunk >= row.n) return;                      // written by its only chunk
     const int n = (int)((row.n + chunk - 1) / chunk);
     const float2 *st = a.stats + head * a.nsplit;
+    const float *part = a.part + head * a.nsplit * D;
     float top = -INFINITY;
-    for (int i = 0; i < n; ++i) top = fmaxf(top, st[i].x);
+    for (int i = tid; i < n; i += 256) top = fmaxf(top, st[i].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (tid % 32 == 0) red[tid / 32] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (int i = 0; i < n; ++i) sum += st[i].y * exp2f(st[i].x - ref);
-    for (int d = threadIdx.x; d < a.D; d += 128) {
-        float x = 0.f;
-        for (int i = 0; i < n; ++i) x += a.part[(head * a.nsplit + i) * a.D + d] * exp2f(st[i].x - ref);
-        ((T *)a.o)[head * a.D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x / sum);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += 256) {
+        __syncthreads();
+        weight[tid] = i0 + tid < n ? exp2f(st[i0 + tid].x - ref) : 0.f;
+        __syncthreads();
+        const int m = min(256, n - i0);
+        for (int i = 0; i < m; ++i) sum += st[i0 + i].y * weight[i];
+        if (k < lanes)
+#pragma unroll 4
+            for (int i = k; i < m; i += lanes) {
+                const float4 y = *reinterpret_cast<const float4 *>(part + (int64_t)(i0 + i) * D + v * 4);
+                const float w = weight[i];
+                x.x = fmaf(y.x, w, x.x); x.y = fmaf(y.y, w, x.y); x.z = fmaf(y.z, w, x.z); x.w = fmaf(y.w, w, x.w);
+            }
     }
+    acc[tid] = x;
+    __syncthreads();
+    if (k > 0) return;
+    for (int i = 1; i < lanes; ++i) {
+        const float4 y = acc[i * vecs + v];
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    T *o = (T *)a.o + head * D + v * 4;
+    o[0] = Elem<T>::from_f(x.x * f); o[1] = Elem<T>::from_f(x.y * f); o[2] = Elem<T>::from_f(x.z * f); o[3] = Elem<T>::from_f(x.w * f);
 }
 
 template <typename T, int LPK, int NV, int GT> int launch_simt(const DecodeArgs &a, cudaStream_t s) {
@@ -248,16 +480,36 @@ template <typename T, int LPK, int NV> int launch_simt_heads(const DecodeArgs &a
     }
 }
 
-template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
+template <typename T, int DP, int NS> int launch_mma(const DecodeArgs &a, cudaStream_t s) {
+    const size_t ring = 4 * NS * 2 * 16 * (DP + 8) * sizeof(T), res = (4 * 16 * (DP + 4) + 128) * sizeof(float);
+    const size_t smem = ring > res ? ring : res;
+    if (int rc = ensure_dynamic_smem((const void *)decode_mma_kernel<T, DP, NS>, smem, "shared memory of the paged decode")) return rc;
+    dim3 grid((unsigned)a.nsplit, (unsigned)(a.Hkv * a.tiles), (unsigned)a.B);
+    decode_mma_kernel<T, DP, NS><<<grid, 128, smem, s>>>(a);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode");
+}
+
+template <typename T> int run_simt(DecodeArgs &a, cudaStream_t s) {
     const int64_t G = a.H / a.Hkv;
     const int gt = G >= 4 ? 4 : (G >= 2 ? 2 : 1);
     a.tiles = (int)((G + gt - 1) / gt);
     const int vecs = (int)(a.D * sizeof(T) / 16);
-    int rc = vecs <= 8 ? launch_simt_heads<T, 8, 1>(a, gt, s)
-           : vecs <= 16 ? launch_simt_heads<T, 16, 1>(a, gt, s)
-           : vecs <= 32 ? launch_simt_heads<T, 32, 1>(a, gt, s) : launch_simt_heads<T, 32, 2>(a, gt, s);
+    return vecs <= 8 ? launch_simt_heads<T, 8, 1>(a, gt, s)
+         : vecs <= 16 ? launch_simt_heads<T, 16, 1>(a, gt, s)
+         : vecs <= 32 ? launch_simt_heads<T, 32, 1>(a, gt, s) : launch_simt_heads<T, 32, 2>(a, gt, s);
+}
+
+template <typename T> int run_mma(DecodeArgs &a, cudaStream_t s) {
+    a.tiles = (int)((a.H / a.Hkv + 15) / 16);
+    return a.D <= 64 ? launch_mma<T, 64, 5>(a, s) : a.D <= 128 ? launch_mma<T, 128, 3>(a, s) : launch_mma<T, 256, 2>(a, s);
+}
+template <> int run_mma<float>(DecodeArgs &a, cudaStream_t s) { return run_simt<float>(a, s); }
+
+template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
+    const int rc = a.aligned ? run_mma<T>(a, s) : run_simt<T>(a, s);
     if (rc || a.nsplit == 1) return rc;
-    join_kernel<T><<<dim3((unsigned)a.H, (unsigned)a.B), 128, 0, s>>>(a);
+    join_kernel<T><<<dim3((unsigned)a.H, (unsigned)a.B), 256, 0, s>>>(a);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode's join");
 }
@@ -268,7 +520,7 @@ void plan(const mat_paged_cache *c, int64_t B, int64_t H, int64_t width, int64_t
           int &nsplit, int &min_chunk) {
     int64_t most = width * c->page_size;
     if (list) most = n_sel * c->page_size;
-    else if (left >= 0 && left + 1 < most) most = left + 1;
+    else if (left >= 0 && left + 16 < most) most = left + 16;   // up to 15 tokens before the window's first
     const int64_t rows = B * c->H_kv;
     min_chunk = rows >= 8 * kSms ? 1024 : rows >= 2 * kSms ? 512 : 128;
     int64_t cap = 16 * kSms / rows;
@@ -329,7 +581,9 @@ extern "C" int mat_paged_decode(const mat_paged_cache *cache, const void *q, int
     a.stats = (float2 *)workspace;
     a.part = (float *)((char *)workspace + align256((size_t)B * H * a.nsplit * sizeof(float2)));
     if (!(a.status = paged_status_word())) return fail(MAT_ERR_CUDA, "no device status word");
-    note_kernel("paged_decode");
+    // 16 neighbouring tokens at a time on the tensor cores: 16-bit types, pages of 16 tokens and more, no dilation
+    a.aligned = cache->dtype != MAT_F32 && cache->page_size >= 16 && (left < 0 || dilation == 1);
+    note_kernel(a.aligned ? "paged_decode_mma" : "paged_decode_simt");
     cudaStream_t s = (cudaStream_t)stream;
     switch (cache->dtype) {
         case MAT_F32: return launch_decode<float>(a, s);
