@@ -13,6 +13,7 @@
 #include <limits.h>
 
 #include "paged.cuh"
+#include "pdl.cuh"
 
 namespace mat {
 namespace {
@@ -27,24 +28,44 @@ __device__ __forceinline__ uint64_t key_of(double x) {
 }
 
 // ---- bounds of the blocks of whole sequences ------------------------------------------------------------------------
+// One CTA per block and 64 bytes x 8 of its columns: 32 vectors of columns, 8 threads each taking every 8th token, four
+// tokens in flight.
 template <typename T>
-__global__ void __launch_bounds__(128) block_bounds_kernel(const T *k, T *bounds, int64_t S, int64_t nb, int block, int64_t HD) {
+__global__ void __launch_bounds__(256) block_bounds_kernel(const T *k, T *bounds, int64_t S, int64_t nb, int block, int64_t HD) {
+    pdl_trigger();
     constexpr int W = Vec16<T>::N;
-    const int64_t n = blockIdx.x, b = blockIdx.y;
+    __shared__ float red[2][8][32 * W];
+    const int64_t n = blockIdx.x, b = blockIdx.z, c = ((int64_t)blockIdx.y * 32 + threadIdx.x % 32) * W;
+    const int part = threadIdx.x / 32;
     const int64_t s0 = n * block, s1 = s0 + block < S ? s0 + block : S;
-    for (int64_t c = (int64_t)threadIdx.x * W; c < HD; c += 128 * W) {
-        float lo[W], hi[W];
+    float lo[W], hi[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j) { lo[j] = INFINITY; hi[j] = -INFINITY; }
-        for (int64_t s = s0; s < s1; ++s) {
+    for (int j = 0; j < W; ++j) { lo[j] = INFINITY; hi[j] = -INFINITY; }
+    if (c < HD)
+#pragma unroll 4
+        for (int64_t s = s0 + part; s < s1; s += 8) {
             float x[W];
             Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(k + (b * S + s) * HD + c)), x);
 #pragma unroll
             for (int j = 0; j < W; ++j) { lo[j] = fminf(lo[j], x[j]); hi[j] = fmaxf(hi[j], x[j]); }
         }
-        T *out = bounds + (b * nb + n) * 2 * HD + c;
-        *reinterpret_cast<uint4 *>(out) = Vec16<T>::pack(lo);
-        *reinterpret_cast<uint4 *>(out + HD) = Vec16<T>::pack(hi);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        red[0][part][j * 32 + threadIdx.x % 32] = lo[j];
+        red[1][part][j * 32 + threadIdx.x % 32] = hi[j];
+    }
+    __syncthreads();
+    if (part < 2 && c < HD) {          // warp 0 joins the smallest, warp 1 the largest
+        float m[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            m[j] = red[part][0][j * 32 + threadIdx.x % 32];
+            for (int x = 1; x < 8; ++x) {
+                const float y = red[part][x][j * 32 + threadIdx.x % 32];
+                m[j] = part ? fmaxf(m[j], y) : fminf(m[j], y);
+            }
+        }
+        *reinterpret_cast<uint4 *>(bounds + ((b * nb + n) * 2 + part) * HD + c) = Vec16<T>::pack(m);
     }
 }
 
@@ -55,6 +76,8 @@ __global__ void __launch_bounds__(256) block_scores_kernel(const T *q, const T *
     const int64_t b = blockIdx.z / Hkv, h = blockIdx.z % Hkv, G = H / Hkv;
     const int64_t s0 = s_lo + (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
     const int64_t s_last = (s0 + 63 < s_hi ? s0 + 63 : s_hi - 1);
+    pdl_trigger();
+    pdl_wait();
     if (causal && n0 > s_last / block) return;
     __shared__ double up[16][65], down[16][65], hi[16][65], lo[16][65];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
@@ -97,44 +120,70 @@ __global__ void __launch_bounds__(256) block_scores_kernel(const T *q, const T *
     }
 }
 
-// ---- scores of a cache's pages: one warp per page --------------------------------------------------------------------
-template <typename T>
+// ---- scores of a cache's pages ---------------------------------------------------------------------------------------
+// LP lanes share a page: a lane holds the weights of its NV vectors (of the 2 D bounds: smallest keys, then largest) in
+// 64 bits in registers and reads four pages' vectors at once.
+template <typename T, int LP, int NV>
 __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
                                                           const int32_t *lengths, uint64_t *keys, int *status) {
-    constexpr int W = Vec16<T>::N;
+    constexpr int W = Vec16<T>::N, GROUPS = 256 / LP, U = NV >= 4 ? 2 : 4;
     const int64_t b = blockIdx.z, h = blockIdx.y, G = H / Hkv;
+    pdl_trigger();
     const int64_t len = lengths[b];
     if (len <= 0) return;
     const int64_t held = ((len - 1) >> c.page_shift) + 1;      // pages that hold tokens; the last is the token's own
     const int64_t n = held < c.width ? held : c.width;
-    if ((int64_t)blockIdx.x * 8 >= n) return;
-    __shared__ double up[256], down[256];
-    for (int d = threadIdx.x; d < D; d += 256) {
-        double u = 0, w = 0;
-        for (int64_t g = 0; g < G; ++g) {
-            const double y = (double)Elem<T>::to_f(q[b * q_stride + (h * G + g) * D + d]);
-            if (y > 0) u += y; else w += y;
-        }
-        up[d] = u; down[d] = w;
+    if ((int64_t)blockIdx.x * GROUPS >= n) return;
+    const int part = threadIdx.x % LP, vecs = (int)D / W;
+    double w[NV][W];
+    int64_t off[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = i * LP + part;
+        const bool high = v >= vecs;
+        const int col = (high ? v - vecs : v) * W;
+        off[i] = v < 2 * vecs ? (high ? Hkv * D : 0) + h * D + col : -1;
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[i][j] = 0;
+        if (off[i] >= 0)
+            for (int64_t g = 0; g < G; ++g) {
+                float x[W];
+                Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(q + b * q_stride + (h * G + g) * D + col)), x);
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if ((x[j] > 0) == high) w[i][j] += (double)x[j];       // a NaN lands among the smallest keys' weights
+            }
     }
-    __syncthreads();
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vecs = (int)D / W;
-    for (int64_t p = (int64_t)blockIdx.x * 8 + warp; p < n; p += (int64_t)gridDim.x * 8) {
-        const int64_t phys = physical_page(c, b, p, status);
-        double s = 0;
-        for (int v = lane; v < 2 * vecs; v += 32) {
-            if (phys < 0) break;
-            const bool high = v >= vecs;
-            const int col = (high ? v - vecs : v) * W;
-            float x[W];
-            Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(bounds + ((phys * 2 + high) * Hkv + h) * D + col)), x);
-            const double *w = high ? up : down;
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    // the trip count is the same for all lanes of a warp (they shuffle together): bounded by the CTA's first group
+    for (int64_t p0 = (int64_t)blockIdx.x * GROUPS; p0 < n; p0 += U * step) {
+        uint4 x[U][NV];
+        int64_t phys[U];
 #pragma unroll
-            for (int j = 0; j < W; ++j) s += w[col + j] * (double)x[j];
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = p0 + u * step + threadIdx.x / LP;
+            phys[u] = p < n ? physical_page(c, b, p, status) : -1;
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) keys[(b * Hkv + h) * c.width + p] = p == held - 1 ? kOwnKey : phys < 0 ? 0 : key_of(s);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                x[u][i] = phys[u] >= 0 && off[i] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(bounds + phys[u] * 2 * Hkv * D + off[i])) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            double s = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float y[W];
+                Vec16<T>::unpack(x[u][i], y);
+#pragma unroll
+                for (int j = 0; j < W; ++j) s += w[i][j] * (double)y[j];
+            }
+#pragma unroll
+            for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            const int64_t p = p0 + u * step + threadIdx.x / LP;
+            if (part == 0 && p < n) keys[(b * Hkv + h) * c.width + p] = p == held - 1 ? kOwnKey : phys[u] < 0 ? 0 : key_of(s);
+        }
     }
 }
 
@@ -168,6 +217,8 @@ struct RowsOfPages {
 template <int PER, typename Rows>
 __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, int32_t *out, int64_t rows, int topk, Rows of) {
     const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    pdl_trigger();
+    pdl_wait();
     if (r >= rows) return;
     const int lane = threadIdx.x % 32;
     const int n = (int)of.count(r), k = topk < n ? topk : n;
@@ -205,76 +256,77 @@ __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, in
     for (int i = done + lane; i < topk; i += 32) o[i] = -1;
 }
 
-// One CTA per row of any length, a byte of the key at a time.
-template <typename Rows>
-__global__ void __launch_bounds__(1024) topk_block_kernel(const uint64_t *keys, int32_t *out, int topk, Rows of) {
+// One CTA per row of any length: THREADS x PER keys in registers, the rest read again for every bit.
+template <int THREADS> __device__ __forceinline__ int block_sum(int x, int *of_warp) {
+    x = __reduce_add_sync(0xffffffffu, x);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = x;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, threadIdx.x % 32 < THREADS / 32 ? of_warp[threadIdx.x % 32] : 0);
+}
+
+template <int THREADS, int PER, typename Rows>
+__global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *keys, int32_t *out, int topk, Rows of) {
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    pdl_trigger();
+    pdl_wait();
     const int64_t n = of.count(r);
     const int k = topk < n ? topk : (int)n;
     const uint64_t *row = keys + r * of.stride();
     int32_t *o = out + of.out_row(r) * topk;
-    __shared__ int hist[256];
-    __shared__ int s_digit, s_left;
-    __shared__ int taken_of[32], tied_of[32];
+    __shared__ int of_warp[32], tied_of[32];
+    uint64_t key[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = j * THREADS + tid < n ? row[j * THREADS + tid] : 0;
+    auto count = [&](auto &&test) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) c += test(key[j]) && j * THREADS + tid < n;
+        for (int64_t i = (int64_t)PER * THREADS + tid; i < n; i += THREADS) c += test(row[i]);
+        return block_sum<THREADS>(c, of_warp);
+    };
     uint64_t cut = 0;
-    int left = k;            // how many of the keys that share the prefix so far are wanted
     if (k < n)
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int64_t i = tid; i < n; i += 1024) {
-                const uint64_t x = row[i];
-                if (shift == 56 || (x >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int c = 0, d = 255;
-                while (d > 0 && c + hist[d] < left) c += hist[d--];
-                s_digit = d;
-                s_left = left - c;
-            }
-            __syncthreads();
-            cut |= (uint64_t)s_digit << shift;
-            left = s_left;
-            __syncthreads();
+        for (int bit = 63; bit >= 0; --bit) {
+            const uint64_t want = cut | (1ull << bit);
+            const int c = count([&](uint64_t x) { return x >= want; });
+            if (c >= k) cut = want;
+            if (c == k) break;
         }
-    else
-        left = 0;
-    // `left` of the keys equal to cut are wanted (all keys when k == n: cut = 0 and nothing ties with an eligible one
-    // unless it is NaN, which the take below covers)
-    int done = 0, ties = k < n ? left : INT_MAX;
-    for (int64_t base = 0; base < n; base += 1024) {
+    int ties = k - count([&](uint64_t x) { return x > cut; }), done = 0;
+    for (int64_t base = 0; base < n; base += THREADS) {
         const int64_t i = base + tid;
         const uint64_t x = i < n ? row[i] : 0;
         const bool tie = i < n && x == cut;
+        // most stretches of a long row hold nothing that is taken
+        if (!__syncthreads_or(i < n && x >= cut)) continue;
         const uint32_t tied = __ballot_sync(0xffffffffu, tie), below = (1u << lane) - 1;
         if (lane == 0) tied_of[warp] = __popc(tied);
         __syncthreads();
         int before = 0, all = 0;
-        for (int w = 0; w < 32; ++w) { if (w < warp) before += tied_of[w]; all += tied_of[w]; }
+        for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) before += tied_of[w]; all += tied_of[w]; }
         const bool take = i < n && (x > cut || (tie && before + __popc(tied & below) < ties));
         const uint32_t taken = __ballot_sync(0xffffffffu, take);
-        if (lane == 0) taken_of[warp] = __popc(taken);
+        if (lane == 0) of_warp[warp] = __popc(taken);
         __syncthreads();
         int at = done, total = 0;
-        for (int w = 0; w < 32; ++w) { if (w < warp) at += taken_of[w]; total += taken_of[w]; }
+        for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) at += of_warp[w]; total += of_warp[w]; }
         if (take) o[at + __popc(taken & below)] = (int32_t)i;
         done += total;
         ties -= all < ties ? all : ties;
-        __syncthreads();
     }
-    for (int i = done + tid; i < topk; i += 1024) o[i] = -1;
+    for (int i = done + tid; i < topk; i += THREADS) o[i] = -1;
 }
 
 template <typename Rows>
 int launch_topk(const uint64_t *keys, int32_t *out, int64_t rows, int64_t most, int64_t topk, const Rows &of, cudaStream_t s) {
     const unsigned grid = (unsigned)((rows + 3) / 4);
-    if (most <= 128) topk_warp_kernel<4, Rows><<<grid, 128, 0, s>>>(keys, out, rows, (int)topk, of);
-    else if (most <= 512) topk_warp_kernel<16, Rows><<<grid, 128, 0, s>>>(keys, out, rows, (int)topk, of);
-    else if (most <= kWarpRow) topk_warp_kernel<32, Rows><<<grid, 128, 0, s>>>(keys, out, rows, (int)topk, of);
-    else topk_block_kernel<Rows><<<(unsigned)rows, 1024, 0, s>>>(keys, out, (int)topk, of);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e;
+    if (most <= 128) e = launch_after(topk_warp_kernel<4, Rows>, dim3(grid), dim3(128), 0, s, keys, out, rows, (int)topk, of);
+    else if (most <= 512) e = launch_after(topk_warp_kernel<16, Rows>, dim3(grid), dim3(128), 0, s, keys, out, rows, (int)topk, of);
+    else if (most <= kWarpRow) e = launch_after(topk_warp_kernel<32, Rows>, dim3(grid), dim3(128), 0, s, keys, out, rows, (int)topk, of);
+    else e = launch_after(topk_block_kernel<1024, 16, Rows>, dim3((unsigned)rows), dim3(1024), 0, s, keys, out, (int)topk, of);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the selection");
 }
 
@@ -305,15 +357,15 @@ int run_select_blocks(const T *q, const T *k, int64_t B, int64_t S, int64_t H, i
     const int64_t nb = (S + block - 1) / block, step = rows_at_a_time(B, S, Hkv, nb);
     T *bounds = (T *)ws;
     uint64_t *keys = (uint64_t *)((char *)ws + align256((size_t)B * nb * 2 * Hkv * D * sizeof(T)));
-    block_bounds_kernel<T><<<dim3((unsigned)nb, (unsigned)B), 128, 0, s>>>(k, bounds, S, nb, (int)block, Hkv * D);
+    block_bounds_kernel<T><<<dim3((unsigned)nb, (unsigned)((Hkv * D + 32 * Vec16<T>::N - 1) / (32 * Vec16<T>::N)), (unsigned)B), 256, 0, s>>>(k, bounds, S, nb, (int)block, Hkv * D);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "launching the block bounds");
     for (int64_t s0 = 0; s0 < S; s0 += step) {
         const int64_t s1 = s0 + step < S ? s0 + step : S;
         const int64_t seen = causal ? (s1 - 1) / block + 1 : nb;
         dim3 grid((unsigned)((seen + 63) / 64), (unsigned)((s1 - s0 + 63) / 64), (unsigned)(B * Hkv));
-        block_scores_kernel<T><<<grid, 256, 0, s>>>(q, bounds, keys, S, H, Hkv, D, nb, (int)block, causal, s0, s1);
-        if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "launching the block scores");
+        e = launch_after(block_scores_kernel<T>, grid, dim3(256), 0, s, q, (const T *)bounds, keys, S, H, Hkv, D, nb, (int)block, causal, s0, s1);
+        if (e != cudaSuccess) return cuda_fail(e, "launching the block scores");
         RowsOfBlocks of{B, S, Hkv, nb, s0, (int)block, causal};
         if (int rc = launch_topk(keys, blocks, (s1 - s0) * B * Hkv, seen, topk, of, s)) return rc;
     }
@@ -331,10 +383,19 @@ int check_paged_select(const mat_paged_cache *c, int64_t B, int64_t H, int64_t w
 template <typename T>
 int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, int64_t q_stride, int64_t B, int64_t H, const int32_t *lengths,
                      int64_t topk, int32_t *pages, uint64_t *keys, int *status, cudaStream_t s) {
-    int64_t gx = (v.width + 7) / 8;
-    const int64_t cap = 8 * 148 * 4 / (B * c->H_kv) + 1;     // enough CTAs to fill the GPU; each walks several pages
+    const int vecs = 2 * (int)c->D / Vec16<T>::N;            // of one page and head
+    const int lp = vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
+    int64_t gx = (v.width * lp + 4 * 256 - 1) / (4 * 256);
+    const int64_t cap = 148 * 8 / (B * c->H_kv) + 1;         // enough CTAs to fill the GPU; each walks several pages
     if (gx > cap) gx = cap;
-    page_scores_kernel<T><<<dim3((unsigned)gx, (unsigned)c->H_kv, (unsigned)B), 256, 0, s>>>(v, (const T *)c->key_bounds, q, q_stride, H, c->H_kv, c->D, lengths, keys, status);
+    const dim3 grid((unsigned)gx, (unsigned)c->H_kv, (unsigned)B);
+#define PAGE_SCORES(LP, NV) page_scores_kernel<T, LP, NV><<<grid, 256, 0, s>>>(v, (const T *)c->key_bounds, q, q_stride, H, c->H_kv, c->D, lengths, keys, status)
+    if (lp == 8) PAGE_SCORES(8, 1);
+    else if (lp == 16) PAGE_SCORES(16, 1);
+    else if (vecs <= 32) PAGE_SCORES(32, 1);
+    else if (vecs <= 64) PAGE_SCORES(32, 2);
+    else PAGE_SCORES(32, 4);
+#undef PAGE_SCORES
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "launching the page scores");
     RowsOfPages of{lengths, c->H_kv, v.width, v.page_shift};

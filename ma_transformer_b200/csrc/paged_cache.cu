@@ -12,6 +12,8 @@
 // back and written again ends with the same bits as one that never was.
 #include <limits.h>
 
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace mat {
@@ -19,8 +21,17 @@ namespace mat {
 __device__ int g_paged_status;
 
 int *paged_status_word() {
-    void *p = nullptr;
-    return cudaGetSymbolAddress(&p, g_paged_status) == cudaSuccess ? (int *)p : nullptr;
+    static std::atomic<int *> known[64];        // by device: looking the symbol up takes longer than the rest of a launch
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return nullptr;
+    int *p = dev < 64 ? known[dev].load(std::memory_order_acquire) : nullptr;
+    if (!p) {
+        void *at = nullptr;
+        if (cudaGetSymbolAddress(&at, g_paged_status) != cudaSuccess) return nullptr;
+        p = (int *)at;
+        if (dev < 64) known[dev].store(p, std::memory_order_release);
+    }
+    return p;
 }
 
 int paged_status_read_and_clear(int *out) {
@@ -90,11 +101,12 @@ __device__ __forceinline__ void angle_of(double pos, double freq, float &c, floa
     sincospif((float)r, &s, &c);
 }
 
-// Columns of one row in units of two 16-byte vectors (W pairs): unit u's vectors start at columns at0, at1, and its
-// pairs are (first vector, second vector) element by element, or neighbours when interleaved.  Pairs from npair on are
-// not rotated.
-template <typename T> struct Unit {
-    static constexpr int W = Vec16<T>::N;
+// Columns of one row in units of two vectors of four: unit u's vectors start at columns at0, at1, and its pairs are
+// (first vector, second vector) element by element, or neighbours when interleaved.  Four columns (8 bytes of a 16-bit
+// type) keep the kernel within 64 registers, four CTAs a SM: with 16-byte vectors it held two, and packed prompts of
+// 32768 tokens x (12 + 2 * 4) heads of 64 took 177 us instead of WIDE_US.
+constexpr int W = 4;
+struct Unit {
     int at0, at1, pair;   // pair: index of the unit's first rotated pair, -1 for none
     __device__ __forceinline__ Unit(int u, int rot, bool interleaved) {
         if (u * 2 * W < rot) {
@@ -109,31 +121,37 @@ template <typename T> struct Unit {
     }
 };
 
-template <typename T> __device__ __forceinline__ void load_unit(const T *row, const Unit<T> &u, bool two, float *x) {
-    Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(row + u.at0), x);
-    if (two) Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(row + u.at1), x + Unit<T>::W);
-}
+// four elements as fp32 values and back
+template <typename T> struct Four {
+    static __device__ __forceinline__ void load(const T *p, float *x) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        x[0] = Vec16<T>::one((uint16_t)(u.x & 0xffffu)); x[1] = Vec16<T>::one((uint16_t)(u.x >> 16));
+        x[2] = Vec16<T>::one((uint16_t)(u.y & 0xffffu)); x[3] = Vec16<T>::one((uint16_t)(u.y >> 16));
+    }
+    static __device__ __forceinline__ void store(T *p, const float *x) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(Vec16<T>::two(x[0], x[1]), Vec16<T>::two(x[2], x[3]));
+    }
+};
+template <> struct Four<float> {
+    static __device__ __forceinline__ void load(const float *p, float *x) { *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p); }
+    static __device__ __forceinline__ void store(float *p, const float *x) { *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(x); }
+};
 
-template <typename T> __device__ __forceinline__ void store_unit(T *row, const Unit<T> &u, bool two, const float *x) {
-    *reinterpret_cast<uint4 *>(row + u.at0) = Vec16<T>::pack(x);
-    if (two) *reinterpret_cast<uint4 *>(row + u.at1) = Vec16<T>::pack(x + Unit<T>::W);
-}
-
-// x: the 2 W values of a unit; cs: cosine and sine of its W pairs
-template <int W> __device__ __forceinline__ void turn(float *x, const float *c, const float *s, bool interleaved) {
+// x: the 2 N values of a unit; c, s: cosine and sine of its N pairs
+template <int N> __device__ __forceinline__ void turn(float *x, const float *c, const float *s, bool interleaved) {
     if (interleaved) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
+        for (int i = 0; i < N; ++i) {
             const float a = x[2 * i], b = x[2 * i + 1];
             x[2 * i] = a * c[i] - b * s[i];
             x[2 * i + 1] = b * c[i] + a * s[i];
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const float a = x[i], b = x[W + i];
+        for (int i = 0; i < N; ++i) {
+            const float a = x[i], b = x[N + i];
             x[i] = a * c[i] - b * s[i];
-            x[W + i] = b * c[i] + a * s[i];
+            x[N + i] = b * c[i] + a * s[i];
         }
     }
 }
@@ -152,10 +170,10 @@ template <typename T> __device__ __forceinline__ void pair_columns(int r, int ro
 // One page of one sequence: rows [n0, n0 + count) of the packed batch land in slots [slot0, slot0 + count).
 template <typename T, bool VEC>
 __device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int count, int64_t pos0, float *red) {
-    constexpr int W = VEC ? Vec16<T>::N : 1;
+    constexpr int N = VEC ? W : 1;
     const int h = blockIdx.y, G = a.q ? (int)(a.H / a.Hkv) : 0;
     const int D = (int)a.D;
-    const int units = (D + 2 * W - 1) / (2 * W);      // the last unit may hold one vector only (D = 8 mod 16 columns)
+    const int units = D / (2 * N);
     const int lanes = kThreads / units;               // rows in flight
     const int u = threadIdx.x % units, lane = threadIdx.x / units;
     const bool active = lane < lanes;
@@ -168,27 +186,24 @@ __device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int coun
     while (tl * 2 <= lanes && tl < count) tl *= 2;
     const int rl = lanes / tl, my_t = lane % tl, my_r = lane / tl;
 
-    float lo[2 * W], hi[2 * W];
+    float lo[2 * N], hi[2 * N];
 #pragma unroll
-    for (int i = 0; i < 2 * W; ++i) { lo[i] = INFINITY; hi[i] = -INFINITY; }
+    for (int i = 0; i < 2 * N; ++i) { lo[i] = INFINITY; hi[i] = -INFINITY; }
 
     int c0[2] = {0, 0};
-    Unit<T> un(VEC ? u : 0, a.rot, a.interleaved);
-    bool two = true, rotated;
-    if (VEC) {
-        rotated = un.pair >= 0;
-        two = rotated || un.at1 < D;
-    } else {
+    Unit un(VEC ? u : 0, a.rot, a.interleaved);
+    bool rotated = un.pair >= 0;
+    if (!VEC) {
         pair_columns<T>(u, a.rot, a.interleaved, c0[0], c0[1]);
         rotated = 2 * u < a.rot;
     }
     auto load = [&](const T *row, float *x) {
-        if (VEC) load_unit<T>(row, un, two, x);
-        else { x[0] = Elem<T>::to_f(row[c0[0]]); x[W] = Elem<T>::to_f(row[c0[1]]); }
+        if (VEC) { Four<T>::load(row + un.at0, x); Four<T>::load(row + un.at1, x + N); }
+        else { x[0] = Elem<T>::to_f(row[c0[0]]); x[N] = Elem<T>::to_f(row[c0[1]]); }
     };
     auto store = [&](T *row, const float *x) {
-        if (VEC) store_unit<T>(row, un, two, x);
-        else { row[c0[0]] = Elem<T>::from_f(x[0]); row[c0[1]] = Elem<T>::from_f(x[W]); }
+        if (VEC) { Four<T>::store(row + un.at0, x); Four<T>::store(row + un.at1, x + N); }
+        else { row[c0[0]] = Elem<T>::from_f(x[0]); row[c0[1]] = Elem<T>::from_f(x[N]); }
     };
     T *kp = (T *)a.c.k + (phys < 0 ? 0 : phys * a.c.k_page) + (int64_t)h * a.c.k_head;
     T *vp = (T *)a.c.v + (phys < 0 ? 0 : phys * a.c.v_page) + (int64_t)h * a.c.v_head;
@@ -196,14 +211,14 @@ __device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int coun
     if (active && my_r < rl) {
         for (int t = my_t; t < count; t += tl) {
             const int64_t n = n0 + t;
-            float cs[W], sn[W];
+            float cs[N], sn[N];
             if (rotated) {
                 const int pair = VEC ? un.pair : u;
 #pragma unroll
-                for (int i = 0; i < W; ++i) angle_of((double)(pos0 + t), a.inv_freq[pair + i], cs[i], sn[i]);
+                for (int i = 0; i < N; ++i) angle_of((double)(pos0 + t), a.inv_freq[pair + i], cs[i], sn[i]);
             }
             for (int role = my_r; role < G + 2; role += rl) {
-                float x[2 * W];
+                float x[2 * N];
                 if (role == 1) {          // value
                     if (phys >= 0) {
                         load((const T *)a.vn + n * a.vn_tok + (int64_t)h * D, x);
@@ -215,11 +230,11 @@ __device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int coun
                                          : (const T *)a.q + n * a.q_tok + ((int64_t)h * G + role - 2) * D;
                 if (role == 0 && phys < 0) continue;
                 load(src, x);
-                if (rotated) turn<W>(x, cs, sn, a.interleaved);
+                if (rotated) turn<N>(x, cs, sn, a.interleaved);
                 if (role == 0) {
                     store(kp + (int64_t)(slot0 + t) * a.c.k_tok, x);
 #pragma unroll
-                    for (int i = 0; i < 2 * W; ++i) {
+                    for (int i = 0; i < 2 * N; ++i) {
                         const float y = Elem<T>::to_f(Elem<T>::from_f(x[i]));   // the key as the cache holds it
                         lo[i] = fminf(lo[i], y);
                         hi[i] = fmaxf(hi[i], y);
@@ -231,10 +246,10 @@ __device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int coun
         }
         if (a.bounds && phys >= 0)
             for (int s = lane; s < slot0; s += lanes) {      // slots filled by earlier calls
-                float x[2 * W];
+                float x[2 * N];
                 load(kp + (int64_t)s * a.c.k_tok, x);
 #pragma unroll
-                for (int i = 0; i < 2 * W; ++i) {
+                for (int i = 0; i < 2 * N; ++i) {
                     lo[i] = fminf(lo[i], x[i]);
                     hi[i] = fmaxf(hi[i], x[i]);
                 }
@@ -243,35 +258,34 @@ __device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int coun
     if (!a.bounds) return;            // the same for the whole grid
     // join the lanes' bounds; red: [lo, hi][element of a unit][thread]
 #pragma unroll
-    for (int i = 0; i < 2 * W; ++i) {
+    for (int i = 0; i < 2 * N; ++i) {
         red[i * kThreads + threadIdx.x] = lo[i];
-        red[(2 * W + i) * kThreads + threadIdx.x] = hi[i];
+        red[(2 * N + i) * kThreads + threadIdx.x] = hi[i];
     }
     __syncthreads();
     if (phys < 0) return;
     const int used = min(lanes, max(tl, slot0));        // lanes that saw a key
     T *out = (T *)a.bounds + (phys * 2 * a.Hkv + h) * (int64_t)D;
-    for (int o = threadIdx.x; o < 4 * W * units; o += kThreads) {
-        const bool is_hi = o >= 2 * W * units;
-        const int r = is_hi ? o - 2 * W * units : o, i = r / units, v = r % units;
+    for (int o = threadIdx.x; o < 4 * N * units; o += kThreads) {
+        const bool is_hi = o >= 2 * N * units;
+        const int r = is_hi ? o - 2 * N * units : o, i = r / units, v = r % units;
         int col[2] = {0, 0};
         if (VEC) {
-            const Unit<T> w(v, a.rot, a.interleaved);
-            col[0] = w.at0 + i; col[1] = w.at1 + i - W;
+            const Unit w(v, a.rot, a.interleaved);
+            col[0] = w.at0 + i; col[1] = w.at1 + i - N;
         } else {
             pair_columns<T>(v, a.rot, a.interleaved, col[0], col[1]);
         }
-        const int c = i < W ? col[0] : col[1];
-        if (c >= D) continue;
-        const float *x = red + (is_hi ? 2 * W + i : i) * kThreads + v;
+        const int c = i < N ? col[0] : col[1];
+        const float *x = red + (is_hi ? 2 * N + i : i) * kThreads + v;
         float m = x[0];
         for (int l = 1; l < used; ++l) m = is_hi ? fmaxf(m, x[l * units]) : fminf(m, x[l * units]);
         out[(is_hi ? a.Hkv * (int64_t)D : 0) + c] = Elem<T>::from_f(m);
     }
 }
 
-template <typename T, bool VEC> __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
-    __shared__ float red[4 * (VEC ? Vec16<T>::N : 1) * kThreads];
+template <typename T, bool VEC> __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a) {
+    __shared__ float red[4 * (VEC ? W : 1) * kThreads];
     const int page = 1 << a.c.page_shift;
     auto first_row = [&](int64_t b) -> int64_t {
         if (!a.cu) return b;
@@ -292,10 +306,13 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(kThreads) appe
     }
     // pages that begin inside this tile of rows and are not a sequence's first
     const int64_t t0 = (int64_t)(blockIdx.x - a.B) * page, t1 = t0 + page;
-    int64_t lo = 0, hi = a.B - 1;                    // the last sequence that starts at or before t0
+    int64_t lo = 0, hi = a.B - 1;                    // the last sequence that starts at or before t0, 32 guesses at a time
     while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) >> 1;
-        if (first_row(mid) <= t0) lo = mid; else hi = mid - 1;
+        const int64_t step = (hi - lo + 32) / 32, at = lo + (threadIdx.x % 32) * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, at <= hi && first_row(at) <= t0);
+        if (!before) break;                          // only for malformed cu_seqlens
+        lo += (31 - __clz(before)) * step;
+        hi = hi < lo + step - 1 ? hi : lo + step - 1;
     }
     for (int64_t b = lo; b < a.B && first_row(b) < t1; ++b) {
         const int64_t n0 = first_row(b), end = first_row(b + 1), pos = a.start[b];
@@ -353,12 +370,12 @@ extern "C" int mat_paged_append(const mat_paged_cache *cache, const void *k_new,
     a.rot = inv_freq ? (int)rot : 0;
     a.interleaved = interleaved != 0;
     if (!(a.status = paged_status_word())) return fail(MAT_ERR_CUDA, "no device status word");
-    const bool v16 = a.rot % (2 * vec) == 0;   // both halves of a rotated pair start on 16 bytes
-    note_kernel(v16 ? "paged_append" : "paged_append_pairs");
+    const bool v4 = a.rot % (2 * W) == 0;   // both halves of a rotated pair start on a vector
+    note_kernel(v4 ? "paged_append" : "paged_append_pairs");
     cudaStream_t s = (cudaStream_t)stream;
     switch (cache->dtype) {
-        case MAT_F32: return launch_append<float>(a, v16, s);
-        case MAT_BF16: return launch_append<__nv_bfloat16>(a, v16, s);
-        default: return launch_append<__half>(a, v16, s);
+        case MAT_F32: return launch_append<float>(a, v4, s);
+        case MAT_BF16: return launch_append<__nv_bfloat16>(a, v4, s);
+        default: return launch_append<__half>(a, v4, s);
     }
 }

@@ -11,6 +11,7 @@
 #include <cmath>
 
 #include "paged.cuh"
+#include "pdl.cuh"
 #include "ptx.cuh"
 
 namespace mat {
@@ -84,6 +85,7 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     const int64_t b = blockIdx.z, h = blockIdx.y / a.tiles, g0 = (int64_t)(blockIdx.y % a.tiles) * GT;
     const int64_t G = a.H / a.Hkv;
     const int D = (int)a.D;
+    pdl_trigger();
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a), t0 = blockIdx.x * chunk;
     const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
@@ -233,6 +235,7 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
     const int64_t b = blockIdx.z, h = blockIdx.y / a.tiles, G = a.H / a.Hkv;
     const int g0 = (blockIdx.y % a.tiles) * 16, heads = min(16, (int)G - g0);
     const int D = (int)a.D;
+    pdl_trigger();
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a), t0 = blockIdx.x * chunk;
     const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
@@ -413,7 +416,7 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
 }
 
 // ---- joining the chunks of a row -------------------------------------------------------------------------------------
-// One CTA per (sequence, query head).  The chunks' weights first, then the sum: D / 4 lanes of four columns, the other
+// One CTA per (sequence, query head): the chunks' weights first, then the sum.  D / 4 lanes of four columns, the other
 // threads take every k-th chunk, and their sums are added in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a) {
     __shared__ float4 acc[256];
@@ -422,12 +425,14 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
     const int tid = threadIdx.x, D = (int)a.D, vecs = D / 4, lanes = 256 / vecs, v = tid % vecs, k = tid / vecs;
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a);
+    pdl_wait();
     if (chunk >= row.n) return;                      // written by its only chunk
     const int n = (int)((row.n + chunk - 1) / chunk);
     const float2 *st = a.stats + head * a.nsplit;
     const float *part = a.part + head * a.nsplit * D;
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += 256) top = fmaxf(top, st[i].x);
+    const float2 first = tid < n ? st[tid] : make_float2(-INFINITY, 0.f);
+    float top = first.x;
+    for (int i = tid + 256; i < n; i += 256) top = fmaxf(top, st[i].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (tid % 32 == 0) red[tid / 32] = top;
@@ -435,14 +440,16 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
     const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    float sum = 0.f;                                 // this thread's chunks; added up below
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = 0; i0 < n; i0 += 256) {
+        const float2 mine = i0 == 0 ? first : i0 + tid < n ? st[i0 + tid] : make_float2(-INFINITY, 0.f);
+        const float w0 = exp2f(mine.x - ref);
+        sum += mine.y * w0;
         __syncthreads();
-        weight[tid] = i0 + tid < n ? exp2f(st[i0 + tid].x - ref) : 0.f;
+        weight[tid] = w0;
         __syncthreads();
         const int m = min(256, n - i0);
-        for (int i = 0; i < m; ++i) sum += st[i0 + i].y * weight[i];
         if (k < lanes)
 #pragma unroll 4
             for (int i = k; i < m; i += lanes) {
@@ -451,9 +458,16 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
                 x.x = fmaf(y.x, w, x.x); x.y = fmaf(y.y, w, x.y); x.z = fmaf(y.z, w, x.z); x.w = fmaf(y.w, w, x.w);
             }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     acc[tid] = x;
     __syncthreads();
+    if (tid % 32 == 0) red[tid / 32] = sum;
+    __syncthreads();
     if (k > 0) return;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += red[i];
     for (int i = 1; i < lanes; ++i) {
         const float4 y = acc[i * vecs + v];
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
@@ -509,8 +523,7 @@ template <> int run_mma<float>(DecodeArgs &a, cudaStream_t s) { return run_simt<
 template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
     const int rc = a.aligned ? run_mma<T>(a, s) : run_simt<T>(a, s);
     if (rc || a.nsplit == 1) return rc;
-    join_kernel<T><<<dim3((unsigned)a.H, (unsigned)a.B), 256, 0, s>>>(a);
-    cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_after(join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B), dim3(256), 0, s, a);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode's join");
 }
 
@@ -522,7 +535,11 @@ void plan(const mat_paged_cache *c, int64_t B, int64_t H, int64_t width, int64_t
     if (list) most = n_sel * c->page_size;
     else if (left >= 0 && left + 16 < most) most = left + 16;   // up to 15 tokens before the window's first
     const int64_t rows = B * c->H_kv;
-    min_chunk = rows >= 8 * kSms ? 1024 : rows >= 2 * kSms ? 512 : 128;
+    // Every CTA pays some 4 us to look up its pages, fill its rings and write its result.  64 sequences of up to 8192
+    // tokens x 8 key heads of 128: 172 us with chunks of 512 tokens and more, 163 with 1024, 159 with 2048; 32 x 2048
+    // chosen tokens x 8: 78, 61, 53 us.  Few rows need the shorter chunks to fill the GPU: one sequence of 777 tokens x
+    // 8 heads has 7 x 8 CTAs with chunks of 128.
+    min_chunk = rows >= kSms ? 2048 : rows >= 16 ? 512 : 128;
     int64_t cap = 16 * kSms / rows;
     if (cap < 8) cap = 8;
     int64_t n = (most + min_chunk - 1) / min_chunk;

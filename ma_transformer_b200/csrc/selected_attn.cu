@@ -10,6 +10,7 @@
 #include <cmath>
 
 #include "paged.cuh"
+#include "pdl.cuh"
 #include "selected_attn.cuh"
 
 namespace mat {
@@ -30,7 +31,9 @@ template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const
     const int64_t tile = blockIdx.x, bh = blockIdx.z, b = bh / p.Hkv, h = bh % p.Hkv;
     const int n0 = blockIdx.y * kRange, n1 = min(n0 + kRange, (int)p.nb);
     const int tid = threadIdx.x;
+    pdl_trigger();
     for (int i = tid; i < (n1 - n0) * (kTile / 32); i += kTile) (&mask[0][0])[i] = 0;
+    pdl_wait();
     __syncthreads();
     const int64_t i = tile * kTile + tid;
     const int32_t *row = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
@@ -65,6 +68,8 @@ template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const
 // counts of a block's tiles -> offsets within its list, one warp per (bh, block)
 __global__ void __launch_bounds__(128) lists_offsets_kernel(SelLists l, int64_t rows) {
     const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    pdl_trigger();
+    pdl_wait();
     if (r >= rows) return;
     const int lane = threadIdx.x % 32;
     int32_t *c = l.counts + r * l.tiles;
@@ -103,6 +108,8 @@ __device__ __forceinline__ int block_scan(int x, int *of_warp) {
 __global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb, int G, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item) {
     __shared__ int of_warp[32], carry[2];
     const int64_t bh = blockIdx.x;
+    pdl_trigger();
+    pdl_wait();
     int entries = 0, before = 0;
     for (int64_t n0 = 0; n0 < nb; n0 += 1024) {
         const int64_t n = n0 + threadIdx.x;
@@ -319,9 +326,9 @@ int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_
     const dim3 grid((unsigned)l.tiles, (unsigned)((p.nb + kRange - 1) / kRange), bh);
     lists_kernel<false><<<grid, kTile, 0, p.stream>>>(p, l);
     const int64_t rows = (int64_t)bh * p.nb;
-    lists_offsets_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, p.stream>>>(l, rows);
-    lists_base_kernel<<<bh, 1024, 0, p.stream>>>(l, p.nb, (int)(p.H / p.Hkv), items, item_base, max_items, rows_per_item);
-    lists_kernel<true><<<grid, kTile, 0, p.stream>>>(p, l);
+    launch_after(lists_offsets_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, p.stream, l, rows);
+    launch_after(lists_base_kernel, dim3(bh), dim3(1024), 0, p.stream, l, p.nb, (int)(p.H / p.Hkv), items, item_base, max_items, rows_per_item);
+    launch_after(lists_kernel<true>, grid, dim3(kTile), 0, p.stream, p, l);
     return launched("launching the lists of a block selection");
 }
 

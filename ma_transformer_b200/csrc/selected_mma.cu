@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include "selected_attn.cuh"
+#include "pdl.cuh"
 #include "ptx.cuh"
 
 namespace mat {
@@ -60,6 +61,8 @@ __device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_str
 template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, DP == 64 ? 4 : 3) sel_fwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8;
     const int64_t bh = t.bh0 + blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
+    pdl_trigger();
+    pdl_wait();
     if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
     const int2 item = t.items[bh * t.max_items + blockIdx.x];
     const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n];
@@ -261,6 +264,8 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
 template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t, int64_t rows) {
     const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;     // (bh of the group, i, g)
     const int lane = threadIdx.x % LPR, col = lane * 4, D = (int)p.D, T_ = (int)p.topk;
+    pdl_trigger();
+    pdl_wait();
     const bool live = r < rows, in = live && col < D;
     const int64_t rr = live ? r : 0;
     const int g = (int)(rr % t.G);
@@ -334,6 +339,8 @@ template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) 
 template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, 2) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW, NBUF = DP == 64 ? 2 : 1;
     const int64_t bhl = blockIdx.z, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
+    pdl_trigger();
+    pdl_wait();
     if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
     const int2 item = t.items[bh * t.max_items + blockIdx.x];
     const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n], sub = blockIdx.y;
@@ -525,6 +532,8 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
 // dk and dv of a (sub-)block: the sum of its items' shares in order; zeros for a block that nobody chose
 template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(const SelProblem p, const SelTile t) {
     const int64_t bhl = blockIdx.y, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
+    pdl_trigger();
+    pdl_wait();
     const int n = blockIdx.x / t.nsub, sub = blockIdx.x % t.nsub, D = (int)p.D;
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
     const int held = (int)min((int64_t)min((int)p.block - sub * 64, 64), p.S - j0);
@@ -551,6 +560,8 @@ template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(
 template <typename T, int LPR> __global__ void __launch_bounds__(128) sel_delta_kernel(const T *o, const T *dout, float *delta, int64_t rows, int D) {
     const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;
     const int col = (threadIdx.x % LPR) * 8;
+    pdl_trigger();
+    pdl_wait();
     float s = 0.f;
     if (r < rows && col < D) {
         const uint4 a = __ldg(reinterpret_cast<const uint4 *>(o + r * D + col)), b = __ldg(reinterpret_cast<const uint4 *>(dout + r * D + col));
@@ -622,9 +633,9 @@ template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, 
     if (int rc = ensure_dynamic_smem((const void *)sel_fwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention")) return rc;
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
         const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
-        sel_fwd_mma_kernel<T, DP, NKP, EXACT><<<dim3((unsigned)w.max_items, (unsigned)n), 128, smem, p.stream>>>(p, t);
-        if (p.D <= 64) sel_join_kernel<T, 16, false><<<(unsigned)((rows * 16 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
-        else sel_join_kernel<T, 32, false><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
+        launch_after(sel_fwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)n), dim3(128), smem, p.stream, p, t);
+        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, false>, dim3((unsigned)((rows * 16 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
+        else launch_after(sel_join_kernel<T, 32, false>, dim3((unsigned)((rows * 32 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
     }
     return launched("launching the selected attention");
 }
@@ -634,14 +645,14 @@ template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, 
     const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 2 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20;
     if (int rc = ensure_dynamic_smem((const void *)sel_bwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention's backward")) return rc;
     float *delta = const_cast<float *>(t.delta);
-    if (p.D <= 64) sel_delta_kernel<T, 8><<<(unsigned)((all * 8 + 127) / 128), 128, 0, p.stream>>>((const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
-    else sel_delta_kernel<T, 16><<<(unsigned)((all * 16 + 127) / 128), 128, 0, p.stream>>>((const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
+    if (p.D <= 64) launch_after(sel_delta_kernel<T, 8>, dim3((unsigned)((all * 8 + 127) / 128)), dim3(128), 0, p.stream, (const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
+    else launch_after(sel_delta_kernel<T, 16>, dim3((unsigned)((all * 16 + 127) / 128)), dim3(128), 0, p.stream, (const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
         const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
-        sel_bwd_mma_kernel<T, DP, NKP, EXACT><<<dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), 128, smem, p.stream>>>(p, t);
-        if (p.D <= 64) sel_join_kernel<T, 16, true><<<(unsigned)((rows * 16 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
-        else sel_join_kernel<T, 32, true><<<(unsigned)((rows * 32 + 127) / 128), 128, 0, p.stream>>>(p, t, rows);
-        sel_kv_join_kernel<T><<<dim3((unsigned)(p.nb * w.nsub), (unsigned)n, (unsigned)((64 * p.D / 4 + 127) / 128)), 128, 0, p.stream>>>(p, t);
+        launch_after(sel_bwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), dim3(128), smem, p.stream, p, t);
+        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, true>, dim3((unsigned)((rows * 16 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
+        else launch_after(sel_join_kernel<T, 32, true>, dim3((unsigned)((rows * 32 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
+        launch_after(sel_kv_join_kernel<T>, dim3((unsigned)(p.nb * w.nsub), (unsigned)n, (unsigned)((64 * p.D / 4 + 127) / 128)), dim3(128), 0, p.stream, p, t);
     }
     return launched("launching the selected attention's backward");
 }

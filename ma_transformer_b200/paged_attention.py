@@ -12,13 +12,15 @@ cache is skipped (its tokens count as absent) and sets bit 1 of ``device_status(
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from contextlib import nullcontext
+from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _native as nat
 from .patterns import PatternSpec, WINDOW
 
+_HERE = nullcontext()
 _DTYPES = {torch.float32: nat.MAT_F32, torch.bfloat16: nat.MAT_BF16, torch.float16: nat.MAT_F16}
 
 
@@ -82,28 +84,44 @@ class PagedKVCache:
         nat.check(nat.lib.mat_paged_append(C.byref(s), None, None, 0, 0, 0, at, at, at, 1, 1, 1, None, None, 0, 0, None, 0, 0, None))
         self._struct, self._ref = s, C.byref(s)
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = (int(x) for x in k.shape)
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self._dev = k.dtype, k.device, k.get_device()
+        self._decode_bytes: Dict[tuple, int] = {}     # workspace sizes by the shapes they depend on
 
 
-def _index(t: torch.Tensor, name: str, cache: PagedKVCache, dim: int) -> None:
-    if t.dtype is not torch.int32 or t.dim() != dim or t.device != cache.device or t.stride(-1) != 1:
-        raise RuntimeError(f"{name} must be a {dim}-d int32 tensor on the cache's device with packed rows")
+# A decoding step is a few microseconds of GPU work, so the checks below go through the cheapest accessors there are:
+# get_device() instead of device objects, the raw stream handle instead of a Stream.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_lib_append, _lib_decode, _lib_select = nat.lib.mat_paged_append, nat.lib.mat_paged_decode, nat.lib.mat_paged_select
 
 
-def _table(table: torch.Tensor, cache: PagedKVCache) -> int:
-    _index(table, "page_table", cache, 2)
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+def _table(table: torch.Tensor, cache: PagedKVCache) -> Tuple[int, int, int]:
+    """(B, width, elements between rows) of a page table."""
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != cache._dev:
+        raise RuntimeError("page_table must be a 2-d int32 tensor on the cache's device")
+    B, width = table.shape
+    if table.is_contiguous():
+        return B, width, width
+    if table.stride(1) != 1:
+        raise RuntimeError("the rows of page_table must be packed")
+    return B, width, table.stride(0) if B > 1 else width
 
 
-def _rows(t: torch.Tensor, name: str, cache: PagedKVCache, n: int, heads: Optional[int]) -> int:
+def _per_sequence(t: torch.Tensor, name: str, cache: PagedKVCache, n: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != cache._dev or t.shape[0] != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a packed int32 tensor of {n} entries on the cache's device")
+
+
+def _rows(t: torch.Tensor, name: str, cache: PagedKVCache, n: int, heads: int) -> int:
     """Checks a [n, heads, head_dim] tensor with packed heads; elements between its rows."""
-    if t.dtype is not cache.dtype or t.device != cache.device:
+    if t.dtype is not cache.dtype or t.get_device() != cache._dev:
         raise RuntimeError(f"{name} must be of the cache's dtype and on its device")
-    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise RuntimeError(f"{name} must be [{n}, {heads if heads is not None else 'heads'}, {cache.head_dim}], got {list(t.shape)}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    if t.shape != (n, heads, cache.head_dim):
+        raise RuntimeError(f"{name} must be [{n}, {heads}, {cache.head_dim}], got {list(t.shape)}")
+    if t.is_contiguous():
+        return heads * cache.head_dim
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != cache.head_dim):
         raise RuntimeError(f"the heads and columns of {name} must be packed")
-    return t.stride(0) if n > 1 else t.shape[1] * t.shape[2]
+    return t.stride(0) if n > 1 else heads * cache.head_dim
 
 
 def _heads(query: torch.Tensor, cache: PagedKVCache) -> int:
@@ -115,24 +133,17 @@ def _heads(query: torch.Tensor, cache: PagedKVCache) -> int:
     return H
 
 
-class _Device:
-    """The cache's device as the current one, only where it is not already."""
-    __slots__ = ("_ctx",)
-
-    def __init__(self, device: torch.device):
-        self._ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+def _on_device(cache: PagedKVCache):
+    """A context that makes the cache's device the current one; nothing where it is already."""
+    return _HERE if torch.cuda.current_device() == cache._dev else torch.cuda.device(cache._dev)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _result(out: Optional[torch.Tensor], name: str, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype is not like.dtype or out.get_device() != like.get_device() or not out.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous tensor of query's shape, dtype and device")
+    return out
 
 
 def append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
@@ -154,20 +165,15 @@ def append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, page_tab
     N = key.shape[0] if key.dim() == 3 else -1
     k_ts = _rows(key, "key", cache, N, cache.n_kv_heads)
     v_ts = _rows(value, "value", cache, N, cache.n_kv_heads)
-    t_stride = _table(page_table, cache)
-    B, width = page_table.shape
-    _index(start, "start", cache, 1)
-    if start.shape[0] != B:
-        raise RuntimeError(f"start must name a position for each of the {B} rows of page_table")
+    B, width, t_stride = _table(page_table, cache)
+    _per_sequence(start, "start", cache, B)
     if cu_seqlens is not None:
-        _index(cu_seqlens, "cu_seqlens", cache, 1)
-        if cu_seqlens.shape[0] != B + 1:
-            raise RuntimeError(f"cu_seqlens must have {B + 1} entries")
+        _per_sequence(cu_seqlens, "cu_seqlens", cache, B + 1)
     elif N != B:
         raise RuntimeError(f"without cu_seqlens every sequence gets one token: got {N} for {B}")
     rot = 0
     if inv_freq is not None:
-        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or inv_freq.device != cache.device or not inv_freq.is_contiguous():
+        if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or inv_freq.get_device() != cache._dev or not inv_freq.is_contiguous():
             raise RuntimeError("inv_freq must be a contiguous 1-d float64 tensor on the cache's device")
         rot = 2 * inv_freq.shape[0]
         if rot == 0 or rot > cache.head_dim:
@@ -177,21 +183,17 @@ def append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, page_tab
     if query is not None:
         H = _heads(query, cache)
         q_ts = _rows(query, "query", cache, N, H)
-        if query_out is None:
-            query_out = torch.empty((N, H, cache.head_dim), dtype=query.dtype, device=query.device)
-        elif query_out.shape != query.shape or query_out.dtype != query.dtype or query_out.device != query.device \
-                or not query_out.is_contiguous():
-            raise RuntimeError("query_out must be a contiguous tensor of query's shape, dtype and device")
+        query_out = _result(query_out, "query_out", query)
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()
     elif query_out is not None:
         raise RuntimeError("query_out needs a query")
     if N == 0:
         return query_out
-    with _Device(cache.device):
-        rc = nat.lib.mat_paged_append(
+    with _on_device(cache):
+        rc = _lib_append(
             cache._ref, key.data_ptr(), value.data_ptr(), k_ts, v_ts, N, cu_seqlens.data_ptr() if cu_seqlens is not None else None,
             start.data_ptr(), page_table.data_ptr(), width, t_stride, B, q_ptr, out_ptr, H, q_ts,
-            inv_freq.data_ptr() if inv_freq is not None else None, rot, bool(interleaved), _stream(cache.device))
+            inv_freq.data_ptr() if inv_freq is not None else None, rot, bool(interleaved), _raw_stream(cache._dev))
     if rc:
         nat.check(rc)
     return query_out
@@ -208,12 +210,9 @@ def decode(query: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, l
     [B, n_kv_heads, n] int32 result of ``select_pages``.  With neither, every cached token is read.
     """
     H = _heads(query, cache)
-    t_stride = _table(page_table, cache)
-    B, width = page_table.shape
+    B, width, t_stride = _table(page_table, cache)
     q_stride = _rows(query, "query", cache, B, H)
-    _index(lengths, "lengths", cache, 1)
-    if lengths.shape[0] != B:
-        raise RuntimeError(f"lengths must have an entry for each of the {B} rows of page_table")
+    _per_sequence(lengths, "lengths", cache, B)
     left, dilation, n_sel, pages_ptr = -1, 1, 0, None
     if spec is not None:
         if spec.kind != WINDOW or spec.q_offset:
@@ -222,21 +221,21 @@ def decode(query: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, l
             raise RuntimeError("spec and pages cannot be combined")
         left, dilation = int(spec.left), int(spec.dilation)
     if pages is not None:
-        if pages.dtype is not torch.int32 or pages.device != cache.device or not pages.is_contiguous() or pages.dim() != 3 \
-                or pages.shape[0] != B or pages.shape[1] != cache.n_kv_heads or pages.shape[2] < 1:
+        if pages.dtype is not torch.int32 or pages.get_device() != cache._dev or not pages.is_contiguous() or pages.dim() != 3 \
+                or pages.shape[:2] != (B, cache.n_kv_heads) or pages.shape[2] < 1:
             raise RuntimeError(f"pages must be a contiguous int32 [{B}, {cache.n_kv_heads}, n] tensor on the cache's device")
         n_sel, pages_ptr = pages.shape[2], pages.data_ptr()
-    if out is None:
-        out = torch.empty((B, H, cache.head_dim), dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or not out.is_contiguous():
-        raise RuntimeError("out must be a contiguous tensor of query's shape, dtype and device")
-    with _Device(cache.device):
-        nbytes = nat.lib.mat_paged_decode_workspace_bytes(cache._ref, B, H, width, left, n_sel)
+    out = _result(out, "out", query)
+    nbytes = cache._decode_bytes.get((B, H, width, left, n_sel))
+    if nbytes is None:
+        nbytes = cache._decode_bytes[B, H, width, left, n_sel] = \
+            nat.lib.mat_paged_decode_workspace_bytes(cache._ref, B, H, width, left, n_sel)
+    with _on_device(cache):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
-        rc = nat.lib.mat_paged_decode(
+        rc = _lib_decode(
             cache._ref, query.data_ptr(), q_stride, out.data_ptr(), B, H, page_table.data_ptr(), width, t_stride,
             lengths.data_ptr(), left, dilation, pages_ptr, n_sel, float(scale) if scale else 0.0,
-            ws.data_ptr() if ws is not None else None, nbytes, _stream(cache.device))
+            ws.data_ptr() if ws is not None else None, nbytes, _raw_stream(cache._dev))
     if rc:
         nat.check(rc)
     return out
@@ -249,22 +248,19 @@ def select_pages(query: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     give (sum over query heads and columns of max(q * lo, q * hi)).  Scores are compared in 64 bits, equal ones go to
     the lower page."""
     H = _heads(query, cache)
-    t_stride = _table(page_table, cache)
-    B, width = page_table.shape
+    B, width, t_stride = _table(page_table, cache)
     q_stride = _rows(query, "query", cache, B, H)
-    _index(lengths, "lengths", cache, 1)
-    if lengths.shape[0] != B:
-        raise RuntimeError(f"lengths must have an entry for each of the {B} rows of page_table")
+    _per_sequence(lengths, "lengths", cache, B)
     topk = int(topk)
     if topk < 1:
         raise RuntimeError("topk must be >= 1")
     pages = torch.empty((B, cache.n_kv_heads, topk), dtype=torch.int32, device=cache.device)
-    with _Device(cache.device):
-        nbytes = nat.lib.mat_paged_select_workspace_bytes(cache._ref, B, H, width, topk)
+    nbytes = 8 * B * cache.n_kv_heads * width       # what mat_paged_select_workspace_bytes says
+    with _on_device(cache):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
-        rc = nat.lib.mat_paged_select(
+        rc = _lib_select(
             cache._ref, query.data_ptr(), q_stride, B, H, page_table.data_ptr(), width, t_stride, lengths.data_ptr(), topk,
-            pages.data_ptr(), ws.data_ptr(), nbytes, _stream(cache.device))
+            pages.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(cache._dev))
     if rc:
         nat.check(rc)
     return pages
