@@ -8,12 +8,17 @@
 // Bounds are exact in the keys' type, and scores are formed and compared in 64 bits, so a selection does not depend on
 // how the sums are split: two blocks change places only where their true scores agree to about 1e-15.
 //
-// A score becomes a 64-bit key whose order as an integer is the score's (NaN lowest, the query's own block highest); the
-// topk-th largest key is found bit by bit (byte by byte for long rows), ties go to the lower index.
+// 64-bit scores of everything would be the whole cost (conversions and 64-bit adds at an eighth of the fp32 rate), and
+// few of them matter.  So scores are first formed in fp32 with a bound eps on their error; what lies more than 2 eps
+// above or below the topk-th largest is decided by that, and the rest is scored again in 64 bits.  Where the two scores
+// at the border are nearer than 2 eps to many others (equal keys, say), all of those are scored again: slower, not
+// different.  A 64-bit score becomes a key whose order as an integer is the score's (NaN lowest, the query's own block
+// highest); ties go to the lower index.
 #include <limits.h>
 
 #include "paged.cuh"
 #include "pdl.cuh"
+#include "ptx.cuh"
 
 namespace mat {
 namespace {
@@ -25,6 +30,16 @@ __device__ __forceinline__ uint64_t key_of(double x) {
     if (x != x) return 0;
     const uint64_t u = (uint64_t)__double_as_longlong(x);
     return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+}
+
+// fp32 scores as integers of the same order (NaN lowest)
+__device__ __forceinline__ uint32_t key32_of(float x) {
+    if (x != x) return 0;
+    const uint32_t u = __float_as_uint(x);
+    return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_key32(uint32_t k) {
+    return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
 // ---- bounds of the blocks of whole sequences ------------------------------------------------------------------------
@@ -120,12 +135,115 @@ __global__ void __launch_bounds__(256) block_scores_kernel(const T *q, const T *
     }
 }
 
+// ---- the same for 16-bit types on the tensor cores, in fp32 ---------------------------------------------------------
+// With q+ = max(q, 0) and q- = min(q, 0) a score is [q+ q-] . [hi lo], products of 16-bit numbers that the tensor cores
+// form exactly; heads of a group follow each other in the same accumulator.  64 queries x 64 blocks per CTA, a warp per
+// 16 queries.  Leaves the score and, per row, the sum of its heads' norms (times a block's norm: a bound of the terms).
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) block_scores_mma_kernel(const T *q, const T *bounds, float *scores, float *norms, int64_t S, int64_t H, int64_t Hkv,
+                                                               int64_t D_, int64_t nb, int block, int causal, int64_t s_lo, int64_t s_hi) {
+    constexpr int PITCH = DP + 8;
+    __shared__ __align__(16) T hi[64 * PITCH], lo[64 * PITCH];
+    extern __shared__ __align__(16) char smem[];
+    T *qs = (T *)smem;
+    const int64_t b = blockIdx.z / Hkv, h = blockIdx.z % Hkv, G = H / Hkv;
+    const int64_t s0 = s_lo + (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+    const int64_t s_last = (s0 + 63 < s_hi ? s0 + 63 : s_hi - 1);
+    const int D = (int)D_, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    pdl_trigger();
+    pdl_wait();
+    if (causal && n0 > s_last / block) return;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < 64 * (DP / 8); i += 128) {
+        const int r = i / (DP / 8), c = i % (DP / 8) * 8;
+        const bool in = n0 + r < nb && c < D;
+        const T *src = bounds + ((b * nb + n0 + r) * 2 * Hkv + h) * D + c;
+        *reinterpret_cast<uint4 *>(lo + r * PITCH + c) = in ? __ldg(reinterpret_cast<const uint4 *>(src)) : zero;
+        *reinterpret_cast<uint4 *>(hi + r * PITCH + c) = in ? __ldg(reinterpret_cast<const uint4 *>(src + Hkv * D)) : zero;
+    }
+    float s[8][4] = {}, norm0 = 0.f, norm1 = 0.f;
+    for (int64_t g = 0; g < G; ++g) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * (DP / 8); i += 128) {
+            const int r = i / (DP / 8), c = i % (DP / 8) * 8;
+            const bool in = s0 + r < s_hi && c < D;
+            *reinterpret_cast<uint4 *>(qs + r * PITCH + c) = in ? __ldg(reinterpret_cast<const uint4 *>(q + ((b * S + s0 + r) * H + h * G + g) * D + c)) : zero;
+        }
+        __syncthreads();
+        float sq0 = 0.f, sq1 = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+            uint32_t a[4], up[4], down[4];
+            ptx::ldmatrix_x4(a, ptx::smem_u32(qs + (warp * 16 + lane % 16) * PITCH + kk * 16 + (lane / 16) * 8));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t neg = ((a[y] >> 15) & 0x00010001u) * 0xffffu;      // ones where the half is negative
+                up[y] = a[y] & ~neg;
+                down[y] = a[y] & neg;
+                const float x0 = ptx::Mma<T>::lo(a[y]), x1 = ptx::Mma<T>::hi(a[y]);
+                if (y % 2 == 0) sq0 += x0 * x0 + x1 * x1; else sq1 += x0 * x0 + x1 * x1;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t r[4];
+                const int at = (c * 16 + lane % 8 + (lane / 16) * 8) * PITCH + kk * 16 + (lane / 8 % 2) * 8;
+                ptx::ldmatrix_x4(r, ptx::smem_u32(hi + at));
+                ptx::Mma<T>::run(s[2 * c], up, r[0], r[1]);
+                ptx::Mma<T>::run(s[2 * c + 1], up, r[2], r[3]);
+                ptx::ldmatrix_x4(r, ptx::smem_u32(lo + at));
+                ptx::Mma<T>::run(s[2 * c], down, r[0], r[1]);
+                ptx::Mma<T>::run(s[2 * c + 1], down, r[2], r[3]);
+            }
+        }
+#pragma unroll
+        for (int y = 1; y < 4; y <<= 1) {
+            sq0 += __shfl_xor_sync(0xffffffffu, sq0, y);
+            sq1 += __shfl_xor_sync(0xffffffffu, sq1, y);
+        }
+        norm0 += sqrtf(sq0);
+        norm1 += sqrtf(sq1);
+    }
+    const int64_t r0 = s0 + warp * 16 + lane / 4, r1 = r0 + 8;
+    const int64_t row0 = (r0 - s_lo) * gridDim.z + blockIdx.z, row1 = (r1 - s_lo) * gridDim.z + blockIdx.z;
+    if (blockIdx.x == 0 && lane % 4 == 0) {
+        if (r0 < s_hi) norms[row0] = norm0;
+        if (r1 < s_hi) norms[row1] = norm1;
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const int64_t n = n0 + c * 8 + (lane % 4) * 2 + y;
+            if (n >= nb) continue;
+            if (r0 < s_hi) scores[row0 * nb + n] = s[c][y];
+            if (r1 < s_hi) scores[row1 * nb + n] = s[c][2 + y];
+        }
+}
+
+// Euclidean norm of max(|lo|, |hi|) of every block and head, one warp each
+template <typename T>
+__global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float *norms, int64_t rows, int64_t Hkv, int64_t D) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;      // (b * nb + n) * Hkv + h
+    pdl_trigger();
+    pdl_wait();
+    if (r >= rows) return;
+    const T *lo = bounds + (r / Hkv * 2 * Hkv + r % Hkv) * D, *hi = lo + Hkv * D;
+    float s = 0.f;
+    for (int d = threadIdx.x % 32; d < D; d += 32) {
+        const float x = fabsf(Elem<T>::to_f(lo[d])), y = fabsf(Elem<T>::to_f(hi[d]));
+        s += x > y || x != x ? x * x : y * y;          // a NaN must show
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x % 32 == 0) norms[r] = sqrtf(s);
+}
+
 // ---- scores of a cache's pages ---------------------------------------------------------------------------------------
 // LP lanes share a page: a lane holds the weights of its NV vectors (of the 2 D bounds: smallest keys, then largest) in
-// 64 bits in registers and reads four pages' vectors at once.
+// registers and reads four pages' vectors at once.  Leaves (score, sum of the terms' absolute values) in fp32.
 template <typename T, int LP, int NV>
 __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
-                                                          const int32_t *lengths, uint64_t *keys, int *status) {
+                                                          const int32_t *lengths, float2 *scores, int *status) {
     constexpr int W = Vec16<T>::N, GROUPS = 256 / LP, U = NV >= 4 ? 2 : 4;
     const int64_t b = blockIdx.z, h = blockIdx.y, G = H / Hkv;
     pdl_trigger();
@@ -135,23 +253,23 @@ __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *
     const int64_t n = held < c.width ? held : c.width;
     if ((int64_t)blockIdx.x * GROUPS >= n) return;
     const int part = threadIdx.x % LP, vecs = (int)D / W;
-    double w[NV][W];
-    int64_t off[NV];
+    float w[NV][W];
+    int off[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int v = i * LP + part;
         const bool high = v >= vecs;
         const int col = (high ? v - vecs : v) * W;
-        off[i] = v < 2 * vecs ? (high ? Hkv * D : 0) + h * D + col : -1;
+        off[i] = v < 2 * vecs ? (int)((high ? Hkv * D : 0) + h * D + col) : -1;
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[i][j] = 0;
+        for (int j = 0; j < W; ++j) w[i][j] = 0.f;
         if (off[i] >= 0)
             for (int64_t g = 0; g < G; ++g) {
                 float x[W];
                 Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(q + b * q_stride + (h * G + g) * D + col)), x);
 #pragma unroll
                 for (int j = 0; j < W; ++j)
-                    if ((x[j] > 0) == high) w[i][j] += (double)x[j];       // a NaN lands among the smallest keys' weights
+                    if ((x[j] > 0) == high) w[i][j] += x[j];       // a NaN lands among the smallest keys' weights
             }
     }
     const int64_t step = (int64_t)gridDim.x * GROUPS;
@@ -171,18 +289,25 @@ __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *
                 x[u][i] = phys[u] >= 0 && off[i] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(bounds + phys[u] * 2 * Hkv * D + off[i])) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            double s = 0;
+            float s = 0.f, size = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float y[W];
                 Vec16<T>::unpack(x[u][i], y);
 #pragma unroll
-                for (int j = 0; j < W; ++j) s += w[i][j] * (double)y[j];
+                for (int j = 0; j < W; ++j) {
+                    s = fmaf(w[i][j], y[j], s);
+                    size = fmaf(fabsf(w[i][j]), fabsf(y[j]), size);
+                }
             }
 #pragma unroll
-            for (int o = LP / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            for (int o = LP / 2; o > 0; o >>= 1) {
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+                size += __shfl_xor_sync(0xffffffffu, size, o);
+            }
             const int64_t p = p0 + u * step + threadIdx.x / LP;
-            if (part == 0 && p < n) keys[(b * Hkv + h) * c.width + p] = p == held - 1 ? kOwnKey : phys[u] < 0 ? 0 : key_of(s);
+            // a page outside the cache is no number: it sends its row to the 64-bit scores, where it ranks last
+            if (part == 0 && p < n) scores[(b * Hkv + h) * c.width + p] = make_float2(phys[u] < 0 ? -INFINITY : s, size);
         }
     }
 }
@@ -199,33 +324,9 @@ struct RowsOfBlocks {
         return (b * S + s) * Hkv + h;
     }
 };
-// Rows of a cache: row r = (b, h).
-struct RowsOfPages {
-    const int32_t *lengths;
-    int64_t Hkv, width;
-    int page_shift;
-    __device__ __forceinline__ int64_t count(int64_t r) const {
-        const int64_t len = lengths[r / Hkv];
-        const int64_t n = len <= 0 ? 0 : ((len - 1) >> page_shift) + 1;
-        return n < width ? n : width;
-    }
-    __device__ __forceinline__ int64_t stride() const { return width; }
-    __device__ __forceinline__ int64_t out_row(int64_t r) const { return r; }
-};
-
-// One warp per row, its keys in registers.
-template <int PER, typename Rows>
-__global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, int32_t *out, int64_t rows, int topk, Rows of) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-    pdl_trigger();
-    pdl_wait();
-    if (r >= rows) return;
+// The k largest of a row's n keys, held by one warp: key[j] of lane l is number 32 j + l (0 past n).
+template <int PER> __device__ __forceinline__ void topk_of_warp(const uint64_t (&key)[PER], int n, int k, int topk, int32_t *o) {
     const int lane = threadIdx.x % 32;
-    const int n = (int)of.count(r), k = topk < n ? topk : n;
-    const uint64_t *row = keys + r * of.stride();
-    uint64_t key[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < n ? row[j * 32 + lane] : 0;
     uint64_t cut = 0;
     if (k < n) {
         for (int bit = 63; bit >= 0; --bit) {
@@ -242,7 +343,6 @@ __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, in
 #pragma unroll
     for (int j = 0; j < PER; ++j) above += key[j] > cut && j * 32 + lane < n;
     int ties = k - __reduce_add_sync(0xffffffffu, above), done = 0;
-    int32_t *o = out + of.out_row(r) * topk;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const bool in = j * 32 + lane < n, tie = in && key[j] == cut;
@@ -256,6 +356,135 @@ __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, in
     for (int i = done + lane; i < topk; i += 32) o[i] = -1;
 }
 
+template <int PER, typename Rows>
+__global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, int32_t *out, int64_t rows, int topk, Rows of) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    pdl_trigger();
+    pdl_wait();
+    if (r >= rows) return;
+    const int lane = threadIdx.x % 32;
+    const int n = (int)of.count(r), k = topk < n ? topk : n;
+    const uint64_t *row = keys + r * of.stride();
+    uint64_t key[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < n ? row[j * 32 + lane] : 0;
+    topk_of_warp<PER>(key, n, k, topk, out + of.out_row(r) * topk);
+}
+
+// One warp per row over fp32 scores: the topk-th largest by halving the interval of the scores' integers (about ten
+// counts: any value between the topk-th and the next will do), the border again in 64 bits where it is too close.
+// 65536 rows of up to 128 blocks: TOPKW_US us; 64 steps over 64-bit keys took 65.
+template <int PER, typename T>
+__global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *bounds, const float *scores, const float *q_norms, const float *block_norms,
+                                                          int32_t *out, int64_t rows, int topk, int64_t H, int64_t D, RowsOfBlocks of) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    pdl_trigger();
+    pdl_wait();
+    if (r >= rows) return;
+    const int lane = threadIdx.x % 32;
+    const int64_t s = of.s_lo + r / (of.B * of.Hkv), b = r / of.Hkv % of.B, h = r % of.Hkv, G = H / of.Hkv;
+    const int n = (int)of.count(r), k = topk < n ? topk : n, own = (int)(s / of.block);
+    const float *row = scores + r * of.nb;
+    uint32_t key[PER];
+    float size = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = j * 32 + lane;
+        key[j] = 0;
+        if (i < n) {
+            const float x = row[i], y = block_norms[(b * of.nb + i) * of.Hkv + h];
+            key[j] = i == own ? 0xffffffffu : key32_of(x);
+            size = fmaxf(size, y);
+            odd |= !(fabsf(x) < INFINITY && y < INFINITY);
+        }
+    }
+    int32_t *o = out + of.out_row(r) * topk;
+    uint32_t cut = 0;                       // taken: key >= cut
+    bool close = false;
+    if (k < n) {
+        if (k == 1) {
+            cut = 0xffffffffu;
+        } else {
+            uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (j * 32 + lane < n && key[j] != 0xffffffffu) { lo = min(lo, key[j]); hi = max(hi, key[j]); }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi) + 1;
+            bool met = false;               // count(key >= lo) == k, else it is more and count(key >= hi) is less
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                int c = 0;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) c += key[j] >= mid;
+                c = __reduce_add_sync(0xffffffffu, c);
+                if (c >= k) lo = mid; else hi = mid;
+                met = c == k;
+                if (met) break;
+            }
+            cut = lo;
+            size = fmaxf(size, 0.f);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, x));
+            odd = __any_sync(0xffffffffu, odd);
+            // A product step adds 16 products to the accumulator; aligned to the largest and cut at 24 bits, each of the
+            // 17 terms may lose 2^-23 of the largest: 2.1e-6 of the terms' size per step.
+            const float eps = (float)(2 * G * ((D + 15) / 16) + 1) * 2.1e-6f * q_norms[r] * size + 1e-42f;
+            // the least that is taken and the most that is not
+            uint32_t in = 0xffffffffu, not_in = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (j * 32 + lane < n) { if (key[j] >= cut) in = min(in, key[j]); else not_in = max(not_in, key[j]); }
+            in = __reduce_min_sync(0xffffffffu, in);
+            not_in = __reduce_max_sync(0xffffffffu, not_in);
+            odd |= !(eps < INFINITY);
+            const float kth = of_key32(in);
+            close = odd || !met || !(kth - of_key32(not_in) > 2.f * eps);
+            if (close) {
+                // 64-bit keys: certain ones highest, hopeless ones lowest, the border by its scores
+                uint64_t exact[PER];
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int i = j * 32 + lane;
+                    const float x = of_key32(key[j]);
+                    const bool sure = i == own || (!odd && x > kth + 2.f * eps);
+                    exact[j] = i < n && sure ? kOwnKey : 0;
+                    uint32_t border = __ballot_sync(0xffffffffu, i < n && !sure && (odd || x >= kth - 2.f * eps));
+                    while (border) {
+                        const int who = __ffs(border) - 1;
+                        border &= border - 1;
+                        const T *low = bounds + ((b * of.nb + j * 32 + who) * 2 * of.Hkv + h) * D, *high = low + of.Hkv * D;
+                        double t = 0;
+                        for (int d = lane; d < D; d += 32) {
+                            double u = 0, w = 0;
+                            for (int64_t g = 0; g < G; ++g) {
+                                const double y = (double)Elem<T>::to_f(q[((b * of.S + s) * H + h * G + g) * D + d]);
+                                if (y > 0) u += y; else w += y;
+                            }
+                            t += u * (double)Elem<T>::to_f(high[d]) + w * (double)Elem<T>::to_f(low[d]);
+                        }
+#pragma unroll
+                        for (int x2 = 16; x2 > 0; x2 >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x2);
+                        if (lane == who) exact[j] = key_of(t);
+                    }
+                }
+                topk_of_warp<PER>(exact, n, k, topk, o);
+                return;
+            }
+        }
+    }
+    int done = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const bool take = j * 32 + lane < n && key[j] >= cut;
+        const uint32_t taken = __ballot_sync(0xffffffffu, take);
+        if (take) o[done + __popc(taken & ((1u << lane) - 1))] = j * 32 + lane;
+        done += __popc(taken);
+    }
+    for (int i = done + lane; i < topk; i += 32) o[i] = -1;
+}
+
 // One CTA per row of any length: THREADS x PER keys in registers, the rest read again for every bit.
 template <int THREADS> __device__ __forceinline__ int block_sum(int x, int *of_warp) {
     x = __reduce_add_sync(0xffffffffu, x);
@@ -265,17 +494,11 @@ template <int THREADS> __device__ __forceinline__ int block_sum(int x, int *of_w
     return __reduce_add_sync(0xffffffffu, threadIdx.x % 32 < THREADS / 32 ? of_warp[threadIdx.x % 32] : 0);
 }
 
-template <int THREADS, int PER, typename Rows>
-__global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *keys, int32_t *out, int topk, Rows of) {
-    const int64_t r = blockIdx.x;
+// The k largest of n keys, k < n or not, by a whole CTA.
+template <int THREADS> __device__ void topk_of_row(const uint64_t *row, int64_t n, int topk, int32_t *o, int *of_warp, int *tied_of) {
+    constexpr int PER = 16;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    pdl_trigger();
-    pdl_wait();
-    const int64_t n = of.count(r);
     const int k = topk < n ? topk : (int)n;
-    const uint64_t *row = keys + r * of.stride();
-    int32_t *o = out + of.out_row(r) * topk;
-    __shared__ int of_warp[32], tied_of[32];
     uint64_t key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) key[j] = j * THREADS + tid < n ? row[j * THREADS + tid] : 0;
@@ -319,6 +542,164 @@ __global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *key
     for (int i = done + tid; i < topk; i += THREADS) o[i] = -1;
 }
 
+template <int THREADS, typename Rows>
+__global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *keys, int32_t *out, int topk, Rows of) {
+    __shared__ int of_warp[32], tied_of[32];
+    const int64_t r = blockIdx.x;
+    pdl_trigger();
+    pdl_wait();
+    topk_of_row<THREADS>(keys + r * of.stride(), of.count(r), topk, out + of.out_row(r) * topk, of_warp, tied_of);
+}
+
+// ---- the topk pages of a row: one CTA -------------------------------------------------------------------------------
+// 1. Every thread takes the largest fp32 score of its share of the pages; the (topk - 1)-th largest of those maxima is
+//    a floor under the (topk - 1)-th largest score (the token's own page is taken anyway), so no page more than 2 eps
+//    below it can be chosen.  With 256 or 1024 threads and few pages wanted, little more than topk pages remain.
+// 2. The remaining pages, up to kCandidates, are scored again in 64 bits, one warp each.
+// 3. Each candidate counts the candidates that beat it; the winners count the winners before them: their place.
+// Rows where more remain (many equal pages; topk above the number of threads) are scored in 64 bits throughout, by the
+// same warps, and searched bit by bit.
+constexpr int kCandidates = 1024;
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
+                                                               const int32_t *lengths, float2 *scores, int32_t *out, int topk, int *status) {
+    constexpr int W = Vec16<T>::N;
+    const int64_t b = blockIdx.y, h = blockIdx.x, G = H / Hkv, row = b * Hkv + h;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, vecs = (int)D / W;
+    __shared__ double up[256], down[256];
+    __shared__ uint64_t key[kCandidates];
+    __shared__ int page_of[kCandidates];
+    __shared__ int of_warp[32], tied_of[32], s_count;
+    __shared__ float f_warp[32];
+    pdl_trigger();
+    pdl_wait();
+    const int64_t len = lengths[b];
+    const int64_t held = len <= 0 ? 0 : ((len - 1) >> c.page_shift) + 1;
+    const int n = (int)(held < c.width ? held : c.width);
+    int32_t *o = out + row * topk;
+    if (n <= topk) {
+        for (int i = tid; i < topk; i += THREADS) o[i] = i < n ? i : -1;
+        return;
+    }
+    // the token's own page is in (where the table reaches it); `want` of the `others` before it
+    const int others = held <= c.width ? n - 1 : n, want = topk - (n - others);
+    for (int d = tid; d < D; d += THREADS) {
+        double u = 0, w = 0;
+        for (int64_t g = 0; g < G; ++g) {
+            const double y = (double)Elem<T>::to_f(q[b * q_stride + (h * G + g) * D + d]);
+            if (y > 0) u += y; else w += y;
+        }
+        up[d] = u; down[d] = w;
+    }
+    const float2 *mine = scores + row * c.width;
+    float best = -INFINITY, size = 0.f;
+    bool odd = false;
+    for (int i = tid; i < others; i += THREADS) {
+        const float2 x = mine[i];
+        best = fmaxf(best, x.x);
+        size = fmaxf(size, x.y);
+        odd |= !(fabsf(x.x) < INFINITY && x.y < INFINITY);
+    }
+    if (tid == 0) s_count = 0;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, x));
+    if (lane == 0) f_warp[warp] = size;
+    odd = __syncthreads_or(odd);
+    size = f_warp[lane % (THREADS / 32)];
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, x));
+    // a lane adds up to 32 products, the lanes 5 times; the weights are rounded (G times): 2^-24 each of the terms' sizes
+    const float eps = (float)(64 + G) * 5.9604645e-8f * size + 1e-42f;
+    // the want-th largest of the threads' maxima, bit by bit
+    uint32_t cut = 0;
+    if (want > 0 && want <= THREADS) {
+        const uint32_t k32 = tid < others ? key32_of(best) : 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t x = cut | (1u << bit);
+            const int cnt = block_sum<THREADS>(k32 >= x, of_warp);
+            if (cnt >= want) cut = x;
+            if (cnt == want) break;
+        }
+    }
+    // cut 0: fewer maxima than wanted.  An early end leaves cut at or below the want-th maximum: a lower floor.
+    const float floor = cut == 0 || odd ? -INFINITY : of_key32(cut) - 2.f * eps;
+    // 64-bit score of a page, by a warp
+    auto exact = [&](int p) {
+        const int64_t phys = physical_page(c, b, p, status);
+        if (phys < 0) return (uint64_t)0;
+        double s = 0;
+        for (int v = lane; v < 2 * vecs; v += 32) {
+            const bool high = v >= vecs;
+            const int col = (high ? v - vecs : v) * W;
+            float x[W];
+            Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(bounds + ((phys * 2 + high) * Hkv + h) * D + col)), x);
+            const double *w = high ? up : down;
+#pragma unroll
+            for (int j = 0; j < W; ++j) s += w[col + j] * (double)x[j];
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        return key_of(s);
+    };
+    if (want > 0)
+        for (int i = tid; i < others; i += THREADS)
+            if (odd || mine[i].x >= floor) {
+                const int at = atomicAdd(&s_count, 1);       // the order in the list does not matter: ranks are counted
+                if (at < kCandidates) page_of[at] = i;
+            }
+    __syncthreads();
+    const int m = s_count;
+    if (m <= kCandidates) {
+        for (int i = warp; i < m; i += THREADS / 32) {
+            const uint64_t k = exact(page_of[i]);
+            if (lane == 0) key[i] = k;
+        }
+        __syncthreads();
+        // rank of each candidate, then (marked by a set sign of its page) its place among the winners
+        bool wins[(kCandidates + THREADS - 1) / THREADS];
+#pragma unroll
+        for (int y = 0; y < (kCandidates + THREADS - 1) / THREADS; ++y) {
+            const int i = y * THREADS + tid;
+            wins[y] = false;
+            if (i < m) {
+                const uint64_t k = key[i];
+                const int p = page_of[i];
+                int before = 0;
+                for (int j = 0; j < m; ++j) before += key[j] > k || (key[j] == k && page_of[j] < p);
+                wins[y] = before < want;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < (kCandidates + THREADS - 1) / THREADS; ++y) {
+            const int i = y * THREADS + tid;
+            if (i < m && !wins[y]) page_of[i] = INT_MAX;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < (kCandidates + THREADS - 1) / THREADS; ++y) {
+            const int i = y * THREADS + tid;
+            if (i < m && wins[y]) {
+                const int p = page_of[i];
+                int before = 0;
+                for (int j = 0; j < m; ++j) before += page_of[j] < p;
+                o[before] = p;
+            }
+        }
+        if (tid == 0 && others < n) o[want] = others;
+        return;
+    }
+    // everything in 64 bits, over the fp32 scores
+    uint64_t *keys = reinterpret_cast<uint64_t *>(scores + row * c.width);
+    for (int i = warp; i < n; i += THREADS / 32) {
+        const uint64_t k = i == held - 1 ? kOwnKey : exact(i);
+        if (lane == 0) keys[i] = k;
+    }
+    __syncthreads();
+    topk_of_row<THREADS>(keys, n, topk, o, of_warp, tied_of);
+}
+
 template <typename Rows>
 int launch_topk(const uint64_t *keys, int32_t *out, int64_t rows, int64_t most, int64_t topk, const Rows &of, cudaStream_t s) {
     const unsigned grid = (unsigned)((rows + 3) / 4);
@@ -326,7 +707,7 @@ int launch_topk(const uint64_t *keys, int32_t *out, int64_t rows, int64_t most, 
     if (most <= 128) e = launch_after(topk_warp_kernel<4, Rows>, dim3(grid), dim3(128), 0, s, keys, out, rows, (int)topk, of);
     else if (most <= 512) e = launch_after(topk_warp_kernel<16, Rows>, dim3(grid), dim3(128), 0, s, keys, out, rows, (int)topk, of);
     else if (most <= kWarpRow) e = launch_after(topk_warp_kernel<32, Rows>, dim3(grid), dim3(128), 0, s, keys, out, rows, (int)topk, of);
-    else e = launch_after(topk_block_kernel<1024, 16, Rows>, dim3((unsigned)rows), dim3(1024), 0, s, keys, out, (int)topk, of);
+    else e = launch_after(topk_block_kernel<1024, Rows>, dim3((unsigned)rows), dim3(1024), 0, s, keys, out, (int)topk, of);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the selection");
 }
 
@@ -351,22 +732,79 @@ int check_select(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dt
     return MAT_OK;
 }
 
+// 16-bit rows of up to kWarpRow blocks: fp32 scores on the tensor cores, one warp per row.
+bool scores_in_fp32(int dtype, int64_t nb) { return dtype != MAT_F32 && nb <= kWarpRow; }
+
+struct SelectPlan {
+    int64_t nb, step;          // blocks, queries whose scores are held at a time
+    size_t norms, q_norms, scores, total;
+};
+
+SelectPlan select_plan(int64_t B, int64_t S, int64_t Hkv, int64_t D, int dtype, int64_t block) {
+    SelectPlan p;
+    p.nb = (S + block - 1) / block;
+    p.step = rows_at_a_time(B, S, Hkv, p.nb);
+    p.norms = align256((size_t)B * p.nb * 2 * Hkv * D * dtype_size(dtype));      // the blocks' bounds lie first
+    p.q_norms = p.norms + align256((size_t)B * p.nb * Hkv * 4);
+    p.scores = p.q_norms + align256((size_t)p.step * B * Hkv * 4);
+    p.total = p.scores + (size_t)p.step * B * Hkv * p.nb * (scores_in_fp32(dtype, p.nb) ? 4 : 8);
+    return p;
+}
+
+template <typename T, int DP>
+cudaError_t launch_scores_mma(dim3 grid, cudaStream_t s, const T *q, const T *bounds, float *scores, float *norms, int64_t S, int64_t H, int64_t Hkv,
+                              int64_t D, int64_t nb, int block, int causal, int64_t s0, int64_t s1) {
+    const size_t smem = 64 * (DP + 8) * sizeof(T);
+    if (ensure_dynamic_smem((const void *)block_scores_mma_kernel<T, DP>, smem, "shared memory of the block scores")) return cudaErrorInvalidValue;
+    return launch_after(block_scores_mma_kernel<T, DP>, grid, dim3(128), smem, s, q, bounds, scores, norms, S, H, Hkv, D, nb, block, causal, s0, s1);
+}
+
 template <typename T>
-int run_select_blocks(const T *q, const T *k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk,
+int select_in_fp32(const T *q, const T *bounds, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk, int causal,
+                   int32_t *blocks, char *ws, const SelectPlan &p, cudaStream_t s) {
+    float *norms = (float *)(ws + p.norms), *q_norms = (float *)(ws + p.q_norms), *scores = (float *)(ws + p.scores);
+    const int64_t all = B * p.nb * Hkv;
+    cudaError_t e = launch_after(block_norms_kernel<T>, dim3((unsigned)((all + 3) / 4)), dim3(128), 0, s, bounds, norms, all, Hkv, D);
+    for (int64_t s0 = 0; s0 < S && e == cudaSuccess; s0 += p.step) {
+        const int64_t s1 = s0 + p.step < S ? s0 + p.step : S, seen = causal ? (s1 - 1) / block + 1 : p.nb, rows = (s1 - s0) * B * Hkv;
+        const dim3 grid((unsigned)((seen + 63) / 64), (unsigned)((s1 - s0 + 63) / 64), (unsigned)(B * Hkv));
+        e = D <= 64 ? launch_scores_mma<T, 64>(grid, s, q, bounds, scores, q_norms, S, H, Hkv, D, p.nb, (int)block, causal, s0, s1)
+                    : launch_scores_mma<T, 128>(grid, s, q, bounds, scores, q_norms, S, H, Hkv, D, p.nb, (int)block, causal, s0, s1);
+        if (e != cudaSuccess) break;
+        const RowsOfBlocks of{B, S, Hkv, p.nb, s0, (int)block, causal};
+        const dim3 ctas((unsigned)((rows + 3) / 4));
+#define SELECT_ROWS(PER) e = launch_after(select_rows_kernel<PER, T>, ctas, dim3(128), 0, s, q, bounds, scores, q_norms, norms, blocks, rows, (int)topk, H, D, of)
+        if (seen <= 128) SELECT_ROWS(4);
+        else if (seen <= 256) SELECT_ROWS(8);
+        else if (seen <= 512) SELECT_ROWS(16);
+        else SELECT_ROWS(32);
+#undef SELECT_ROWS
+    }
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the block selection");
+}
+template <>
+int select_in_fp32<float>(const float *, const float *, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int, int32_t *, char *,
+                          const SelectPlan &, cudaStream_t) {
+    return fail(MAT_ERR_UNSUPPORTED, "fp32 inputs are scored in 64 bits");
+}
+
+template <typename T>
+int run_select_blocks(const T *q, const T *k, int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t block, int64_t topk,
                       int causal, int32_t *blocks, void *ws, cudaStream_t s) {
-    const int64_t nb = (S + block - 1) / block, step = rows_at_a_time(B, S, Hkv, nb);
+    const SelectPlan p = select_plan(B, S, Hkv, D, dtype, block);
     T *bounds = (T *)ws;
-    uint64_t *keys = (uint64_t *)((char *)ws + align256((size_t)B * nb * 2 * Hkv * D * sizeof(T)));
-    block_bounds_kernel<T><<<dim3((unsigned)nb, (unsigned)((Hkv * D + 32 * Vec16<T>::N - 1) / (32 * Vec16<T>::N)), (unsigned)B), 256, 0, s>>>(k, bounds, S, nb, (int)block, Hkv * D);
+    block_bounds_kernel<T><<<dim3((unsigned)p.nb, (unsigned)((Hkv * D + 32 * Vec16<T>::N - 1) / (32 * Vec16<T>::N)), (unsigned)B), 256, 0, s>>>(k, bounds, S, p.nb, (int)block, Hkv * D);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "launching the block bounds");
-    for (int64_t s0 = 0; s0 < S; s0 += step) {
-        const int64_t s1 = s0 + step < S ? s0 + step : S;
-        const int64_t seen = causal ? (s1 - 1) / block + 1 : nb;
+    if (scores_in_fp32(dtype, p.nb)) return select_in_fp32<T>(q, bounds, B, S, H, Hkv, D, block, topk, causal, blocks, (char *)ws, p, s);
+    uint64_t *keys = (uint64_t *)((char *)ws + p.scores);
+    for (int64_t s0 = 0; s0 < S; s0 += p.step) {
+        const int64_t s1 = s0 + p.step < S ? s0 + p.step : S;
+        const int64_t seen = causal ? (s1 - 1) / block + 1 : p.nb;
         dim3 grid((unsigned)((seen + 63) / 64), (unsigned)((s1 - s0 + 63) / 64), (unsigned)(B * Hkv));
-        e = launch_after(block_scores_kernel<T>, grid, dim3(256), 0, s, q, (const T *)bounds, keys, S, H, Hkv, D, nb, (int)block, causal, s0, s1);
+        e = launch_after(block_scores_kernel<T>, grid, dim3(256), 0, s, q, (const T *)bounds, keys, S, H, Hkv, D, p.nb, (int)block, causal, s0, s1);
         if (e != cudaSuccess) return cuda_fail(e, "launching the block scores");
-        RowsOfBlocks of{B, S, Hkv, nb, s0, (int)block, causal};
+        RowsOfBlocks of{B, S, Hkv, p.nb, s0, (int)block, causal};
         if (int rc = launch_topk(keys, blocks, (s1 - s0) * B * Hkv, seen, topk, of, s)) return rc;
     }
     return MAT_OK;
@@ -382,14 +820,15 @@ int check_paged_select(const mat_paged_cache *c, int64_t B, int64_t H, int64_t w
 
 template <typename T>
 int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, int64_t q_stride, int64_t B, int64_t H, const int32_t *lengths,
-                     int64_t topk, int32_t *pages, uint64_t *keys, int *status, cudaStream_t s) {
+                     int64_t topk, int32_t *pages, float2 *scores, int *status, cudaStream_t s) {
     const int vecs = 2 * (int)c->D / Vec16<T>::N;            // of one page and head
     const int lp = vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
+    const T *bounds = (const T *)c->key_bounds;
     int64_t gx = (v.width * lp + 4 * 256 - 1) / (4 * 256);
     const int64_t cap = 148 * 8 / (B * c->H_kv) + 1;         // enough CTAs to fill the GPU; each walks several pages
     if (gx > cap) gx = cap;
     const dim3 grid((unsigned)gx, (unsigned)c->H_kv, (unsigned)B);
-#define PAGE_SCORES(LP, NV) page_scores_kernel<T, LP, NV><<<grid, 256, 0, s>>>(v, (const T *)c->key_bounds, q, q_stride, H, c->H_kv, c->D, lengths, keys, status)
+#define PAGE_SCORES(LP, NV) page_scores_kernel<T, LP, NV><<<grid, 256, 0, s>>>(v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, status)
     if (lp == 8) PAGE_SCORES(8, 1);
     else if (lp == 16) PAGE_SCORES(16, 1);
     else if (vecs <= 32) PAGE_SCORES(32, 1);
@@ -398,8 +837,11 @@ int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, i
 #undef PAGE_SCORES
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "launching the page scores");
-    RowsOfPages of{lengths, c->H_kv, v.width, v.page_shift};
-    return launch_topk(keys, pages, B * c->H_kv, v.width, topk, of, s);
+    const dim3 rows((unsigned)c->H_kv, (unsigned)B);
+    // few pages per row: a small CTA, whose steps wait for fewer warps
+    if (v.width <= 2048 && topk <= 128) e = launch_after(select_pages_kernel<T, 256>, rows, dim3(256), 0, s, v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status);
+    else e = launch_after(select_pages_kernel<T, 1024>, rows, dim3(1024), 0, s, v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status);
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the selection");
 }
 
 }  // namespace
@@ -409,8 +851,7 @@ using namespace mat;
 
 extern "C" size_t mat_select_blocks_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype, int64_t block, int64_t topk) {
     if (check_select(B, S, H, H_kv, D, dtype, block, topk)) return 0;
-    const int64_t nb = (S + block - 1) / block;
-    return align256((size_t)B * nb * 2 * H_kv * D * dtype_size(dtype)) + (size_t)rows_at_a_time(B, S, H_kv, nb) * B * H_kv * nb * 8;
+    return select_plan(B, S, H_kv, D, dtype, block).total;
 }
 
 extern "C" int mat_select_blocks(const void *q, const void *k, int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype, int64_t block,
@@ -425,9 +866,9 @@ extern "C" int mat_select_blocks(const void *q, const void *k, int64_t B, int64_
     cudaStream_t s = (cudaStream_t)stream;
     causal = causal != 0;
     switch (dtype) {
-        case MAT_F32: return run_select_blocks((const float *)q, (const float *)k, B, S, H, H_kv, D, block, topk, causal, blocks, workspace, s);
-        case MAT_BF16: return run_select_blocks((const __nv_bfloat16 *)q, (const __nv_bfloat16 *)k, B, S, H, H_kv, D, block, topk, causal, blocks, workspace, s);
-        default: return run_select_blocks((const __half *)q, (const __half *)k, B, S, H, H_kv, D, block, topk, causal, blocks, workspace, s);
+        case MAT_F32: return run_select_blocks((const float *)q, (const float *)k, B, S, H, H_kv, D, dtype, block, topk, causal, blocks, workspace, s);
+        case MAT_BF16: return run_select_blocks((const __nv_bfloat16 *)q, (const __nv_bfloat16 *)k, B, S, H, H_kv, D, dtype, block, topk, causal, blocks, workspace, s);
+        default: return run_select_blocks((const __half *)q, (const __half *)k, B, S, H, H_kv, D, dtype, block, topk, causal, blocks, workspace, s);
     }
 }
 
@@ -453,10 +894,10 @@ extern "C" int mat_paged_select(const mat_paged_cache *cache, const void *q, int
     if (!status) return fail(MAT_ERR_CUDA, "no device status word");
     note_kernel("paged_select");
     cudaStream_t s = (cudaStream_t)stream;
-    uint64_t *keys = (uint64_t *)workspace;
+    float2 *scores = (float2 *)workspace;      // and 64-bit keys in their place where a row needs them
     switch (cache->dtype) {
-        case MAT_F32: return run_select_pages(cache, v, (const float *)q, q_stride, B, H, lengths, topk, pages, keys, status, s);
-        case MAT_BF16: return run_select_pages(cache, v, (const __nv_bfloat16 *)q, q_stride, B, H, lengths, topk, pages, keys, status, s);
-        default: return run_select_pages(cache, v, (const __half *)q, q_stride, B, H, lengths, topk, pages, keys, status, s);
+        case MAT_F32: return run_select_pages(cache, v, (const float *)q, q_stride, B, H, lengths, topk, pages, scores, status, s);
+        case MAT_BF16: return run_select_pages(cache, v, (const __nv_bfloat16 *)q, q_stride, B, H, lengths, topk, pages, scores, status, s);
+        default: return run_select_pages(cache, v, (const __half *)q, q_stride, B, H, lengths, topk, pages, scores, status, s);
     }
 }

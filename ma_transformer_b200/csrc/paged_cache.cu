@@ -1,20 +1,24 @@
 // Appends new tokens to a paged key-value cache: keys (and optionally the queries of the same tokens) turned by their
-// positions, values copied, and the touched pages' key bounds set, in one launch.
+// positions, values copied, and the touched pages' key bounds set.
 //
 // Rotation: column pair (a, b) at position p with frequency f becomes (a cos t - b sin t, b cos t + a sin t), t = p f.
 // The angle is formed in 64 bits as a number of half turns, p * (f / pi), and reduced by its nearest even integer
 // before it is rounded to fp32 (an fp32 product would be off by p * f * 2^-24: 0.06 rad at position 10^6).
 //
-// One CTA owns one page of one sequence: it writes the call's tokens of that page and then knows every filled slot, so
-// the bounds (smallest and largest key per column) need no atomics.  CTA x < B takes sequence x's first page, CTA B + t
-// the pages that begin inside rows [t * page, (t + 1) * page) of the packed batch; y is the key head (with the query
-// heads that read it).  Bounds are taken from all filled slots, not merged with the old ones: a cache that was rolled
-// back and written again ends with the same bits as one that never was.
+// append_rows_kernel streams: a CTA takes a tile of tokens with all their heads, finds each token's sequence, page and
+// angles once (a chain of five dependent reads), and then moves 2 x 16 bytes per thread and step.  One CTA per page and
+// key head paid that chain per 10 KB and took 177 us (100 us with 8-byte vectors and more CTAs) where this takes
+// PROMPTS_US us: 7 prompts, 32768 tokens x (12 + 2 * 4) heads of 64 in fp16, 172 MB, 27 us at the copy rate.
+//
+// page_bounds_kernel follows where the cache keeps bounds: one warp owns one page and head and takes its bounds from all
+// filled slots (the new ones come from L2), so there are no atomics, and a cache that was rolled back and written again
+// ends with the same bits as one that never was.
 #include <limits.h>
 
 #include <atomic>
 
 #include "paged.cuh"
+#include "pdl.cuh"
 
 namespace mat {
 
@@ -82,7 +86,7 @@ PagedView paged_view(const mat_paged_cache *c, const int32_t *table, int64_t wid
 
 namespace {
 
-constexpr int kThreads = 256;   // at least two lanes per column pair at D = 256
+constexpr int kKnownStarts = 1024;   // sequences whose row ranges a CTA holds in shared memory
 
 struct AppendArgs {
     PagedView c;
@@ -91,7 +95,7 @@ struct AppendArgs {
     int64_t kn_tok, vn_tok, q_tok, N, B, H, Hkv, D;
     const int32_t *cu, *start;
     const double *inv_freq;
-    int rot, interleaved;
+    int rot, interleaved, tile;     // tile: tokens per CTA of the rows kernel
     int *status;
 };
 
@@ -101,13 +105,18 @@ __device__ __forceinline__ void angle_of(double pos, double freq, float &c, floa
     sincospif((float)r, &s, &c);
 }
 
-// Columns of one row in units of two vectors of four: unit u's vectors start at columns at0, at1, and its pairs are
-// (first vector, second vector) element by element, or neighbours when interleaved.  Four columns (8 bytes of a 16-bit
-// type) keep the kernel within 64 registers, four CTAs a SM: with 16-byte vectors it held two, and packed prompts of
-// 32768 tokens x (12 + 2 * 4) heads of 64 took 177 us instead of WIDE_US.
-constexpr int W = 4;
-struct Unit {
-    int at0, at1, pair;   // pair: index of the unit's first rotated pair, -1 for none
+// First row of sequence b (b = B: the end of the last), inside [0, N] whatever cu_seqlens holds.
+__device__ __forceinline__ int64_t first_row(const AppendArgs &a, int64_t b) {
+    if (!a.cu) return b;
+    const int64_t n = __ldg(a.cu + b);
+    return n < 0 ? 0 : n > a.N ? a.N : n;
+}
+
+// Columns of one row in units of two vectors of W: unit u's vectors start at columns at0 and at1.  Its pairs (from
+// `pair` on, -1: not rotated) are (first vector, second vector) element by element, or neighbours when interleaved.
+// W = 1 serves rotations whose halves do not start on 16 bytes, pair by pair.
+template <int W> struct Unit {
+    int at0, at1, pair;
     __device__ __forceinline__ Unit(int u, int rot, bool interleaved) {
         if (u * 2 * W < rot) {
             pair = u * W;
@@ -121,217 +130,244 @@ struct Unit {
     }
 };
 
-// four elements as fp32 values and back
-template <typename T> struct Four {
-    static __device__ __forceinline__ void load(const T *p, float *x) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        x[0] = Vec16<T>::one((uint16_t)(u.x & 0xffffu)); x[1] = Vec16<T>::one((uint16_t)(u.x >> 16));
-        x[2] = Vec16<T>::one((uint16_t)(u.y & 0xffffu)); x[3] = Vec16<T>::one((uint16_t)(u.y >> 16));
-    }
-    static __device__ __forceinline__ void store(T *p, const float *x) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(Vec16<T>::two(x[0], x[1]), Vec16<T>::two(x[2], x[3]));
-    }
-};
-template <> struct Four<float> {
-    static __device__ __forceinline__ void load(const float *p, float *x) { *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p); }
-    static __device__ __forceinline__ void store(float *p, const float *x) { *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(x); }
-};
-
-// x: the 2 N values of a unit; c, s: cosine and sine of its N pairs
-template <int N> __device__ __forceinline__ void turn(float *x, const float *c, const float *s, bool interleaved) {
-    if (interleaved) {
+// x: the 2 W values of a unit; c, s: cosine and sine of its pairs
+template <int W> __device__ __forceinline__ void turn(float *x, const float *c, const float *s, bool interleaved) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = a * c[i] - b * s[i];
-            x[2 * i + 1] = b * c[i] + a * s[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float a = x[i], b = x[N + i];
-            x[i] = a * c[i] - b * s[i];
-            x[N + i] = b * c[i] + a * s[i];
-        }
+    for (int i = 0; i < W; ++i) {
+        const int p = interleaved ? 2 * i : i, q = interleaved ? 2 * i + 1 : W + i;
+        const float a = x[p], b = x[q];
+        x[p] = a * c[i] - b * s[i];
+        x[q] = b * c[i] + a * s[i];
     }
 }
 
-// Columns that no vector path serves (a rotation whose halves do not start on 16 bytes): pair by pair.
-template <typename T> __device__ __forceinline__ void pair_columns(int r, int rot, bool interleaved, int &c0, int &c1) {
-    if (2 * r < rot) {
-        c0 = interleaved ? 2 * r : r;
-        c1 = interleaved ? 2 * r + 1 : r + rot / 2;
-    } else {
-        c0 = 2 * r;
-        c1 = 2 * r + 1;
-    }
-}
-
-// One page of one sequence: rows [n0, n0 + count) of the packed batch land in slots [slot0, slot0 + count).
-template <typename T, bool VEC>
-__device__ void append_page(const AppendArgs &a, int64_t b, int64_t n0, int count, int64_t pos0, float *red) {
-    constexpr int N = VEC ? W : 1;
-    const int h = blockIdx.y, G = a.q ? (int)(a.H / a.Hkv) : 0;
-    const int D = (int)a.D;
-    const int units = D / (2 * N);
-    const int lanes = kThreads / units;               // rows in flight
-    const int u = threadIdx.x % units, lane = threadIdx.x / units;
-    const bool active = lane < lanes;
-    const int page = 1 << a.c.page_shift;
-    const int slot0 = (int)(pos0 & (page - 1));
-    const int64_t phys = physical_page(a.c, b, pos0 >> a.c.page_shift, a.status);
-
-    // tokens over lanes; lanes left over take the roles (key, value, query heads) of a token in turn
-    int tl = 1;
-    while (tl * 2 <= lanes && tl < count) tl *= 2;
-    const int rl = lanes / tl, my_t = lane % tl, my_r = lane / tl;
-
-    float lo[2 * N], hi[2 * N];
-#pragma unroll
-    for (int i = 0; i < 2 * N; ++i) { lo[i] = INFINITY; hi[i] = -INFINITY; }
-
-    int c0[2] = {0, 0};
-    Unit un(VEC ? u : 0, a.rot, a.interleaved);
-    bool rotated = un.pair >= 0;
-    if (!VEC) {
-        pair_columns<T>(u, a.rot, a.interleaved, c0[0], c0[1]);
-        rotated = 2 * u < a.rot;
-    }
-    auto load = [&](const T *row, float *x) {
-        if (VEC) { Four<T>::load(row + un.at0, x); Four<T>::load(row + un.at1, x + N); }
-        else { x[0] = Elem<T>::to_f(row[c0[0]]); x[N] = Elem<T>::to_f(row[c0[1]]); }
-    };
-    auto store = [&](T *row, const float *x) {
-        if (VEC) { Four<T>::store(row + un.at0, x); Four<T>::store(row + un.at1, x + N); }
-        else { row[c0[0]] = Elem<T>::from_f(x[0]); row[c0[1]] = Elem<T>::from_f(x[N]); }
-    };
-    T *kp = (T *)a.c.k + (phys < 0 ? 0 : phys * a.c.k_page) + (int64_t)h * a.c.k_head;
-    T *vp = (T *)a.c.v + (phys < 0 ? 0 : phys * a.c.v_page) + (int64_t)h * a.c.v_head;
-
-    if (active && my_r < rl) {
-        for (int t = my_t; t < count; t += tl) {
-            const int64_t n = n0 + t;
-            float cs[N], sn[N];
-            if (rotated) {
-                const int pair = VEC ? un.pair : u;
-#pragma unroll
-                for (int i = 0; i < N; ++i) angle_of((double)(pos0 + t), a.inv_freq[pair + i], cs[i], sn[i]);
+template <typename T, bool VEC> __global__ void __launch_bounds__(256, 3) append_rows_kernel(const AppendArgs a) {
+    constexpr int W = VEC ? Vec16<T>::N : 1, U = 4;
+    __shared__ int starts[kKnownStarts + 1];
+    __shared__ int pos_of[64];
+    __shared__ int64_t k_of[64], v_of[64];
+    extern __shared__ float turns[];                 // [tile][rot / 2] cosines, then sines
+    pdl_trigger();
+    const int tid = threadIdx.x, D = (int)a.D, half = a.rot / 2;
+    const int64_t n0 = (int64_t)blockIdx.x * a.tile;
+    const int cnt = (int)(a.N - n0 < a.tile ? a.N - n0 : a.tile);
+    float *cosines = turns, *sines = turns + a.tile * half;
+    const bool known = a.B <= kKnownStarts;
+    if (a.cu && known)
+        for (int i = tid; i <= a.B; i += 256) starts[i] = (int)first_row(a, i);
+    __syncthreads();
+    if (tid < cnt) {
+        const int64_t n = n0 + tid;
+        int64_t b = n, begin = n, pos = -1, k = -1, v = -1;
+        if (a.cu) {                                  // the last sequence that starts at or before n
+            int64_t lo = 0, hi = a.B - 1;
+            while (lo < hi) {
+                const int64_t mid = (lo + hi + 1) >> 1;
+                if ((known ? (int64_t)starts[mid] : first_row(a, mid)) <= n) lo = mid; else hi = mid - 1;
             }
-            for (int role = my_r; role < G + 2; role += rl) {
-                float x[2 * N];
-                if (role == 1) {          // value
-                    if (phys >= 0) {
-                        load((const T *)a.vn + n * a.vn_tok + (int64_t)h * D, x);
-                        store(vp + (int64_t)(slot0 + t) * a.c.v_tok, x);
-                    }
-                    continue;
-                }
-                const T *src = role == 0 ? (const T *)a.kn + n * a.kn_tok + (int64_t)h * D
-                                         : (const T *)a.q + n * a.q_tok + ((int64_t)h * G + role - 2) * D;
-                if (role == 0 && phys < 0) continue;
-                load(src, x);
-                if (rotated) turn<N>(x, cs, sn, a.interleaved);
-                if (role == 0) {
-                    store(kp + (int64_t)(slot0 + t) * a.c.k_tok, x);
-#pragma unroll
-                    for (int i = 0; i < 2 * N; ++i) {
-                        const float y = Elem<T>::to_f(Elem<T>::from_f(x[i]));   // the key as the cache holds it
-                        lo[i] = fminf(lo[i], y);
-                        hi[i] = fmaxf(hi[i], y);
-                    }
-                } else {
-                    store((T *)a.qo + (n * a.H + (int64_t)h * G + role - 2) * D, x);
+            b = lo;
+            begin = first_row(a, b);
+            if (n < begin || n >= first_row(a, b + 1)) b = -1;      // padding
+        }
+        if (b >= 0) {
+            const int64_t at = a.start[b];
+            if (at < 0) {
+                atomicOr(a.status, kPagedOutside);
+            } else {
+                pos = at + n - begin;
+                if (pos > INT_MAX) atomicOr(a.status, kPagedOutside);
+                const int64_t phys = pos > INT_MAX ? -1 : physical_page(a.c, b, pos >> a.c.page_shift, a.status);
+                const int64_t slot = pos & ((1 << a.c.page_shift) - 1);
+                if (phys >= 0) {
+                    k = phys * a.c.k_page + slot * a.c.k_tok;
+                    v = phys * a.c.v_page + slot * a.c.v_tok;
                 }
             }
         }
-        if (a.bounds && phys >= 0)
-            for (int s = lane; s < slot0; s += lanes) {      // slots filled by earlier calls
-                float x[2 * N];
-                load(kp + (int64_t)s * a.c.k_tok, x);
-#pragma unroll
-                for (int i = 0; i < 2 * N; ++i) {
-                    lo[i] = fminf(lo[i], x[i]);
-                    hi[i] = fmaxf(hi[i], x[i]);
-                }
-            }
-    }
-    if (!a.bounds) return;            // the same for the whole grid
-    // join the lanes' bounds; red: [lo, hi][element of a unit][thread]
-#pragma unroll
-    for (int i = 0; i < 2 * N; ++i) {
-        red[i * kThreads + threadIdx.x] = lo[i];
-        red[(2 * N + i) * kThreads + threadIdx.x] = hi[i];
+        pos_of[tid] = pos > INT_MAX ? -1 : (int)pos;
+        k_of[tid] = k;
+        v_of[tid] = v;
     }
     __syncthreads();
-    if (phys < 0) return;
-    const int used = min(lanes, max(tl, slot0));        // lanes that saw a key
-    T *out = (T *)a.bounds + (phys * 2 * a.Hkv + h) * (int64_t)D;
-    for (int o = threadIdx.x; o < 4 * N * units; o += kThreads) {
-        const bool is_hi = o >= 2 * N * units;
-        const int r = is_hi ? o - 2 * N * units : o, i = r / units, v = r % units;
-        int col[2] = {0, 0};
-        if (VEC) {
-            const Unit w(v, a.rot, a.interleaved);
-            col[0] = w.at0 + i; col[1] = w.at1 + i - N;
-        } else {
-            pair_columns<T>(v, a.rot, a.interleaved, col[0], col[1]);
+    for (int i = tid; i < cnt * half; i += 256) {
+        const int t = i / half;
+        angle_of((double)pos_of[t], a.inv_freq[i - t * half], cosines[i], sines[i]);
+    }
+    __syncthreads();
+    const int units = (D + 2 * W - 1) / (2 * W), heads_q = a.q ? (int)a.H : 0, heads_k = (int)a.Hkv, roles = heads_q + 2 * heads_k;
+    const int total = cnt * roles * units;
+    for (int i0 = tid; i0 < total; i0 += 256 * U) {
+        uint4 raw[U][2];
+        T *dst[U];
+        int tok[U], un[U];
+        bool turned[U];
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+            const int i = i0 + y * 256;
+            dst[y] = nullptr;
+            if (i >= total) continue;
+            const int rest = i / units;
+            un[y] = i - rest * units;
+            tok[y] = rest / roles;
+            const int role = rest - tok[y] * roles;
+            const int64_t n = n0 + tok[y];
+            const T *src;
+            if (role < heads_q) {
+                src = (const T *)a.q + n * a.q_tok + (int64_t)role * D;
+                if (pos_of[tok[y]] >= 0) dst[y] = (T *)a.qo + (n * a.H + role) * D;
+            } else if (role < heads_q + heads_k) {
+                const int h = role - heads_q;
+                src = (const T *)a.kn + n * a.kn_tok + (int64_t)h * D;
+                if (k_of[tok[y]] >= 0) dst[y] = (T *)a.c.k + k_of[tok[y]] + h * a.c.k_head;
+            } else {
+                const int h = role - heads_q - heads_k;
+                src = (const T *)a.vn + n * a.vn_tok + (int64_t)h * D;
+                if (v_of[tok[y]] >= 0) dst[y] = (T *)a.c.v + v_of[tok[y]] + h * a.c.v_head;
+            }
+            const Unit<W> u(un[y], a.rot, a.interleaved);
+            turned[y] = u.pair >= 0 && role < heads_q + heads_k;
+            // values have no pairs: their vectors are moved where the rotation's halves lie all the same
+            if (!dst[y]) continue;
+            if (VEC) {
+                raw[y][0] = *reinterpret_cast<const uint4 *>(src + u.at0);
+                if (u.at1 < D) raw[y][1] = *reinterpret_cast<const uint4 *>(src + u.at1);
+            } else {
+                raw[y][0].x = __float_as_uint(Elem<T>::to_f(src[u.at0]));
+                raw[y][1].x = __float_as_uint(Elem<T>::to_f(src[u.at1]));
+            }
         }
-        const int c = i < N ? col[0] : col[1];
-        const float *x = red + (is_hi ? 2 * N + i : i) * kThreads + v;
-        float m = x[0];
-        for (int l = 1; l < used; ++l) m = is_hi ? fmaxf(m, x[l * units]) : fminf(m, x[l * units]);
-        out[(is_hi ? a.Hkv * (int64_t)D : 0) + c] = Elem<T>::from_f(m);
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+            if (!dst[y]) continue;
+            const Unit<W> u(un[y], a.rot, a.interleaved);
+            if (turned[y]) {
+                float x[2 * W];
+                const float *c = cosines + tok[y] * half + u.pair, *s = sines + tok[y] * half + u.pair;
+                if (VEC) {
+                    Vec16<T>::unpack(raw[y][0], x);
+                    Vec16<T>::unpack(raw[y][1], x + W);
+                } else {
+                    x[0] = __uint_as_float(raw[y][0].x);
+                    x[W] = __uint_as_float(raw[y][1].x);
+                }
+                turn<W>(x, c, s, a.interleaved);
+                if (VEC) {
+                    raw[y][0] = Vec16<T>::pack(x);
+                    raw[y][1] = Vec16<T>::pack(x + W);
+                } else {
+                    raw[y][0].x = __float_as_uint(x[0]);
+                    raw[y][1].x = __float_as_uint(x[W]);
+                }
+            }
+            if (VEC) {
+                *reinterpret_cast<uint4 *>(dst[y] + u.at0) = raw[y][0];
+                if (u.at1 < D) *reinterpret_cast<uint4 *>(dst[y] + u.at1) = raw[y][1];
+            } else {
+                dst[y][u.at0] = Elem<T>::from_f(__uint_as_float(raw[y][0].x));
+                dst[y][u.at1] = Elem<T>::from_f(__uint_as_float(raw[y][1].x));
+            }
+        }
     }
 }
 
-template <typename T, bool VEC> __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a) {
-    __shared__ float red[4 * (VEC ? W : 1) * kThreads];
-    const int page = 1 << a.c.page_shift;
-    auto first_row = [&](int64_t b) -> int64_t {
-        if (!a.cu) return b;
-        const int64_t n = a.cu[b];
-        return n < 0 ? 0 : (n > a.N ? a.N : n);
-    };
-    if (blockIdx.x < a.B) {
-        const int64_t b = blockIdx.x, n0 = first_row(b), end = first_row(b + 1);
-        if (n0 >= end) return;
-        const int64_t pos = a.start[b];
-        if (pos < 0) {
-            atomicOr(a.status, kPagedOutside);
-            return;
+// Bounds of one page and head from its first `filled` slots, by one warp: LV lanes of 16 bytes share a token.
+template <typename T> __device__ void page_bounds(const AppendArgs &a, int64_t phys, int h, int filled) {
+    constexpr int W = Vec16<T>::N;
+    const int lane = threadIdx.x % 32, D = (int)a.D, vecs = D / W;
+    const int lv = vecs <= 1 ? 1 : vecs <= 2 ? 2 : vecs <= 4 ? 4 : vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32, lt = 32 / lv;
+    const T *rows = (const T *)a.c.k + phys * a.c.k_page + (int64_t)h * a.c.k_head;
+    T *out = (T *)a.bounds + (phys * 2 * a.Hkv + h) * (int64_t)D;
+    for (int v0 = 0; v0 < vecs; v0 += lv) {
+        const int col = (v0 + lane % lv) * W;
+        float lo[W], hi[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) { lo[j] = INFINITY; hi[j] = -INFINITY; }
+        if (col < D)
+#pragma unroll 8
+            for (int s = lane / lv; s < filled; s += lt) {
+                float x[W];
+                Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(rows + s * a.c.k_tok + col), x);
+#pragma unroll
+                for (int j = 0; j < W; ++j) { lo[j] = fminf(lo[j], x[j]); hi[j] = fmaxf(hi[j], x[j]); }
+            }
+        for (int o = lv; o < 32; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
+                hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
+            }
+        if (lane < lv && col < D) {
+            *reinterpret_cast<uint4 *>(out + col) = Vec16<T>::pack(lo);
+            *reinterpret_cast<uint4 *>(out + a.Hkv * (int64_t)D + col) = Vec16<T>::pack(hi);
         }
-        const int64_t room = page - (pos & (page - 1));
-        append_page<T, VEC>(a, b, n0, (int)(room < end - n0 ? room : end - n0), pos, red);
+    }
+}
+
+// Warp x < B: the first page of sequence x; warp B + t: the pages that begin inside rows [t * page, (t + 1) * page) of
+// the packed batch and are not a sequence's first.
+template <typename T> __global__ void __launch_bounds__(128) page_bounds_kernel(const AppendArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32, h = blockIdx.y, page = 1 << a.c.page_shift;
+    auto one = [&](int64_t b, int64_t pos, int64_t count) {       // `count` new tokens from position pos on one page
+        if (pos < 0 || pos > INT_MAX) return;
+        const int64_t phys = physical_page(a.c, b, pos >> a.c.page_shift, a.status);
+        if (phys >= 0) page_bounds<T>(a, phys, h, (int)((pos & (page - 1)) + count));
+    };
+    if (item < a.B) {
+        const int64_t n0 = first_row(a, item), end = first_row(a, item + 1), pos = a.start[item], room = page - (pos & (page - 1));
+        if (n0 < end) one(item, pos, room < end - n0 ? room : end - n0);
         return;
     }
-    // pages that begin inside this tile of rows and are not a sequence's first
-    const int64_t t0 = (int64_t)(blockIdx.x - a.B) * page, t1 = t0 + page;
+    const int64_t t0 = (item - a.B) * page, t1 = t0 + page;
+    if (!a.cu || t0 >= a.N) return;
     int64_t lo = 0, hi = a.B - 1;                    // the last sequence that starts at or before t0, 32 guesses at a time
     while (lo < hi) {
-        const int64_t step = (hi - lo + 32) / 32, at = lo + (threadIdx.x % 32) * step;
-        const uint32_t before = __ballot_sync(0xffffffffu, at <= hi && first_row(at) <= t0);
+        const int64_t step = (hi - lo + 32) / 32, at = lo + lane * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, at <= hi && first_row(a, at) <= t0);
         if (!before) break;                          // only for malformed cu_seqlens
         lo += (31 - __clz(before)) * step;
         hi = hi < lo + step - 1 ? hi : lo + step - 1;
     }
-    for (int64_t b = lo; b < a.B && first_row(b) < t1; ++b) {
-        const int64_t n0 = first_row(b), end = first_row(b + 1), pos = a.start[b];
-        if (n0 >= end || pos < 0) continue;
-        int64_t n = n0 + page - (pos & (page - 1));  // the first row on a page of its own
-        if (n < t0) n += (t0 - n + page - 1) / page * page;
-        if (n >= t1 || n >= end) continue;
-        append_page<T, VEC>(a, b, n, (int)(page < end - n ? page : end - n), pos + n - n0, red);
-        __syncthreads();
+    for (int64_t b0 = lo; b0 < a.B; b0 += 32) {      // 32 sequences at a time: at most one page of each begins here
+        const int64_t b = b0 + lane;
+        int64_t n = -1, pos = 0, count = 0;
+        bool more = false;
+        if (b < a.B) {
+            const int64_t n0 = first_row(a, b), end = first_row(a, b + 1), at = a.start[b];
+            more = n0 < t1;
+            if (more && n0 < end && at >= 0) {
+                n = n0 + page - (at & (page - 1));   // the first row on a page of its own
+                if (n < t0) n += (t0 - n + page - 1) / page * page;
+                if (n >= t1 || n >= end) n = -1;
+                pos = at + n - n0;
+                count = page < end - n ? page : end - n;
+            }
+        }
+        uint32_t found = __ballot_sync(0xffffffffu, n >= 0);
+        while (found) {
+            const int who = __ffs(found) - 1;
+            found &= found - 1;
+            one(b0 + who, __shfl_sync(0xffffffffu, pos, who), __shfl_sync(0xffffffffu, count, who));
+        }
+        if (!__all_sync(0xffffffffu, more)) return;
     }
 }
 
-template <typename T> int launch_append(const AppendArgs &a, bool vec, cudaStream_t stream) {
-    const int64_t page = 1ll << a.c.page_shift;
-    const int64_t gx = a.B + (a.cu ? (a.N + page - 1) / page : 0);
-    dim3 grid((unsigned)gx, (unsigned)a.Hkv);
-    if (vec) append_kernel<T, true><<<grid, kThreads, 0, stream>>>(a);
-    else append_kernel<T, false><<<grid, kThreads, 0, stream>>>(a);
+template <typename T> int launch_append(AppendArgs &a, bool vec, cudaStream_t stream) {
+    // enough tiles to fill the GPU, few enough that a tile's look-ups are shared: 1 to 64 tokens, 32 KB of angles
+    a.tile = 1;
+    while (a.tile < 64 && a.tile * 148 * 4 < a.N && (a.tile * 2) * a.rot * 4 <= 32768) a.tile *= 2;
+    const unsigned tiles = (unsigned)((a.N + a.tile - 1) / a.tile);
+    const size_t smem = (size_t)a.tile * a.rot * sizeof(float);
+    if (vec) append_rows_kernel<T, true><<<tiles, 256, smem, stream>>>(a);
+    else append_rows_kernel<T, false><<<tiles, 256, smem, stream>>>(a);
     cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && a.bounds) {
+        const int64_t page = 1ll << a.c.page_shift, items = a.B + (a.cu ? (a.N + page - 1) / page : 0);
+        e = launch_after(page_bounds_kernel<T>, dim3((unsigned)((items + 3) / 4), (unsigned)a.Hkv), dim3(128), 0, stream, a);
+    }
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged append");
 }
 
@@ -370,12 +406,12 @@ extern "C" int mat_paged_append(const mat_paged_cache *cache, const void *k_new,
     a.rot = inv_freq ? (int)rot : 0;
     a.interleaved = interleaved != 0;
     if (!(a.status = paged_status_word())) return fail(MAT_ERR_CUDA, "no device status word");
-    const bool v4 = a.rot % (2 * W) == 0;   // both halves of a rotated pair start on a vector
-    note_kernel(v4 ? "paged_append" : "paged_append_pairs");
+    const bool whole = a.rot % (2 * vec) == 0;   // both halves of a rotated pair start on 16 bytes
+    note_kernel(whole ? "paged_append" : "paged_append_pairs");
     cudaStream_t s = (cudaStream_t)stream;
     switch (cache->dtype) {
-        case MAT_F32: return launch_append<float>(a, v4, s);
-        case MAT_BF16: return launch_append<__nv_bfloat16>(a, v4, s);
-        default: return launch_append<__half>(a, v4, s);
+        case MAT_F32: return launch_append<float>(a, whole, s);
+        case MAT_BF16: return launch_append<__nv_bfloat16>(a, whole, s);
+        default: return launch_append<__half>(a, whole, s);
     }
 }
