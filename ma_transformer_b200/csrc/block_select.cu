@@ -220,9 +220,9 @@ __global__ void __launch_bounds__(128) block_scores_mma_kernel(const T *q, const
         }
 }
 
-// Euclidean norm of max(|lo|, |hi|) of every block and head, one warp each
+// Euclidean norm of max(|lo|, |hi|) of every block and head, one warp each; norms: [B, H_kv, blocks]
 template <typename T>
-__global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float *norms, int64_t rows, int64_t Hkv, int64_t D) {
+__global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float *norms, int64_t rows, int64_t nb, int64_t Hkv, int64_t D) {
     const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;      // (b * nb + n) * Hkv + h
     pdl_trigger();
     pdl_wait();
@@ -235,23 +235,18 @@ __global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x % 32 == 0) norms[r] = sqrtf(s);
+    if (threadIdx.x % 32 == 0) norms[(r / Hkv / nb * Hkv + r % Hkv) * nb + r / Hkv % nb] = sqrtf(s);
 }
 
 // ---- scores of a cache's pages ---------------------------------------------------------------------------------------
 // LP lanes share a page: a lane holds the weights of its NV vectors (of the 2 D bounds: smallest keys, then largest) in
-// registers and reads four pages' vectors at once.  Leaves (score, sum of the terms' absolute values) in fp32.
+// registers and reads four pages' vectors at once.  Leaves (score, sum of the terms' absolute values) in fp32 for pages
+// first, first + step, ... of a row; `threads` threads take part.
 template <typename T, int LP, int NV>
-__global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
-                                                          const int32_t *lengths, float2 *scores, int *status) {
-    constexpr int W = Vec16<T>::N, GROUPS = 256 / LP, U = NV >= 4 ? 2 : 4;
-    const int64_t b = blockIdx.z, h = blockIdx.y, G = H / Hkv;
-    pdl_trigger();
-    const int64_t len = lengths[b];
-    if (len <= 0) return;
-    const int64_t held = ((len - 1) >> c.page_shift) + 1;      // pages that hold tokens; the last is the token's own
-    const int64_t n = held < c.width ? held : c.width;
-    if ((int64_t)blockIdx.x * GROUPS >= n) return;
+__device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds, const T *q, int64_t H, int64_t Hkv, int64_t D, int64_t b, int64_t h,
+                                            int n, int first, int step, float2 *scores, int *status) {
+    constexpr int W = Vec16<T>::N, U = NV >= 4 ? 2 : 4;
+    const int64_t G = H / Hkv;
     const int part = threadIdx.x % LP, vecs = (int)D / W;
     float w[NV][W];
     int off[NV];
@@ -266,27 +261,33 @@ __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *
         if (off[i] >= 0)
             for (int64_t g = 0; g < G; ++g) {
                 float x[W];
-                Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(q + b * q_stride + (h * G + g) * D + col)), x);
+                Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(q + (h * G + g) * D + col)), x);
 #pragma unroll
                 for (int j = 0; j < W; ++j)
                     if ((x[j] > 0) == high) w[i][j] += x[j];       // a NaN lands among the smallest keys' weights
             }
     }
-    const int64_t step = (int64_t)gridDim.x * GROUPS;
-    // the trip count is the same for all lanes of a warp (they shuffle together): bounded by the CTA's first group
-    for (int64_t p0 = (int64_t)blockIdx.x * GROUPS; p0 < n; p0 += U * step) {
+    // the table is read a step ahead; the trip count is the same for all lanes of a warp (they shuffle together)
+    int next[U];
+    auto look_up = [&](int p0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = p0 + u * step + threadIdx.x / LP;
+            next[u] = p < n ? (int)physical_page(c, b, p, status) : -1;
+        }
+    };
+    look_up(first);
+    for (int p0 = first; p0 < n; p0 += U * step) {
         uint4 x[U][NV];
         int64_t phys[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t p = p0 + u * step + threadIdx.x / LP;
-            phys[u] = p < n ? physical_page(c, b, p, status) : -1;
-        }
+        for (int u = 0; u < U; ++u) phys[u] = next[u];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 x[u][i] = phys[u] >= 0 && off[i] >= 0 ? __ldg(reinterpret_cast<const uint4 *>(bounds + phys[u] * 2 * Hkv * D + off[i])) : make_uint4(0, 0, 0, 0);
+        look_up(p0 + U * step);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float s = 0.f, size = 0.f;
@@ -305,25 +306,40 @@ __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *
                 s += __shfl_xor_sync(0xffffffffu, s, o);
                 size += __shfl_xor_sync(0xffffffffu, size, o);
             }
-            const int64_t p = p0 + u * step + threadIdx.x / LP;
+            const int p = p0 + u * step + threadIdx.x / LP;
             // a page outside the cache is no number: it sends its row to the 64-bit scores, where it ranks last
-            if (part == 0 && p < n) scores[(b * Hkv + h) * c.width + p] = make_float2(phys[u] < 0 ? -INFINITY : s, size);
+            if (part == 0 && p < n) scores[p] = make_float2(phys[u] < 0 ? -INFINITY : s, size);
         }
     }
+}
+
+template <typename T, int LP, int NV>
+__global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
+                                                          const int32_t *lengths, float2 *scores, int *status) {
+    constexpr int GROUPS = 256 / LP;
+    const int64_t b = blockIdx.z, h = blockIdx.y;
+    pdl_trigger();
+    const int64_t len = lengths[b];
+    if (len <= 0) return;
+    const int64_t held = ((len - 1) >> c.page_shift) + 1;      // pages that hold tokens; the last is the token's own
+    const int n = (int)(held < c.width ? held : c.width), first = blockIdx.x * GROUPS;
+    if (first < n)
+        score_pages<T, LP, NV>(c, bounds, q + b * q_stride, H, Hkv, D, b, h, n, first, gridDim.x * GROUPS, scores + (b * Hkv + h) * c.width, status);
 }
 
 // ---- the topk of a row -----------------------------------------------------------------------------------------------
 // Rows of whole sequences: row r = (s - s_lo, b, h), its eligible keys are [0, own] (causal) or [0, nb).
 struct RowsOfBlocks {
-    int64_t B, S, Hkv, nb, s_lo;
-    int block, causal;
-    __device__ __forceinline__ int64_t count(int64_t r) const { return causal ? (s_lo + r / (B * Hkv)) / block + 1 : nb; }
+    int B, S, Hkv, nb, s_lo, block, causal;     // 32-bit: a 64-bit division is some 100 instructions
+    __device__ __forceinline__ int query(uint32_t r) const { return s_lo + (int)(r / (uint32_t)(B * Hkv)); }
+    __device__ __forceinline__ int count(uint32_t r) const { return causal ? query(r) / block + 1 : nb; }
     __device__ __forceinline__ int64_t stride() const { return nb; }
-    __device__ __forceinline__ int64_t out_row(int64_t r) const {
-        const int64_t s = s_lo + r / (B * Hkv), b = r / Hkv % B, h = r % Hkv;
-        return (b * S + s) * Hkv + h;
+    __device__ __forceinline__ int64_t out_row(uint32_t r) const {
+        const int bh = (int)(r % (uint32_t)(B * Hkv)), b = bh / Hkv;
+        return ((int64_t)b * S + query(r)) * Hkv + bh - b * Hkv;
     }
 };
+
 // The k largest of a row's n keys, held by one warp: key[j] of lane l is number 32 j + l (0 past n).
 template <int PER> __device__ __forceinline__ void topk_of_warp(const uint64_t (&key)[PER], int n, int k, int topk, int32_t *o) {
     const int lane = threadIdx.x % 32;
@@ -358,13 +374,13 @@ template <int PER> __device__ __forceinline__ void topk_of_warp(const uint64_t (
 
 template <int PER, typename Rows>
 __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, int32_t *out, int64_t rows, int topk, Rows of) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    const uint32_t r = blockIdx.x * 4 + threadIdx.x / 32;
     pdl_trigger();
     pdl_wait();
     if (r >= rows) return;
     const int lane = threadIdx.x % 32;
     const int n = (int)of.count(r), k = topk < n ? topk : n;
-    const uint64_t *row = keys + r * of.stride();
+    const uint64_t *row = keys + (int64_t)r * of.stride();
     uint64_t key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < n ? row[j * 32 + lane] : 0;
@@ -377,14 +393,14 @@ __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, in
 template <int PER, typename T>
 __global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *bounds, const float *scores, const float *q_norms, const float *block_norms,
                                                           int32_t *out, int64_t rows, int topk, int64_t H, int64_t D, RowsOfBlocks of) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    const uint32_t r = blockIdx.x * 4 + threadIdx.x / 32;
     pdl_trigger();
     pdl_wait();
     if (r >= rows) return;
-    const int lane = threadIdx.x % 32;
-    const int64_t s = of.s_lo + r / (of.B * of.Hkv), b = r / of.Hkv % of.B, h = r % of.Hkv, G = H / of.Hkv;
-    const int n = (int)of.count(r), k = topk < n ? topk : n, own = (int)(s / of.block);
-    const float *row = scores + r * of.nb;
+    const int lane = threadIdx.x % 32, bh = (int)(r % (uint32_t)(of.B * of.Hkv)), G = (int)H / of.Hkv;
+    const int64_t s = of.query(r), b = bh / of.Hkv, h = bh - b * of.Hkv;
+    const int own = (int)s / of.block, n = of.causal ? own + 1 : of.nb, k = topk < n ? topk : n;
+    const float *row = scores + (int64_t)r * of.nb;
     uint32_t key[PER];
     float size = 0.f;
     bool odd = false;
@@ -393,13 +409,13 @@ __global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *b
         const int i = j * 32 + lane;
         key[j] = 0;
         if (i < n) {
-            const float x = row[i], y = block_norms[(b * of.nb + i) * of.Hkv + h];
+            const float x = row[i], y = block_norms[(b * of.Hkv + h) * of.nb + i];
             key[j] = i == own ? 0xffffffffu : key32_of(x);
             size = fmaxf(size, y);
             odd |= !(fabsf(x) < INFINITY && y < INFINITY);
         }
     }
-    int32_t *o = out + of.out_row(r) * topk;
+    int32_t *o = out + ((b * of.S + s) * of.Hkv + h) * topk;
     uint32_t cut = 0;                       // taken: key >= cut
     bool close = false;
     if (k < n) {
@@ -458,7 +474,7 @@ __global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *b
                         double t = 0;
                         for (int d = lane; d < D; d += 32) {
                             double u = 0, w = 0;
-                            for (int64_t g = 0; g < G; ++g) {
+                            for (int g = 0; g < G; ++g) {
                                 const double y = (double)Elem<T>::to_f(q[((b * of.S + s) * H + h * G + g) * D + d]);
                                 if (y > 0) u += y; else w += y;
                             }
@@ -545,10 +561,10 @@ template <int THREADS> __device__ void topk_of_row(const uint64_t *row, int64_t 
 template <int THREADS, typename Rows>
 __global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *keys, int32_t *out, int topk, Rows of) {
     __shared__ int of_warp[32], tied_of[32];
-    const int64_t r = blockIdx.x;
+    const uint32_t r = blockIdx.x;
     pdl_trigger();
     pdl_wait();
-    topk_of_row<THREADS>(keys + r * of.stride(), of.count(r), topk, out + of.out_row(r) * topk, of_warp, tied_of);
+    topk_of_row<THREADS>(keys + (int64_t)r * of.stride(), of.count(r), topk, out + of.out_row(r) * topk, of_warp, tied_of);
 }
 
 // ---- the topk pages of a row: one CTA -------------------------------------------------------------------------------
@@ -561,7 +577,8 @@ __global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *key
 // same warps, and searched bit by bit.
 constexpr int kCandidates = 1024;
 
-template <typename T, int THREADS>
+// LP > 0: the CTA scores its row's pages itself first (rows enough to fill the GPU with one CTA each).
+template <typename T, int THREADS, int LP, int NV>
 __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
                                                                const int32_t *lengths, float2 *scores, int32_t *out, int topk, int *status) {
     constexpr int W = Vec16<T>::N;
@@ -591,6 +608,10 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
             if (y > 0) u += y; else w += y;
         }
         up[d] = u; down[d] = w;
+    }
+    if (LP > 0) {
+        score_pages<T, LP ? LP : 32, NV>(c, bounds, q + b * q_stride, H, Hkv, D, b, h, n, 0, THREADS / (LP ? LP : 32), scores + row * c.width, status);
+        __syncthreads();
     }
     const float2 *mine = scores + row * c.width;
     float best = -INFINITY, size = 0.f;
@@ -764,14 +785,14 @@ int select_in_fp32(const T *q, const T *bounds, int64_t B, int64_t S, int64_t H,
                    int32_t *blocks, char *ws, const SelectPlan &p, cudaStream_t s) {
     float *norms = (float *)(ws + p.norms), *q_norms = (float *)(ws + p.q_norms), *scores = (float *)(ws + p.scores);
     const int64_t all = B * p.nb * Hkv;
-    cudaError_t e = launch_after(block_norms_kernel<T>, dim3((unsigned)((all + 3) / 4)), dim3(128), 0, s, bounds, norms, all, Hkv, D);
+    cudaError_t e = launch_after(block_norms_kernel<T>, dim3((unsigned)((all + 3) / 4)), dim3(128), 0, s, bounds, norms, all, p.nb, Hkv, D);
     for (int64_t s0 = 0; s0 < S && e == cudaSuccess; s0 += p.step) {
         const int64_t s1 = s0 + p.step < S ? s0 + p.step : S, seen = causal ? (s1 - 1) / block + 1 : p.nb, rows = (s1 - s0) * B * Hkv;
         const dim3 grid((unsigned)((seen + 63) / 64), (unsigned)((s1 - s0 + 63) / 64), (unsigned)(B * Hkv));
         e = D <= 64 ? launch_scores_mma<T, 64>(grid, s, q, bounds, scores, q_norms, S, H, Hkv, D, p.nb, (int)block, causal, s0, s1)
                     : launch_scores_mma<T, 128>(grid, s, q, bounds, scores, q_norms, S, H, Hkv, D, p.nb, (int)block, causal, s0, s1);
         if (e != cudaSuccess) break;
-        const RowsOfBlocks of{B, S, Hkv, p.nb, s0, (int)block, causal};
+        const RowsOfBlocks of{(int)B, (int)S, (int)Hkv, (int)p.nb, (int)s0, (int)block, causal};
         const dim3 ctas((unsigned)((rows + 3) / 4));
 #define SELECT_ROWS(PER) e = launch_after(select_rows_kernel<PER, T>, ctas, dim3(128), 0, s, q, bounds, scores, q_norms, norms, blocks, rows, (int)topk, H, D, of)
         if (seen <= 128) SELECT_ROWS(4);
@@ -804,7 +825,7 @@ int run_select_blocks(const T *q, const T *k, int64_t B, int64_t S, int64_t H, i
         dim3 grid((unsigned)((seen + 63) / 64), (unsigned)((s1 - s0 + 63) / 64), (unsigned)(B * Hkv));
         e = launch_after(block_scores_kernel<T>, grid, dim3(256), 0, s, q, (const T *)bounds, keys, S, H, Hkv, D, p.nb, (int)block, causal, s0, s1);
         if (e != cudaSuccess) return cuda_fail(e, "launching the block scores");
-        RowsOfBlocks of{B, S, Hkv, p.nb, s0, (int)block, causal};
+        RowsOfBlocks of{(int)B, (int)S, (int)Hkv, (int)p.nb, (int)s0, (int)block, causal};
         if (int rc = launch_topk(keys, blocks, (s1 - s0) * B * Hkv, seen, topk, of, s)) return rc;
     }
     return MAT_OK;
@@ -824,6 +845,19 @@ int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, i
     const int vecs = 2 * (int)c->D / Vec16<T>::N;            // of one page and head
     const int lp = vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
     const T *bounds = (const T *)c->key_bounds;
+    const dim3 rows((unsigned)c->H_kv, (unsigned)B);
+    cudaError_t e;
+    if (B * c->H_kv >= 148) {
+#define SELECT_PAGES(LP, NV) select_pages_kernel<T, 512, LP, NV><<<rows, 512, 0, s>>>(v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status)
+        if (lp == 8) SELECT_PAGES(8, 1);
+        else if (lp == 16) SELECT_PAGES(16, 1);
+        else if (vecs <= 32) SELECT_PAGES(32, 1);
+        else if (vecs <= 64) SELECT_PAGES(32, 2);
+        else SELECT_PAGES(32, 4);
+#undef SELECT_PAGES
+        e = cudaGetLastError();
+        return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the selection");
+    }
     int64_t gx = (v.width * lp + 4 * 256 - 1) / (4 * 256);
     const int64_t cap = 148 * 8 / (B * c->H_kv) + 1;         // enough CTAs to fill the GPU; each walks several pages
     if (gx > cap) gx = cap;
@@ -835,12 +869,11 @@ int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, i
     else if (vecs <= 64) PAGE_SCORES(32, 2);
     else PAGE_SCORES(32, 4);
 #undef PAGE_SCORES
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "launching the page scores");
-    const dim3 rows((unsigned)c->H_kv, (unsigned)B);
     // few pages per row: a small CTA, whose steps wait for fewer warps
-    if (v.width <= 2048 && topk <= 128) e = launch_after(select_pages_kernel<T, 256>, rows, dim3(256), 0, s, v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status);
-    else e = launch_after(select_pages_kernel<T, 1024>, rows, dim3(1024), 0, s, v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status);
+    if (v.width <= 2048 && topk <= 128) e = launch_after(select_pages_kernel<T, 256, 0, 1>, rows, dim3(256), 0, s, v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status);
+    else e = launch_after(select_pages_kernel<T, 1024, 0, 1>, rows, dim3(1024), 0, s, v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the selection");
 }
 

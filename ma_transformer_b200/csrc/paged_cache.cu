@@ -141,8 +141,8 @@ template <int W> __device__ __forceinline__ void turn(float *x, const float *c, 
     }
 }
 
-template <typename T, bool VEC> __global__ void __launch_bounds__(256, 3) append_rows_kernel(const AppendArgs a) {
-    constexpr int W = VEC ? Vec16<T>::N : 1, U = 4;
+template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) append_rows_kernel(const AppendArgs a) {
+    constexpr int W = VEC ? Vec16<T>::N : 1, U = 2;
     __shared__ int starts[kKnownStarts + 1];
     __shared__ int pos_of[64];
     __shared__ int64_t k_of[64], v_of[64];
@@ -194,77 +194,69 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 3) append
         angle_of((double)pos_of[t], a.inv_freq[i - t * half], cosines[i], sines[i]);
     }
     __syncthreads();
-    const int units = (D + 2 * W - 1) / (2 * W), heads_q = a.q ? (int)a.H : 0, heads_k = (int)a.Hkv, roles = heads_q + 2 * heads_k;
-    const int total = cnt * roles * units;
-    for (int i0 = tid; i0 < total; i0 += 256 * U) {
-        uint4 raw[U][2];
-        T *dst[U];
-        int tok[U], un[U];
-        bool turned[U];
+    // a thread keeps its head and columns and walks over the tokens: 256 (head, unit) pairs at a time, several tokens
+    // side by side where there are fewer
+    const int units = (D + 2 * W - 1) / (2 * W), heads_q = a.q ? (int)a.H : 0, heads_k = (int)a.Hkv, pairs = (heads_q + 2 * heads_k) * units;
+    for (int p0 = 0; p0 < pairs; p0 += 256) {
+        const int width = pairs - p0 < 256 ? pairs - p0 : 256, lanes = 256 / width, lane = tid / width;
+        if (lane >= lanes) continue;
+        const int at = p0 + tid - lane * width, role = at / units;
+        const Unit<W> u(at - role * units, a.rot, a.interleaved);
+        const bool is_q = role < heads_q, is_v = role >= heads_q + heads_k, second = u.at1 < D;
+        const int h = is_q ? role : is_v ? role - heads_q - heads_k : role - heads_q;
+        const bool turned = u.pair >= 0 && !is_v;
+        const int64_t src_tok = is_q ? a.q_tok : is_v ? a.vn_tok : a.kn_tok;
+        const T *src = (const T *)(is_q ? a.q : is_v ? a.vn : a.kn) + n0 * src_tok + (int64_t)h * D;
+        T *dst = is_q ? (T *)a.qo + (n0 * a.H + h) * D : is_v ? (T *)a.c.v + h * a.c.v_head : (T *)a.c.k + h * a.c.k_head;
+        for (int t0 = lane; t0 < cnt; t0 += lanes * U) {
+            uint4 raw[U][2];
+            int64_t to[U];
 #pragma unroll
-        for (int y = 0; y < U; ++y) {
-            const int i = i0 + y * 256;
-            dst[y] = nullptr;
-            if (i >= total) continue;
-            const int rest = i / units;
-            un[y] = i - rest * units;
-            tok[y] = rest / roles;
-            const int role = rest - tok[y] * roles;
-            const int64_t n = n0 + tok[y];
-            const T *src;
-            if (role < heads_q) {
-                src = (const T *)a.q + n * a.q_tok + (int64_t)role * D;
-                if (pos_of[tok[y]] >= 0) dst[y] = (T *)a.qo + (n * a.H + role) * D;
-            } else if (role < heads_q + heads_k) {
-                const int h = role - heads_q;
-                src = (const T *)a.kn + n * a.kn_tok + (int64_t)h * D;
-                if (k_of[tok[y]] >= 0) dst[y] = (T *)a.c.k + k_of[tok[y]] + h * a.c.k_head;
-            } else {
-                const int h = role - heads_q - heads_k;
-                src = (const T *)a.vn + n * a.vn_tok + (int64_t)h * D;
-                if (v_of[tok[y]] >= 0) dst[y] = (T *)a.c.v + v_of[tok[y]] + h * a.c.v_head;
-            }
-            const Unit<W> u(un[y], a.rot, a.interleaved);
-            turned[y] = u.pair >= 0 && role < heads_q + heads_k;
-            // values have no pairs: their vectors are moved where the rotation's halves lie all the same
-            if (!dst[y]) continue;
-            if (VEC) {
-                raw[y][0] = *reinterpret_cast<const uint4 *>(src + u.at0);
-                if (u.at1 < D) raw[y][1] = *reinterpret_cast<const uint4 *>(src + u.at1);
-            } else {
-                raw[y][0].x = __float_as_uint(Elem<T>::to_f(src[u.at0]));
-                raw[y][1].x = __float_as_uint(Elem<T>::to_f(src[u.at1]));
-            }
-        }
-#pragma unroll
-        for (int y = 0; y < U; ++y) {
-            if (!dst[y]) continue;
-            const Unit<W> u(un[y], a.rot, a.interleaved);
-            if (turned[y]) {
-                float x[2 * W];
-                const float *c = cosines + tok[y] * half + u.pair, *s = sines + tok[y] * half + u.pair;
+            for (int y = 0; y < U; ++y) {
+                const int t = t0 + y * lanes;
+                to[y] = t >= cnt || pos_of[t] < 0 ? -1 : is_q ? t * a.H * D : is_v ? v_of[t] : k_of[t];
+                if (to[y] < 0) continue;
+                const T *from = src + t * src_tok;
                 if (VEC) {
-                    Vec16<T>::unpack(raw[y][0], x);
-                    Vec16<T>::unpack(raw[y][1], x + W);
+                    raw[y][0] = *reinterpret_cast<const uint4 *>(from + u.at0);
+                    if (second) raw[y][1] = *reinterpret_cast<const uint4 *>(from + u.at1);
                 } else {
-                    x[0] = __uint_as_float(raw[y][0].x);
-                    x[W] = __uint_as_float(raw[y][1].x);
-                }
-                turn<W>(x, c, s, a.interleaved);
-                if (VEC) {
-                    raw[y][0] = Vec16<T>::pack(x);
-                    raw[y][1] = Vec16<T>::pack(x + W);
-                } else {
-                    raw[y][0].x = __float_as_uint(x[0]);
-                    raw[y][1].x = __float_as_uint(x[W]);
+                    raw[y][0].x = __float_as_uint(Elem<T>::to_f(from[u.at0]));
+                    raw[y][1].x = __float_as_uint(Elem<T>::to_f(from[u.at1]));
                 }
             }
-            if (VEC) {
-                *reinterpret_cast<uint4 *>(dst[y] + u.at0) = raw[y][0];
-                if (u.at1 < D) *reinterpret_cast<uint4 *>(dst[y] + u.at1) = raw[y][1];
-            } else {
-                dst[y][u.at0] = Elem<T>::from_f(__uint_as_float(raw[y][0].x));
-                dst[y][u.at1] = Elem<T>::from_f(__uint_as_float(raw[y][1].x));
+#pragma unroll
+            for (int y = 0; y < U; ++y) {
+                if (to[y] < 0) continue;
+                T *out = dst + to[y];
+                if (turned) {
+                    float x[2 * W], c[W], s[W];
+                    const int first = (t0 + y * lanes) * half + u.pair;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) { c[i] = cosines[first + i]; s[i] = sines[first + i]; }
+                    if (VEC) {
+                        Vec16<T>::unpack(raw[y][0], x);
+                        Vec16<T>::unpack(raw[y][1], x + W);
+                    } else {
+                        x[0] = __uint_as_float(raw[y][0].x);
+                        x[W] = __uint_as_float(raw[y][1].x);
+                    }
+                    turn<W>(x, c, s, a.interleaved);
+                    if (VEC) {
+                        raw[y][0] = Vec16<T>::pack(x);
+                        raw[y][1] = Vec16<T>::pack(x + W);
+                    } else {
+                        raw[y][0].x = __float_as_uint(x[0]);
+                        raw[y][1].x = __float_as_uint(x[W]);
+                    }
+                }
+                if (VEC) {
+                    *reinterpret_cast<uint4 *>(out + u.at0) = raw[y][0];
+                    if (second) *reinterpret_cast<uint4 *>(out + u.at1) = raw[y][1];
+                } else {
+                    out[u.at0] = Elem<T>::from_f(__uint_as_float(raw[y][0].x));
+                    out[u.at1] = Elem<T>::from_f(__uint_as_float(raw[y][1].x));
+                }
             }
         }
     }
@@ -358,7 +350,7 @@ template <typename T> __global__ void __launch_bounds__(128) page_bounds_kernel(
 template <typename T> int launch_append(AppendArgs &a, bool vec, cudaStream_t stream) {
     // enough tiles to fill the GPU, few enough that a tile's look-ups are shared: 1 to 64 tokens, 32 KB of angles
     a.tile = 1;
-    while (a.tile < 64 && a.tile * 148 * 4 < a.N && (a.tile * 2) * a.rot * 4 <= 32768) a.tile *= 2;
+    while (a.tile < 64 && a.tile * 148 * 8 < a.N && (a.tile * 2) * a.rot * 4 <= 32768) a.tile *= 2;
     const unsigned tiles = (unsigned)((a.N + a.tile - 1) / a.tile);
     const size_t smem = (size_t)a.tile * a.rot * sizeof(float);
     if (vec) append_rows_kernel<T, true><<<tiles, 256, smem, stream>>>(a);

@@ -29,7 +29,7 @@ struct DecodeArgs {
     const int32_t *pages;
     int64_t n_sel;
     float scale_log2;
-    int nsplit, min_chunk, tiles;   // tiles: groups of query heads per key head
+    int G, nsplit, min_chunk, tiles;   // tiles: groups of query heads per key head
     int aligned;                    // the kernel reads 16 neighbouring positions at a time: first is a multiple of 16
     float2 *stats;                  // [B, H, nsplit] (maximum, sum)
     float *part;                    // [B, H, nsplit, D]
@@ -53,7 +53,7 @@ struct RowTokens {
             n = len;
         } else {
             dil = a.dilation;
-            const int64_t back = (len - 1) / dil;
+            const int64_t back = dil == 1 ? len - 1 : (len - 1) / dil;
             n = (a.left < back ? a.left : back) + 1;
             first = lo = len - 1 - (n - 1) * dil;
             if (a.aligned) {
@@ -64,8 +64,8 @@ struct RowTokens {
     }
     // tokens per chunk; rows of up to c tokens are one chunk
     __device__ __forceinline__ int64_t chunk(const DecodeArgs &a) const {
-        const int64_t c = ((n + a.nsplit - 1) / a.nsplit + 63) / 64 * 64;
-        return c > a.min_chunk ? c : a.min_chunk;
+        if (n <= (int64_t)a.min_chunk * a.nsplit) return a.min_chunk;     // no division in the common case
+        return ((n + a.nsplit - 1) / a.nsplit + 63) / 64 * 64;
     }
     // position of virtual token t, or -1
     __device__ __forceinline__ int64_t position(const DecodeArgs &a, int64_t t) const {
@@ -82,8 +82,8 @@ struct RowTokens {
 template <typename T, int LPK, int NV, int GT, int U>
 __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     constexpr int W = Vec16<T>::N, KPW = 32 / LPK, C = NV * W;
-    const int64_t b = blockIdx.z, h = blockIdx.y / a.tiles, g0 = (int64_t)(blockIdx.y % a.tiles) * GT;
-    const int64_t G = a.H / a.Hkv;
+    const int64_t b = blockIdx.z, h = blockIdx.y / (unsigned)a.tiles, g0 = (int64_t)(blockIdx.y % (unsigned)a.tiles) * GT;
+    const int64_t G = a.G;
     const int D = (int)a.D;
     pdl_trigger();
     const RowTokens row(a, b, h);
@@ -232,8 +232,8 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) 
 
 template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) decode_mma_kernel(const DecodeArgs a) {
     constexpr int PITCH = DP + 8, TILE = 16 * PITCH, CH = DP / 8;
-    const int64_t b = blockIdx.z, h = blockIdx.y / a.tiles, G = a.H / a.Hkv;
-    const int g0 = (blockIdx.y % a.tiles) * 16, heads = min(16, (int)G - g0);
+    const int64_t b = blockIdx.z, h = blockIdx.y / (unsigned)a.tiles, G = a.G;
+    const int g0 = (int)(blockIdx.y % (unsigned)a.tiles) * 16, heads = min(16, (int)G - g0);
     const int D = (int)a.D;
     pdl_trigger();
     const RowTokens row(a, b, h);
@@ -421,7 +421,7 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
 template <typename T> __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a) {
     __shared__ float4 acc[256];
     __shared__ float red[8], weight[256];
-    const int64_t b = blockIdx.y, head = b * a.H + blockIdx.x, h = blockIdx.x / (a.H / a.Hkv);
+    const int64_t b = blockIdx.y, head = b * a.H + blockIdx.x, h = blockIdx.x / (unsigned)a.G;
     const int tid = threadIdx.x, D = (int)a.D, vecs = D / 4, lanes = 256 / vecs, v = tid % vecs, k = tid / vecs;
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a);
@@ -591,6 +591,7 @@ extern "C" int mat_paged_decode(const mat_paged_cache *cache, const void *q, int
     a.c = paged_view(cache, page_table, table_width, table_stride);
     a.q = q; a.o = o; a.q_stride = q_stride;
     a.B = B; a.H = H; a.Hkv = cache->H_kv; a.D = cache->D;
+    a.G = (int)(H / cache->H_kv);
     a.lengths = lengths; a.left = left; a.dilation = dilation;
     a.pages = pages; a.n_sel = n_sel;
     a.scale_log2 = (scale > 0.f ? scale : 1.0f / std::sqrt((float)cache->D)) * 1.4426950408889634f;

@@ -40,6 +40,7 @@ template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const
     const int limit = i < p.S ? own_limit(p, i) : 0;
     if (i < p.S) {
         int prev = -1;
+#pragma unroll 8
         for (int s = 0; s < p.topk; ++s) {
             const int n = row[s];
             if (sel_entry_counts(n, prev, limit) && n >= n0 && n < n1) atomicOr(&mask[n - n0][tid / 32], 1u << (tid % 32));
@@ -55,12 +56,24 @@ template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const
         }
     } else if (i < p.S) {
         int prev = -1;
-        for (int s = 0; s < p.topk; ++s) {
-            const int n = row[s];
-            if (!sel_entry_counts(n, prev, limit) || n < n0 || n >= n1) continue;
-            int rank = __popc(mask[n - n0][tid / 32] & ((1u << (tid % 32)) - 1));
-            for (int w = 0; w < tid / 32; ++w) rank += __popc(mask[n - n0][w]);
-            l.entry[bh * p.S * p.topk + l.base[bh * (p.nb + 1) + n] + l.counts[(bh * p.nb + n) * l.tiles + tile] + rank] = (int32_t)(i * p.topk + s);
+        int32_t *entries = l.entry + bh * p.S * p.topk;
+        for (int s0 = 0; s0 < p.topk; s0 += 8) {       // eight entries' offsets in flight
+            int n[8], at[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) n[y] = s0 + y < p.topk ? row[s0 + y] : -1;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                if (!sel_entry_counts(n[y], prev, limit) || n[y] < n0 || n[y] >= n1) n[y] = -1;
+                at[y] = n[y] < 0 ? 0 : l.base[bh * (p.nb + 1) + n[y]] + l.counts[(bh * p.nb + n[y]) * l.tiles + tile];
+            }
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                if (n[y] < 0) continue;
+                const uint32_t *m = mask[n[y] - n0];
+                int rank = __popc(m[tid / 32] & ((1u << (tid % 32)) - 1));
+                for (int w = 0; w < tid / 32; ++w) rank += __popc(m[w]);
+                entries[at[y] + rank] = (int32_t)(i * p.topk + s0 + y);
+            }
         }
     }
 }

@@ -60,11 +60,12 @@ __device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_str
 // EXACT: D == DP and a block is a whole number of NKP keys, known to the compiler.
 template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, DP == 64 ? 4 : 3) sel_fwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8;
-    const int64_t bh = t.bh0 + blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
+    const int bh = (int)t.bh0 + blockIdx.y;
+    const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
     if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
-    const int2 item = t.items[bh * t.max_items + blockIdx.x];
+    const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
     const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n];
     const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
     const int r_end = min(item.y + kFwdRows, rows_all);
@@ -87,7 +88,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
         const int r = item.y + x;
         int i = -1, src = 0, at = 0;
         if (r < r_end) {
-            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bh * p.S * T_ + e0 + e];
+            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[(int64_t)bh * p.S * T_ + e0 + e];
             i = entry / T_;
             src = i * (int)p.H + g;
             at = (i * t.G + g) * T_ + entry - i * T_;
@@ -261,18 +262,20 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
 // Joins a row's partials in the order of its list: LPR lanes of 4 columns per row.  The lanes first look at LPR entries
 // of the list together (which count, and with what weight), then read the partials of those that do, four at a time.
 // BWD: the sum of a row's shares of dq.
-template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t, int64_t rows) {
-    const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;     // (bh of the group, i, g)
+template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t) {
+    const uint32_t x0 = (blockIdx.x * 128u + threadIdx.x) / LPR, G = t.G;                       // (i, g) of the pair
     const int lane = threadIdx.x % LPR, col = lane * 4, D = (int)p.D, T_ = (int)p.topk;
     pdl_trigger();
     pdl_wait();
-    const bool live = r < rows, in = live && col < D;
-    const int64_t rr = live ? r : 0;
-    const int g = (int)(rr % t.G);
-    const int64_t i = rr / t.G % p.S, bh = t.bh0 + rr / t.G / p.S, b = bh / p.Hkv, h = bh % p.Hkv;
-    const int32_t *list = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
-    const int limit = p.causal ? (int)(i / p.block) + 1 : (int)p.nb;
-    const int64_t out = ((b * p.S + i) * p.H + h * t.G + g);
+    const bool live = x0 < (uint32_t)p.S * G, in = live && col < D;
+    const uint32_t x = live ? x0 : 0;
+    const int i = (int)(x / G), g = (int)(x - i * G);
+    const int bh = (int)t.bh0 + blockIdx.y;
+    const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
+    const int64_t rr = (int64_t)blockIdx.y * p.S * G + x;                                       // among the group's rows
+    const int32_t *list = p.blocks + ((b * p.S + i) * p.Hkv + h) * T_;
+    const int limit = p.causal ? i / (int)p.block + 1 : (int)p.nb;
+    const int64_t out = ((b * p.S + i) * p.H + h * G + g);
     const float *part = t.part + rr * T_ * t.nsub * D + col;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
@@ -338,11 +341,13 @@ template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) 
 // and half of the columns (NKP = 32).
 template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, 2) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW, NBUF = DP == 64 ? 2 : 1;
-    const int64_t bhl = blockIdx.z, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
+    const int64_t bhl = blockIdx.z;
+    const int bh = (int)t.bh0 + blockIdx.z;
+    const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
     if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
-    const int2 item = t.items[bh * t.max_items + blockIdx.x];
+    const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
     const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n], sub = blockIdx.y;
     const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
     const int r_end = min(item.y + kBwdRows, rows_all);
@@ -366,7 +371,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
         int i = -1, at = 0, src = 0;
         float lse = 0.f, delta = 0.f;
         if (r < r_end) {
-            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bh * p.S * T_ + e0 + e];
+            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[(int64_t)bh * p.S * T_ + e0 + e];
             i = entry / T_;
             at = (i * t.G + g) * T_ + entry - i * T_;
             src = i * (int)p.H + g;
@@ -531,7 +536,9 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
 
 // dk and dv of a (sub-)block: the sum of its items' shares in order; zeros for a block that nobody chose
 template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(const SelProblem p, const SelTile t) {
-    const int64_t bhl = blockIdx.y, bh = t.bh0 + bhl, b = bh / p.Hkv, h = bh % p.Hkv;
+    const int64_t bhl = blockIdx.y;
+    const int bh = (int)t.bh0 + blockIdx.y;
+    const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
     const int n = blockIdx.x / t.nsub, sub = blockIdx.x % t.nsub, D = (int)p.D;
@@ -632,10 +639,10 @@ template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, 
     const size_t smem = ((p.block + NKP - 1) / NKP * NKP * 2 + 4 * 2 * 16) * (DP + 8) * sizeof(T);
     if (int rc = ensure_dynamic_smem((const void *)sel_fwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention")) return rc;
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
-        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
+        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = p.S * t.G;
         launch_after(sel_fwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)n), dim3(128), smem, p.stream, p, t);
-        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, false>, dim3((unsigned)((rows * 16 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
-        else launch_after(sel_join_kernel<T, 32, false>, dim3((unsigned)((rows * 32 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
+        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, false>, dim3((unsigned)((rows + 128 / 16 - 1) / (128 / 16)), (unsigned)n), dim3(128), 0, p.stream, p, t);
+        else launch_after(sel_join_kernel<T, 32, false>, dim3((unsigned)((rows + 128 / 32 - 1) / (128 / 32)), (unsigned)n), dim3(128), 0, p.stream, p, t);
     }
     return launched("launching the selected attention");
 }
@@ -648,10 +655,10 @@ template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, 
     if (p.D <= 64) launch_after(sel_delta_kernel<T, 8>, dim3((unsigned)((all * 8 + 127) / 128)), dim3(128), 0, p.stream, (const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
     else launch_after(sel_delta_kernel<T, 16>, dim3((unsigned)((all * 16 + 127) / 128)), dim3(128), 0, p.stream, (const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
-        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = n * p.S * t.G;
+        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = p.S * t.G;
         launch_after(sel_bwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), dim3(128), smem, p.stream, p, t);
-        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, true>, dim3((unsigned)((rows * 16 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
-        else launch_after(sel_join_kernel<T, 32, true>, dim3((unsigned)((rows * 32 + 127) / 128)), dim3(128), 0, p.stream, p, t, rows);
+        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, true>, dim3((unsigned)((rows + 128 / 16 - 1) / (128 / 16)), (unsigned)n), dim3(128), 0, p.stream, p, t);
+        else launch_after(sel_join_kernel<T, 32, true>, dim3((unsigned)((rows + 128 / 32 - 1) / (128 / 32)), (unsigned)n), dim3(128), 0, p.stream, p, t);
         launch_after(sel_kv_join_kernel<T>, dim3((unsigned)(p.nb * w.nsub), (unsigned)n, (unsigned)((64 * p.D / 4 + 127) / 128)), dim3(128), 0, p.stream, p, t);
     }
     return launched("launching the selected attention's backward");
