@@ -1,5 +1,5 @@
-// Attention over selected blocks of keys and its gradients: the C entry points, the lists of the queries that chose a
-// block, and the kernels that serve every type and width: one warp per row with fp32 arithmetic.
+// Attention over selected blocks of keys and its gradients: the C entry points and the lists of the queries that chose a
+// block.  The tiles are in selected_tiles.cu.
 //
 //   forward   o_i = sum_j p_ij v_j, p_ij = exp(scale q_i . k_j - lse_i) over the keys j of the query's blocks
 //   backward  delta_i = do_i . o_i, ds_ij = p_ij (do_i . v_j - delta_i),
@@ -147,159 +147,9 @@ __global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb
     }
 }
 
-// ---- one warp per row -----------------------------------------------------------------------------------------------
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
-}
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-    return x;
-}
-
-// dot of a row in shared memory (fp32) with a row of elements
-template <typename T> __device__ __forceinline__ float dot_row(const float *a, const T *x, int D) {
-    constexpr int W = Vec16<T>::N;
-    float s = 0.f;
-    for (int d = 0; d < D; d += W) {
-        float y[W];
-        Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(x + d)), y);
-#pragma unroll
-        for (int j = 0; j < W; ++j) s = fmaf(a[d + j], y[j], s);
-    }
-    return s;
-}
-
-// BWD false: o and lse of row (b, i, head).  BWD true: dq of the row; delta is left in delta_out for the key pass.
-template <typename T, bool BWD> __global__ void __launch_bounds__(128) sel_rows_kernel(const SelProblem p, float *delta_out) {
-    __shared__ float qs[4][128], ds_row[4][128];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, D = (int)p.D;
-    const int64_t r = (int64_t)blockIdx.x * 4 + warp;       // (b, i, head)
-    if (r >= p.B * p.S * p.H) return;
-    const int64_t head = r % p.H, i = r / p.H % p.S, b = r / p.H / p.S, h = head / (p.H / p.Hkv);
-    float delta = 0.f;
-    for (int d = lane; d < D; d += 32) {
-        qs[warp][d] = Elem<T>::to_f(((const T *)p.q)[r * D + d]);
-        if (BWD) {
-            const float g = Elem<T>::to_f(((const T *)p.dout)[r * D + d]);
-            ds_row[warp][d] = g;
-            delta = fmaf(g, Elem<T>::to_f(((const T *)p.o)[r * D + d]), delta);
-        }
-    }
-    __syncwarp();
-    const float lse = BWD ? p.lse_in[r] : 0.f;
-    if (BWD) {
-        delta = warp_sum(delta);
-        if (lane == 0) delta_out[r] = delta;
-    }
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int32_t *list = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
-    const int limit = p.causal ? (int)(i / p.block) + 1 : (int)p.nb;
-    int prev = -1;
-    for (int s = 0; s < p.topk; ++s) {
-        const int n = list[s];
-        if (!sel_entry_counts(n, prev, limit)) continue;
-        const int64_t j0 = n * p.block;
-        int64_t j1 = j0 + p.block < p.S ? j0 + p.block : p.S;
-        if (p.causal && j1 > i + 1) j1 = i + 1;
-        for (int64_t base = j0; base < j1; base += 32) {
-            const int64_t j = base + lane;
-            const bool in = j < j1;
-            const int64_t at = ((b * p.S + (in ? j : j0)) * p.Hkv + h) * D;
-            const float x = dot_row<T>(qs[warp], (const T *)p.k + at, D) * p.scale;
-            float w;     // the weight of this lane's key in the sum below
-            if (BWD) {
-                const float dp = dot_row<T>(ds_row[warp], (const T *)p.v + at, D);
-                w = in && lse != -INFINITY ? expf(x - lse) * (dp - delta) : 0.f;
-            } else {
-                const float top = fmaxf(m, warp_max(in ? x : -INFINITY)), ref = top == -INFINITY ? 0.f : top;
-                const float keep = expf(m - ref);
-                w = in ? expf(x - ref) : 0.f;
-                m = top;
-                l = l * keep + warp_sum(w);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] *= keep;
-            }
-            const int64_t row0 = ((b * p.S + base) * p.Hkv + h) * D;
-            const int cnt = (int)(j1 - base < 32 ? j1 - base : 32);
-            const T *src = (const T *)(BWD ? p.k : p.v) + row0;
-            for (int t = 0; t < cnt; ++t) {
-                const float wt = __shfl_sync(0xffffffffu, w, t);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c * 32 + lane < D) acc[c] = fmaf(wt, Elem<T>::to_f(src[t * p.Hkv * D + c * 32 + lane]), acc[c]);
-            }
-        }
-    }
-    T *out = (T *)(BWD ? p.dq : p.out) + r * D;
-    const float f = BWD ? p.scale : (l == 0.f ? 0.f : 1.f / l);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (c * 32 + lane < D) out[c * 32 + lane] = Elem<T>::from_f(l == 0.f && !BWD ? 0.f : acc[c] * f);
-    if (!BWD && lane == 0) p.lse[r] = l == 0.f ? -INFINITY : m + logf(l);
-}
-
-// dk and dv of one key: one warp, lanes over columns
-template <typename T> __global__ void __launch_bounds__(128) sel_keys_kernel(const SelProblem p, const SelLists l, const float *delta) {
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, D = (int)p.D, G = (int)(p.H / p.Hkv);
-    const int64_t r = (int64_t)blockIdx.x * 4 + warp;       // (b, j, h)
-    if (r >= p.B * p.S * p.Hkv) return;
-    const int64_t h = r % p.Hkv, j = r / p.Hkv % p.S, b = r / p.Hkv / p.S, bh = b * p.Hkv + h, n = j / p.block;
-    float k[4], v[4], dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const bool in = c * 32 + lane < D;
-        k[c] = in ? Elem<T>::to_f(((const T *)p.k)[r * D + c * 32 + lane]) : 0.f;
-        v[c] = in ? Elem<T>::to_f(((const T *)p.v)[r * D + c * 32 + lane]) : 0.f;
-    }
-    const int32_t *list = l.entry + bh * p.S * p.topk;
-    for (int e = l.base[bh * (p.nb + 1) + n]; e < l.base[bh * (p.nb + 1) + n + 1]; ++e) {
-        const int64_t i = list[e] / p.topk;
-        if (p.causal && i < j) continue;
-        for (int g = 0; g < G; ++g) {
-            const int64_t row = (b * p.S + i) * p.H + h * G + g;
-            float q[4], o[4], x = 0.f, dp = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const bool in = c * 32 + lane < D;
-                q[c] = in ? Elem<T>::to_f(((const T *)p.q)[row * D + c * 32 + lane]) : 0.f;
-                o[c] = in ? Elem<T>::to_f(((const T *)p.dout)[row * D + c * 32 + lane]) : 0.f;
-                x = fmaf(q[c], k[c], x);
-                dp = fmaf(o[c], v[c], dp);
-            }
-            x = warp_sum(x) * p.scale;
-            dp = warp_sum(dp);
-            const float w = expf(x - p.lse_in[row]), d = w * (dp - delta[row]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) { dv[c] = fmaf(w, o[c], dv[c]); dk[c] = fmaf(d, q[c], dk[c]); }
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (c * 32 + lane < D) {
-            ((T *)p.dk)[r * D + c * 32 + lane] = Elem<T>::from_f(dk[c] * p.scale);
-            ((T *)p.dv)[r * D + c * 32 + lane] = Elem<T>::from_f(dv[c]);
-        }
-}
-
 int launched(const char *what) {
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, what);
-}
-
-template <typename T> int run_fwd(const SelProblem &p) {
-    sel_rows_kernel<T, false><<<(unsigned)((p.B * p.S * p.H + 3) / 4), 128, 0, p.stream>>>(p, nullptr);
-    return launched("launching the selected attention");
-}
-
-template <typename T> int run_bwd(const SelProblem &p, const SelLists &l, float *delta) {
-    if (int rc = launch_sel_lists(p, l, nullptr, nullptr, 0, 1)) return rc;
-    sel_rows_kernel<T, true><<<(unsigned)((p.B * p.S * p.H + 3) / 4), 128, 0, p.stream>>>(p, delta);
-    if (int rc = launched("launching the selected attention's query gradient")) return rc;
-    sel_keys_kernel<T><<<(unsigned)((p.B * p.S * p.Hkv + 3) / 4), 128, 0, p.stream>>>(p, l, delta);
-    return launched("launching the selected attention's key gradients");
 }
 
 int check_selected(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t block, int64_t topk) {
@@ -349,9 +199,13 @@ int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_
 
 using namespace mat;
 
+static int have_workspace(size_t need, const void *workspace, size_t bytes) {
+    if (workspace && bytes >= need && (uintptr_t)workspace % 256 == 0) return MAT_OK;
+    return fail(MAT_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace ? bytes : (size_t)0);
+}
+
 extern "C" size_t mat_selected_attn_fwd_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype, int64_t block, int64_t topk) {
-    if (check_selected(B, S, H, H_kv, D, dtype, block, topk) || dtype == MAT_F32) return 0;
-    return sel_mma_workspace_bytes(B, S, H, H_kv, D, block, topk, false);
+    return check_selected(B, S, H, H_kv, D, dtype, block, topk) ? 0 : sel_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk, false);
 }
 
 extern "C" int mat_selected_attn_fwd(const void *q, const void *k, const void *v, void *o, float *lse, int64_t B, int64_t S, int64_t H,
@@ -366,17 +220,13 @@ extern "C" int mat_selected_attn_fwd(const void *q, const void *k, const void *v
     p.blocks = blocks; p.block = block; p.topk = topk; p.nb = (S + block - 1) / block; p.causal = causal != 0;
     p.scale = scale > 0.f ? scale : 1.0f / std::sqrt((float)D);
     p.stream = (cudaStream_t)stream;
-    const size_t need = mat_selected_attn_fwd_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk);
-    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
-        return fail(MAT_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace ? workspace_bytes : (size_t)0);
-    note_kernel(dtype == MAT_F32 ? "selected_rows" : "selected_mma");
-    return dtype == MAT_F32 ? run_fwd<float>(p) : launch_sel_mma(p, workspace, false);
+    if (int rc = have_workspace(sel_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk, false), workspace, workspace_bytes)) return rc;
+    note_kernel(dtype == MAT_F32 ? "selected_f32" : "selected_mma");
+    return launch_sel(p, workspace, false);
 }
 
 extern "C" size_t mat_selected_attn_bwd_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype, int64_t block, int64_t topk) {
-    if (check_selected(B, S, H, H_kv, D, dtype, block, topk)) return 0;
-    if (dtype != MAT_F32) return sel_mma_workspace_bytes(B, S, H, H_kv, D, block, topk, true);
-    return sel_align((size_t)B * S * H * 4) + sel_lists_bytes(B, S, H_kv, (S + block - 1) / block, topk);
+    return check_selected(B, S, H, H_kv, D, dtype, block, topk) ? 0 : sel_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk, true);
 }
 
 extern "C" int mat_selected_attn_bwd(const void *q, const void *k, const void *v, const void *o, const float *lse, const void *dout, void *dq,
@@ -387,16 +237,13 @@ extern "C" int mat_selected_attn_bwd(const void *q, const void *k, const void *v
     if (!q || !k || !v || !o || !lse || !dout || !dq || !dk || !dv || !blocks) return fail(MAT_ERR_INVALID, "all tensors must be non-NULL");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16)
         return fail(MAT_ERR_INVALID, "all tensors must be 16-byte aligned");
-    const size_t need = mat_selected_attn_bwd_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk);
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
-        return fail(MAT_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+    if (int rc = have_workspace(sel_workspace_bytes(B, S, H, H_kv, D, dtype, block, topk, true), workspace, workspace_bytes)) return rc;
     SelProblem p{};
     p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse_in = lse; p.dq = dq; p.dk = dk; p.dv = dv;
     p.B = B; p.S = S; p.H = H; p.Hkv = H_kv; p.D = D; p.dtype = dtype;
     p.blocks = blocks; p.block = block; p.topk = topk; p.nb = (S + block - 1) / block; p.causal = causal != 0;
     p.scale = scale > 0.f ? scale : 1.0f / std::sqrt((float)D);
     p.stream = (cudaStream_t)stream;
-    note_kernel(dtype == MAT_F32 ? "selected_bwd_rows" : "selected_bwd_mma");
-    if (dtype != MAT_F32) return launch_sel_mma(p, workspace, true);
-    return run_bwd<float>(p, sel_lists_at((char *)workspace + sel_align((size_t)B * S * H * 4), B, S, H_kv, p.nb, topk), (float *)workspace);
+    note_kernel(dtype == MAT_F32 ? "selected_bwd_f32" : "selected_bwd_mma");
+    return launch_sel(p, workspace, true);
 }

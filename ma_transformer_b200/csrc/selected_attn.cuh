@@ -35,9 +35,9 @@ SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, i
 // rows_per_item: items[bh * max_items + x] = (block, first row) for x in [item_base[bh * (nb + 1) + n], ...[n + 1]).
 int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item);
 
-// selected_mma.cu: 16-bit types on the tensor cores
-size_t sel_mma_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk, bool bwd);
-int launch_sel_mma(const SelProblem &p, void *workspace, bool bwd);
+// selected_tiles.cu
+size_t sel_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t block, int64_t topk, bool bwd);
+int launch_sel(const SelProblem &p, void *workspace, bool bwd);
 
 // An entry of a query's list counts when it names a block of the sequence, is above every entry before it and, with
 // causal, not behind the query's own block.  `prev` carries the largest entry so far (start at -1).

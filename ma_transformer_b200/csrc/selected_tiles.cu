@@ -1,4 +1,5 @@
-// Block-selected attention for 16-bit types on the warp-level tensor-core instructions.
+// Block-selected attention in tiles: 16-bit types on the warp-level tensor-core instructions (here), fp32 on the FMA pipe
+// (selected_f32.cuh).
 //
 // Queries of one sequence choose different blocks, so a tile of neighbouring queries shares no keys.  The selection is
 // turned round instead: per block the list of the rows (query, head) that chose it, gathered 16 or 64 at a time into
@@ -13,6 +14,7 @@
 // and backward at 8192 tokens x 8 heads of 64 x 16 blocks, so the budget only bounds the workspace.
 #include <cmath>
 
+#include "paged.cuh"
 #include "selected_attn.cuh"
 #include "pdl.cuh"
 #include "ptx.cuh"
@@ -21,6 +23,7 @@ namespace mat {
 namespace {
 
 constexpr int kFwdRows = 256;        // rows per forward item (a multiple of 64)
+constexpr int kF32Rows = 128;        // rows per item in fp32, both ways
 constexpr int kBwdRows = 512;        // rows per backward item
 constexpr size_t kPartBudget = 1024ull << 20;
 
@@ -38,6 +41,11 @@ struct SelTile {                     // what the kernels need beside SelProblem
     float scale_log2;
 };
 
+template <typename T> __device__ __forceinline__ void store4(T *at, const float4 &x) {
+    T y[4] = {Elem<T>::from_f(x.x), Elem<T>::from_f(x.y), Elem<T>::from_f(x.z), Elem<T>::from_f(x.w)};
+    if (sizeof(T) == 4) *reinterpret_cast<float4 *>(at) = *reinterpret_cast<const float4 *>(&x);
+    else *reinterpret_cast<uint2 *>(at) = *reinterpret_cast<uint2 *>(y);
+}
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -53,6 +61,12 @@ __device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_str
         cp_async16(dst + r * (DP + 8) + c, in ? src + r * row_stride + c : src, in);
     }
 }
+
+}  // namespace
+}  // namespace mat
+#include "selected_f32.cuh"
+namespace mat {
+namespace {
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // One warp per 16 rows, NKP keys at a time; keys and values of the block are shared by the CTA's warps, each warp's
@@ -303,9 +317,9 @@ template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) 
             float mx = st.x;
 #pragma unroll
             for (int x = LPR / 2; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x, LPR));
-            const float now = fmaxf(m, mx), ref = now == -INFINITY ? 0.f : now, keep = ptx::ex2(m - ref);
+            const float now = fmaxf(m, mx), ref = now == -INFINITY ? 0.f : now, keep = exp2f(m - ref);
             m = now;
-            w = ptx::ex2(st.x - ref);
+            w = exp2f(st.x - ref);
             float sum = st.y * w;
 #pragma unroll
             for (int x = LPR / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x, LPR);
@@ -331,8 +345,7 @@ template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) 
     if (!in) return;
     const float f = BWD ? p.scale : l == 0.f ? 0.f : 1.f / l;
     if (!BWD && lane == 0) p.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-    T y[4] = {Elem<T>::from_f(acc.x * f), Elem<T>::from_f(acc.y * f), Elem<T>::from_f(acc.z * f), Elem<T>::from_f(acc.w * f)};
-    *reinterpret_cast<uint2 *>((T *)(BWD ? p.dq : p.out) + out * D + col) = *reinterpret_cast<uint2 *>(y);
+    store4((T *)(BWD ? p.dq : p.out) + out * D + col, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
@@ -556,32 +569,49 @@ template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(
             c.x += w.x; c.y += w.y; c.z += w.z; c.w += w.w;
         }
         const int64_t at = ((b * p.S + j0 + x * 4 / D) * p.Hkv + h) * D + x * 4 % D;
-        T ya[4] = {Elem<T>::from_f(a.x * p.scale), Elem<T>::from_f(a.y * p.scale), Elem<T>::from_f(a.z * p.scale), Elem<T>::from_f(a.w * p.scale)};
-        T yc[4] = {Elem<T>::from_f(c.x), Elem<T>::from_f(c.y), Elem<T>::from_f(c.z), Elem<T>::from_f(c.w)};
-        *reinterpret_cast<uint2 *>((T *)p.dk + at) = *reinterpret_cast<uint2 *>(ya);
-        *reinterpret_cast<uint2 *>((T *)p.dv + at) = *reinterpret_cast<uint2 *>(yc);
+        store4((T *)p.dk + at, make_float4(a.x * p.scale, a.y * p.scale, a.z * p.scale, a.w * p.scale));
+        store4((T *)p.dv + at, c);
     }
 }
 
-// delta = dO . O of every row: D / 8 lanes of 16 bytes, padded to a power of two
+// delta = dO . O of every row: LPR lanes of 16 bytes
 template <typename T, int LPR> __global__ void __launch_bounds__(128) sel_delta_kernel(const T *o, const T *dout, float *delta, int64_t rows, int D) {
-    const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) / LPR;
-    const int col = (threadIdx.x % LPR) * 8;
+    constexpr int W = Vec16<T>::N;
+    const int64_t r = (int64_t)blockIdx.x * (128 / LPR) + threadIdx.x / LPR;
+    const int col = (threadIdx.x % LPR) * W;
     pdl_trigger();
     pdl_wait();
     float s = 0.f;
     if (r < rows && col < D) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(o + r * D + col)), b = __ldg(reinterpret_cast<const uint4 *>(dout + r * D + col));
-        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+        float x[W], y[W];
+        Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(o + r * D + col)), x);
+        Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(dout + r * D + col)), y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s = fmaf(ptx::Mma<T>::lo(x[j]), ptx::Mma<T>::lo(y[j]), s);
-            s = fmaf(ptx::Mma<T>::hi(x[j]), ptx::Mma<T>::hi(y[j]), s);
-        }
+        for (int j = 0; j < W; ++j) s = fmaf(x[j], y[j], s);
     }
 #pragma unroll
     for (int x = 1; x < LPR; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
     if (r < rows && col == 0) delta[r] = s;
+}
+
+template <typename T> void launch_delta(const SelProblem &p, float *delta) {
+    const int64_t all = p.B * p.S * p.H;
+    const int lanes = (int)p.D * (int)sizeof(T) / 16 <= 8 ? 8 : (int)p.D * (int)sizeof(T) / 16 <= 16 ? 16 : 32;
+    const dim3 grid((unsigned)((all + 128 / lanes - 1) / (128 / lanes)));
+    const T *o = (const T *)p.o, *g = (const T *)p.dout;
+    if (lanes == 8) launch_after(sel_delta_kernel<T, 8>, grid, dim3(128), 0, p.stream, o, g, delta, all, (int)p.D);
+    else if (lanes == 16) launch_after(sel_delta_kernel<T, 16>, grid, dim3(128), 0, p.stream, o, g, delta, all, (int)p.D);
+    else launch_after(sel_delta_kernel<T, 32>, grid, dim3(128), 0, p.stream, o, g, delta, all, (int)p.D);
+}
+
+template <typename T, bool BWD> void launch_join(const SelProblem &p, const SelTile &t, int64_t pairs) {
+    const int64_t rows = p.S * t.G;
+    if (p.D <= 64) launch_after(sel_join_kernel<T, 16, BWD>, dim3((unsigned)((rows + 7) / 8), (unsigned)pairs), dim3(128), 0, p.stream, p, t);
+    else launch_after(sel_join_kernel<T, 32, BWD>, dim3((unsigned)((rows + 3) / 4), (unsigned)pairs), dim3(128), 0, p.stream, p, t);
+}
+
+template <typename T> void launch_kv_join(const SelProblem &p, const SelTile &t, int64_t pairs) {
+    launch_after(sel_kv_join_kernel<T>, dim3((unsigned)(p.nb * t.nsub), (unsigned)pairs, (unsigned)((64 * p.D / 4 + 127) / 128)), dim3(128), 0, p.stream, p, t);
 }
 
 int launched(const char *what) {
@@ -596,11 +626,13 @@ struct Plan {
     size_t lists, items, base, stats, part, kv, delta, total;
 };
 
-Plan plan(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk, bool bwd) {
+int rows_per_item(int dtype, bool bwd) { return dtype == MAT_F32 ? kF32Rows : bwd ? kBwdRows : kFwdRows; }
+
+Plan plan(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t block, int64_t topk, bool bwd) {
     Plan w;
     const int64_t nb = (S + block - 1) / block, G = H / Hkv, bh = B * Hkv;
     w.nsub = bwd ? (int)((block + 63) / 64) : 1;
-    const int64_t rows = bwd ? kBwdRows : kFwdRows;
+    const int64_t rows = rows_per_item(dtype, bwd);
     w.max_items = S * topk * G / rows + nb;
     const size_t per = (size_t)S * G * topk * w.nsub * D * 4;
     w.group = per >= kPartBudget ? 1 : (int64_t)(kPartBudget / per);
@@ -631,41 +663,57 @@ int prepare(const SelProblem &p, const Plan &w, void *ws, bool bwd, SelTile &t) 
     t.G = (int)(p.H / p.Hkv);
     t.nsub = w.nsub;
     t.scale_log2 = p.scale * 1.4426950408889634f;
-    return launch_sel_lists(p, t.l, (int2 *)(at + w.items), (int32_t *)(at + w.base), t.max_items, bwd ? kBwdRows : kFwdRows);
+    return launch_sel_lists(p, t.l, (int2 *)(at + w.items), (int32_t *)(at + w.base), t.max_items, rows_per_item(p.dtype, bwd));
 }
 
-template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, const Plan &w, SelTile t) {
+// The groups of pairs in turn: their tiles, then their joins.
+template <bool BWD, typename T, typename Launch> int over_groups(const SelProblem &p, const Plan &w, SelTile &t, Launch &&tiles) {
     const int64_t bh = p.B * p.Hkv;
+    for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
+        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group;
+        tiles((unsigned)n);
+        launch_join<T, BWD>(p, t, n);
+        if (BWD) launch_kv_join<T>(p, t, n);
+    }
+    return launched(BWD ? "launching the selected attention's backward" : "launching the selected attention");
+}
+
+template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, const Plan &w, SelTile &t) {
     const size_t smem = ((p.block + NKP - 1) / NKP * NKP * 2 + 4 * 2 * 16) * (DP + 8) * sizeof(T);
     if (int rc = ensure_dynamic_smem((const void *)sel_fwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention")) return rc;
-    for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
-        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = p.S * t.G;
-        launch_after(sel_fwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)n), dim3(128), smem, p.stream, p, t);
-        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, false>, dim3((unsigned)((rows + 128 / 16 - 1) / (128 / 16)), (unsigned)n), dim3(128), 0, p.stream, p, t);
-        else launch_after(sel_join_kernel<T, 32, false>, dim3((unsigned)((rows + 128 / 32 - 1) / (128 / 32)), (unsigned)n), dim3(128), 0, p.stream, p, t);
-    }
-    return launched("launching the selected attention");
+    return over_groups<false, T>(p, w, t, [&](unsigned n) {
+        launch_after(sel_fwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, n), dim3(128), smem, p.stream, p, t);
+    });
 }
 
-template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, const Plan &w, SelTile t) {
-    const int64_t bh = p.B * p.Hkv, all = p.B * p.S * p.H;
+template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, const Plan &w, SelTile &t) {
     const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 2 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20;
     if (int rc = ensure_dynamic_smem((const void *)sel_bwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention's backward")) return rc;
-    float *delta = const_cast<float *>(t.delta);
-    if (p.D <= 64) launch_after(sel_delta_kernel<T, 8>, dim3((unsigned)((all * 8 + 127) / 128)), dim3(128), 0, p.stream, (const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
-    else launch_after(sel_delta_kernel<T, 16>, dim3((unsigned)((all * 16 + 127) / 128)), dim3(128), 0, p.stream, (const T *)p.o, (const T *)p.dout, delta, all, (int)p.D);
-    for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
-        const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group, rows = p.S * t.G;
-        launch_after(sel_bwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)w.nsub, (unsigned)n), dim3(128), smem, p.stream, p, t);
-        if (p.D <= 64) launch_after(sel_join_kernel<T, 16, true>, dim3((unsigned)((rows + 128 / 16 - 1) / (128 / 16)), (unsigned)n), dim3(128), 0, p.stream, p, t);
-        else launch_after(sel_join_kernel<T, 32, true>, dim3((unsigned)((rows + 128 / 32 - 1) / (128 / 32)), (unsigned)n), dim3(128), 0, p.stream, p, t);
-        launch_after(sel_kv_join_kernel<T>, dim3((unsigned)(p.nb * w.nsub), (unsigned)n, (unsigned)((64 * p.D / 4 + 127) / 128)), dim3(128), 0, p.stream, p, t);
-    }
-    return launched("launching the selected attention's backward");
+    launch_delta<T>(p, const_cast<float *>(t.delta));
+    return over_groups<true, T>(p, w, t, [&](unsigned n) {
+        launch_after(sel_bwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)w.nsub, n), dim3(128), smem, p.stream, p, t);
+    });
+}
+
+int run_f32(const SelProblem &p, void *ws, bool back) {
+    const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.dtype, p.block, p.topk, back);
+    SelTile t{};
+    if (int rc = prepare(p, w, ws, back, t)) return rc;
+    const size_t pitch = p.D + 4, key_rows = (p.block + 63) / 64 * 64;
+    const size_t smem = ((back ? 4 * 64 : 2 * key_rows + 64) * pitch + (back ? 2 : 1) * 64 * kWPitch) * sizeof(float);
+    if (int rc = ensure_dynamic_smem(back ? (const void *)sel_bwd_f32_kernel : (const void *)sel_fwd_f32_kernel, smem, "shared memory of the selected attention in fp32")) return rc;
+    if (!back)
+        return over_groups<false, float>(p, w, t, [&](unsigned n) {
+            launch_after(sel_fwd_f32_kernel, dim3((unsigned)w.max_items, n), dim3(kF32Threads), smem, p.stream, p, t);
+        });
+    launch_delta<float>(p, const_cast<float *>(t.delta));
+    return over_groups<true, float>(p, w, t, [&](unsigned n) {
+        launch_after(sel_bwd_f32_kernel, dim3((unsigned)w.max_items, (unsigned)w.nsub, n), dim3(kF32Threads), smem, p.stream, p, t);
+    });
 }
 
 template <typename T> int run(const SelProblem &p, void *ws, bool back) {
-    const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.block, p.topk, back);
+    const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.dtype, p.block, p.topk, back);
     SelTile t{};
     if (int rc = prepare(p, w, ws, back, t)) return rc;
     const int dp = p.D <= 64 ? 64 : 128, nkp = p.block <= 32 ? 32 : 64;
@@ -684,11 +732,12 @@ template <typename T> int run(const SelProblem &p, void *ws, bool back) {
 
 }  // namespace
 
-size_t sel_mma_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t block, int64_t topk, bool bwd) {
-    return plan(B, S, H, Hkv, D, block, topk, bwd).total;
+size_t sel_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t block, int64_t topk, bool bwd) {
+    return plan(B, S, H, Hkv, D, dtype, block, topk, bwd).total;
 }
 
-int launch_sel_mma(const SelProblem &p, void *workspace, bool bwd) {
+int launch_sel(const SelProblem &p, void *workspace, bool bwd) {
+    if (p.dtype == MAT_F32) return run_f32(p, workspace, bwd);
     return p.dtype == MAT_BF16 ? run<__nv_bfloat16>(p, workspace, bwd) : run<__half>(p, workspace, bwd);
 }
 
