@@ -143,7 +143,7 @@ template <int W> __device__ __forceinline__ void turn(float *x, const float *c, 
 
 template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) append_rows_kernel(const AppendArgs a) {
     constexpr int W = VEC ? Vec16<T>::N : 1, U = 2;
-    __shared__ int starts[kKnownStarts + 1];
+    __shared__ int starts[kKnownStarts + 1];         // first rows of the sequences
     __shared__ int pos_of[64];
     __shared__ int64_t k_of[64], v_of[64];
     extern __shared__ float turns[];                 // [tile][rot / 2] cosines, then sines
@@ -348,9 +348,9 @@ template <typename T> __global__ void __launch_bounds__(128) page_bounds_kernel(
 }
 
 template <typename T> int launch_append(AppendArgs &a, bool vec, cudaStream_t stream) {
-    // enough tiles to fill the GPU, few enough that a tile's look-ups are shared: 1 to 64 tokens, 32 KB of angles
-    a.tile = 1;
-    while (a.tile < 64 && a.tile * 148 * 8 < a.N && (a.tile * 2) * a.rot * 4 <= 32768) a.tile *= 2;
+    // one wave of CTAs (four a SM) where a tile of at most 64 tokens and 32 KB of angles allows it
+    const int64_t wave = 148 * 4, most = a.rot ? min((int64_t)64, (int64_t)32768 / (a.rot * 4)) : 64;
+    a.tile = (int)min(most, (a.N + wave - 1) / wave);
     const unsigned tiles = (unsigned)((a.N + a.tile - 1) / a.tile);
     const size_t smem = (size_t)a.tile * a.rot * sizeof(float);
     if (vec) append_rows_kernel<T, true><<<tiles, 256, smem, stream>>>(a);

@@ -64,8 +64,10 @@ struct RowTokens {
     }
     // tokens per chunk; rows of up to c tokens are one chunk
     __device__ __forceinline__ int64_t chunk(const DecodeArgs &a) const {
-        if (n <= (int64_t)a.min_chunk * a.nsplit) return a.min_chunk;     // no division in the common case
-        return ((n + a.nsplit - 1) / a.nsplit + 63) / 64 * 64;
+        if (n <= a.min_chunk) return a.min_chunk;
+        // as few chunks as min_chunk allows, all of one size
+        const uint32_t most = (uint32_t)a.nsplit, m = (uint32_t)n, want = (m + a.min_chunk - 1) / a.min_chunk, k = want < most ? want : most;
+        return (int64_t)(((m + k - 1) / k + 63) / 64 * 64);
     }
     // position of virtual token t, or -1
     __device__ __forceinline__ int64_t position(const DecodeArgs &a, int64_t t) const {
@@ -82,14 +84,14 @@ struct RowTokens {
 template <typename T, int LPK, int NV, int GT, int U>
 __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     constexpr int W = Vec16<T>::N, KPW = 32 / LPK, C = NV * W;
-    const int64_t b = blockIdx.z, h = blockIdx.y / (unsigned)a.tiles, g0 = (int64_t)(blockIdx.y % (unsigned)a.tiles) * GT;
+    const int64_t b = blockIdx.z, h = blockIdx.x / (unsigned)a.tiles, g0 = (int64_t)(blockIdx.x % (unsigned)a.tiles) * GT;
     const int64_t G = a.G;
     const int D = (int)a.D;
     pdl_trigger();
     const RowTokens row(a, b, h);
-    const int64_t chunk = row.chunk(a), t0 = blockIdx.x * chunk;
+    const int64_t chunk = row.chunk(a), t0 = blockIdx.y * chunk;
     const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
-    if (t0 >= row.n && blockIdx.x > 0) return;
+    if (t0 >= row.n && blockIdx.y > 0) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, part = lane % LPK, key = lane / LPK;
 
     float q[GT][C], acc[GT][C], m[GT], l[GT];
@@ -213,9 +215,9 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
             float x = 0.f;
             for (int i = 0; i < 4; ++i) x += w[i * stride + 2 + d] * e[i];
             if (whole) ((T *)a.o)[head * D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x * inv);
-            else a.part[(head * a.nsplit + blockIdx.x) * D + d] = x;
+            else a.part[(head * a.nsplit + blockIdx.y) * D + d] = x;
         }
-        if (!whole && threadIdx.x == 0) a.stats[head * a.nsplit + blockIdx.x] = make_float2(top, sum);
+        if (!whole && threadIdx.x == 0) a.stats[head * a.nsplit + blockIdx.y] = make_float2(top, sum);
     }
 }
 
@@ -232,14 +234,14 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) 
 
 template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) decode_mma_kernel(const DecodeArgs a) {
     constexpr int PITCH = DP + 8, TILE = 16 * PITCH, CH = DP / 8;
-    const int64_t b = blockIdx.z, h = blockIdx.y / (unsigned)a.tiles, G = a.G;
-    const int g0 = (int)(blockIdx.y % (unsigned)a.tiles) * 16, heads = min(16, (int)G - g0);
+    const int64_t b = blockIdx.z, h = blockIdx.x / (unsigned)a.tiles, G = a.G;
+    const int g0 = (int)(blockIdx.x % (unsigned)a.tiles) * 16, heads = min(16, (int)G - g0);
     const int D = (int)a.D;
     pdl_trigger();
     const RowTokens row(a, b, h);
-    const int64_t chunk = row.chunk(a), t0 = blockIdx.x * chunk;
+    const int64_t chunk = row.chunk(a), t0 = blockIdx.y * chunk;
     const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
-    if (t0 >= row.n && blockIdx.x > 0) return;
+    if (t0 >= row.n && blockIdx.y > 0) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     extern __shared__ __align__(16) char smem[];
     T *ring = (T *)smem + warp * NS * 2 * TILE;          // NS x (16 keys, 16 values)
@@ -409,14 +411,50 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
             T z[4] = {Elem<T>::from_f(y.x * f), Elem<T>::from_f(y.y * f), Elem<T>::from_f(y.z * f), Elem<T>::from_f(y.w * f)};
             *reinterpret_cast<uint2 *>((T *)a.o + head * D + col) = *reinterpret_cast<uint2 *>(z);
         } else {
-            *reinterpret_cast<float4 *>(a.part + (head * a.nsplit + blockIdx.x) * D + col) = y;
-            if (col == 0) a.stats[head * a.nsplit + blockIdx.x] = make_float2(top, sum);
+            *reinterpret_cast<float4 *>(a.part + (head * a.nsplit + blockIdx.y) * D + col) = y;
+            if (col == 0) a.stats[head * a.nsplit + blockIdx.y] = make_float2(top, sum);
         }
     }
 }
 
 // ---- joining the chunks of a row -------------------------------------------------------------------------------------
-// One CTA per (sequence, query head): the chunks' weights first, then the sum.  D / 4 lanes of four columns, the other
+// Up to 32 chunks: one warp per (sequence, query head), a lane per chunk for the weights, then lanes over columns.
+template <typename T> __global__ void __launch_bounds__(128) join_few_kernel(const DecodeArgs a) {
+    const int lane = threadIdx.x % 32, D = (int)a.D;
+    const uint32_t x = blockIdx.x * 4 + threadIdx.x / 32, b = x / (uint32_t)a.H, hq = x - b * (uint32_t)a.H;
+    pdl_wait();
+    if (b >= (uint32_t)a.B) return;
+    const int64_t head = x;
+    const RowTokens row(a, b, hq / (uint32_t)a.G);
+    const int64_t chunk = row.chunk(a);
+    if (chunk >= row.n) return;                      // written by its only chunk
+    const int n = (int)((uint32_t)(row.n + chunk - 1) / (uint32_t)chunk);
+    const float2 st = lane < n ? a.stats[head * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
+    float top = st.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float w = exp2f(st.x - (top == -INFINITY ? 0.f : top));
+    float sum = st.y * w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    const float *part = a.part + head * a.nsplit * D;
+    for (int c0 = 0; c0 < D; c0 += 128) {
+        const int col = c0 + lane * 4;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float e = __shfl_sync(0xffffffffu, w, i);
+            const float4 u = col < D ? *reinterpret_cast<const float4 *>(part + i * D + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+            y.x = fmaf(u.x, e, y.x); y.y = fmaf(u.y, e, y.y); y.z = fmaf(u.z, e, y.z); y.w = fmaf(u.w, e, y.w);
+        }
+        if (col >= D) continue;
+        T *o = (T *)a.o + head * D + col;
+        o[0] = Elem<T>::from_f(y.x * f); o[1] = Elem<T>::from_f(y.y * f); o[2] = Elem<T>::from_f(y.z * f); o[3] = Elem<T>::from_f(y.w * f);
+    }
+}
+
+// More: one CTA per (sequence, query head), the chunks' weights first, then the sum.  D / 4 lanes of four columns, the other
 // threads take every k-th chunk, and their sums are added in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a) {
     __shared__ float4 acc[256];
@@ -479,7 +517,8 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
 
 template <typename T, int LPK, int NV, int GT> int launch_simt(const DecodeArgs &a, cudaStream_t s) {
     constexpr int U = NV == 1 ? 4 : 2;
-    dim3 grid((unsigned)a.nsplit, (unsigned)(a.Hkv * a.tiles), (unsigned)a.B);
+    // heads fastest: the CTAs that read neighbouring rows of a page run side by side
+    dim3 grid((unsigned)(a.Hkv * a.tiles), (unsigned)a.nsplit, (unsigned)a.B);
     const size_t smem = 4 * GT * (a.D + 2) * sizeof(float);
     decode_simt_kernel<T, LPK, NV, GT, U><<<grid, 128, smem, s>>>(a);
     cudaError_t e = cudaGetLastError();
@@ -498,7 +537,8 @@ template <typename T, int DP, int NS> int launch_mma(const DecodeArgs &a, cudaSt
     const size_t ring = 4 * NS * 2 * 16 * (DP + 8) * sizeof(T), res = (4 * 16 * (DP + 4) + 128) * sizeof(float);
     const size_t smem = ring > res ? ring : res;
     if (int rc = ensure_dynamic_smem((const void *)decode_mma_kernel<T, DP, NS>, smem, "shared memory of the paged decode")) return rc;
-    dim3 grid((unsigned)a.nsplit, (unsigned)(a.Hkv * a.tiles), (unsigned)a.B);
+    // heads fastest: the CTAs that read neighbouring rows of a page run side by side
+    dim3 grid((unsigned)(a.Hkv * a.tiles), (unsigned)a.nsplit, (unsigned)a.B);
     decode_mma_kernel<T, DP, NS><<<grid, 128, smem, s>>>(a);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode");
@@ -523,7 +563,8 @@ template <> int run_mma<float>(DecodeArgs &a, cudaStream_t s) { return run_simt<
 template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
     const int rc = a.aligned ? run_mma<T>(a, s) : run_simt<T>(a, s);
     if (rc || a.nsplit == 1) return rc;
-    const cudaError_t e = launch_after(join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B), dim3(256), 0, s, a);
+    const cudaError_t e = a.nsplit <= 32 ? launch_after(join_few_kernel<T>, dim3((unsigned)((a.H * a.B + 3) / 4)), dim3(128), 0, s, a)
+                                         : launch_after(join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B), dim3(256), 0, s, a);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode's join");
 }
 

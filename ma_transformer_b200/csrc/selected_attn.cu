@@ -19,86 +19,87 @@ namespace {
 constexpr int kTile = 256;          // queries per tile of the lists
 constexpr int kRange = 1024;        // blocks per CTA of the lists: 32 KB of bit masks
 
-// ---- lists ----------------------------------------------------------------------------------------------------------
+// ---- lists: per tile of queries a count per block, then where each run starts, then the entries ----------------------------------------------------------------------------------------------------------
 // mask[n][w]: the tile's queries that chose block n, a bit each.  A bit set does not depend on the order of the writers,
 // so the lists come out the same every time.
 __device__ __forceinline__ int own_limit(const SelProblem &p, int64_t i) {
     return p.causal ? (int)(i / p.block) + 1 : (int)p.nb;
 }
 
-template <bool FILL> __global__ void __launch_bounds__(kTile) lists_kernel(const SelProblem p, const SelLists l) {
-    __shared__ uint32_t mask[kRange][kTile / 32];
-    const int64_t tile = blockIdx.x, bh = blockIdx.z, b = bh / p.Hkv, h = bh % p.Hkv;
-    const int n0 = blockIdx.y * kRange, n1 = min(n0 + kRange, (int)p.nb);
-    const int tid = threadIdx.x;
+// A tile's lists come through shared memory, kStage entries of every query at a time: read one by one from global memory
+// they lived off the L1, which the next kernel's waiting CTAs take away (fill: 50 us instead of FILL_US at 8192 x 8 x 16).
+constexpr int kStage = 16;
+
+struct TileLists {
+    const SelProblem &p;
+    const int32_t *first;       // of the tile's first query
+    int rows;                   // queries of the tile that exist
+    int (*stage)[kStage + 1];
+    __device__ __forceinline__ void load(int s0) {
+        __syncthreads();
+        const int cnt = min(kStage, (int)p.topk - s0);
+        for (int x = threadIdx.x; x < rows * kStage; x += kTile) {
+            const int r = x / kStage, c = x % kStage;
+            if (c < cnt) stage[r][c] = __ldg(first + (int64_t)r * p.Hkv * p.topk + s0 + c);
+        }
+        __syncthreads();
+    }
+    // calls f(block, place in the list) for this thread's entries that count and lie in [n0, n1)
+    template <typename F> __device__ __forceinline__ void each(int limit, int n0, int n1, F &&f) {
+        int prev = -1;
+        for (int s0 = 0; s0 < p.topk; s0 += kStage) {
+            load(s0);
+            const int cnt = min(kStage, (int)p.topk - s0);
+            if ((int)threadIdx.x < rows)
+                for (int c = 0; c < cnt; ++c) {
+                    const int n = stage[threadIdx.x][c];
+                    if (sel_entry_counts(n, prev, limit) && n >= n0 && n < n1) f(n, s0 + c);
+                }
+        }
+    }
+};
+
+__device__ __forceinline__ TileLists tile_lists(const SelProblem &p, int64_t tile, int64_t bh, int (*stage)[kStage + 1]) {
+    const int64_t b = bh / p.Hkv, h = bh % p.Hkv, i0 = tile * kTile;
+    return TileLists{p, p.blocks + ((b * p.S + i0) * p.Hkv + h) * p.topk, (int)min((int64_t)kTile, p.S - i0), stage};
+}
+
+__global__ void __launch_bounds__(kTile) lists_count_kernel(const SelProblem p, const SelLists l) {
+    __shared__ int hist[kRange], stage[kTile][kStage + 1];
+    const int64_t tile = blockIdx.x, bh = blockIdx.z;
+    const int n0 = blockIdx.y * kRange, n1 = min(n0 + kRange, (int)p.nb), tid = threadIdx.x;
+    pdl_trigger();
+    for (int i = tid; i < n1 - n0; i += kTile) hist[i] = 0;
+    pdl_wait();
+    tile_lists(p, tile, bh, stage).each(own_limit(p, tile * kTile + tid), n0, n1, [&](int n, int) { atomicAdd(&hist[n - n0], 1); });
+    __syncthreads();
+    for (int n = n0 + tid; n < n1; n += kTile) l.counts[(bh * l.tiles + tile) * p.nb + n] = hist[n - n0];
+}
+
+__global__ void __launch_bounds__(kTile) lists_fill_kernel(const SelProblem p, const SelLists l) {
+    extern __shared__ int fill_smem[];
+    uint32_t (*mask)[kTile / 32] = (uint32_t (*)[kTile / 32])fill_smem;            // [kRange][kTile / 32]
+    int *start = fill_smem + kRange * (kTile / 32);                                // [kRange]
+    int (*stage)[kStage + 1] = (int (*)[kStage + 1])(start + kRange);              // [kTile][kStage + 1]
+    const int64_t tile = blockIdx.x, bh = blockIdx.z;
+    const int n0 = blockIdx.y * kRange, n1 = min(n0 + kRange, (int)p.nb), tid = threadIdx.x;
     pdl_trigger();
     for (int i = tid; i < (n1 - n0) * (kTile / 32); i += kTile) (&mask[0][0])[i] = 0;
     pdl_wait();
+    for (int i = tid; i < n1 - n0; i += kTile) start[i] = l.base[bh * (p.nb + 1) + n0 + i] + l.counts[(bh * l.tiles + tile) * p.nb + n0 + i];
+    const int limit = own_limit(p, tile * kTile + tid);
+    TileLists lists = tile_lists(p, tile, bh, stage);
+    lists.each(limit, n0, n1, [&](int n, int) { atomicOr(&mask[n - n0][tid / 32], 1u << (tid % 32)); });
     __syncthreads();
-    const int64_t i = tile * kTile + tid;
-    const int32_t *row = p.blocks + ((b * p.S + i) * p.Hkv + h) * p.topk;
-    const int limit = i < p.S ? own_limit(p, i) : 0;
-    if (i < p.S) {
-        int prev = -1;
-#pragma unroll 8
-        for (int s = 0; s < p.topk; ++s) {
-            const int n = row[s];
-            if (sel_entry_counts(n, prev, limit) && n >= n0 && n < n1) atomicOr(&mask[n - n0][tid / 32], 1u << (tid % 32));
-        }
-    }
-    __syncthreads();
-    if (!FILL) {
-        for (int n = n0 + tid; n < n1; n += kTile) {
-            int c = 0;
+    int32_t *entries = l.entry + bh * p.S * p.topk;
+    const int i = (int)(tile * kTile) + tid;
+    lists.each(limit, n0, n1, [&](int n, int s) {
+        const uint32_t *m = mask[n - n0];
+        int rank = __popc(m[tid / 32] & ((1u << (tid % 32)) - 1));
 #pragma unroll
-            for (int w = 0; w < kTile / 32; ++w) c += __popc(mask[n - n0][w]);
-            l.counts[(bh * p.nb + n) * l.tiles + tile] = c;
-        }
-    } else if (i < p.S) {
-        int prev = -1;
-        int32_t *entries = l.entry + bh * p.S * p.topk;
-        for (int s0 = 0; s0 < p.topk; s0 += 8) {       // eight entries' offsets in flight
-            int n[8], at[8];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) n[y] = s0 + y < p.topk ? row[s0 + y] : -1;
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                if (!sel_entry_counts(n[y], prev, limit) || n[y] < n0 || n[y] >= n1) n[y] = -1;
-                at[y] = n[y] < 0 ? 0 : l.base[bh * (p.nb + 1) + n[y]] + l.counts[(bh * p.nb + n[y]) * l.tiles + tile];
-            }
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                if (n[y] < 0) continue;
-                const uint32_t *m = mask[n[y] - n0];
-                int rank = __popc(m[tid / 32] & ((1u << (tid % 32)) - 1));
-                for (int w = 0; w < tid / 32; ++w) rank += __popc(m[w]);
-                entries[at[y] + rank] = (int32_t)(i * p.topk + s0 + y);
-            }
-        }
-    }
-}
-
-// counts of a block's tiles -> offsets within its list, one warp per (bh, block)
-__global__ void __launch_bounds__(128) lists_offsets_kernel(SelLists l, int64_t rows) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-    pdl_trigger();
-    pdl_wait();
-    if (r >= rows) return;
-    const int lane = threadIdx.x % 32;
-    int32_t *c = l.counts + r * l.tiles;
-    int total = 0;
-    for (int64_t t0 = 0; t0 < l.tiles; t0 += 32) {
-        const int x = t0 + lane < l.tiles ? c[t0 + lane] : 0;
-        int sum = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += y;
-        }
-        if (t0 + lane < l.tiles) c[t0 + lane] = total + sum - x;
-        total += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) l.totals[r] = total;
+        for (int w = 0; w < kTile / 32 - 1; ++w) rank += w < tid / 32 ? __popc(m[w]) : 0;
+        entries[start[n - n0] + rank] = i * (int)p.topk + s;
+    });
 }
 
 // inclusive sum over the CTA's 1024 threads
@@ -117,7 +118,8 @@ __device__ __forceinline__ int block_scan(int x, int *of_warp) {
     return x + before;
 }
 
-// totals of the blocks -> where each list starts, and the items of its rows: one CTA per bh
+// counts of a block's tiles -> offsets within its list; totals of the blocks -> where each list starts, and the items of
+// its rows: one CTA per bh
 __global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb, int G, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item) {
     __shared__ int of_warp[32], carry[2];
     const int64_t bh = blockIdx.x;
@@ -126,7 +128,20 @@ __global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb
     int entries = 0, before = 0;
     for (int64_t n0 = 0; n0 < nb; n0 += 1024) {
         const int64_t n = n0 + threadIdx.x;
-        const int x = n < nb ? l.totals[bh * nb + n] : 0;
+        int x = 0;
+        if (n < nb) {
+            int32_t *c = l.counts + bh * l.tiles * nb + n;
+            for (int64_t t0 = 0; t0 < l.tiles; t0 += 8) {       // eight tiles' counts in flight
+                int y[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) y[u] = t0 + u < l.tiles ? c[(t0 + u) * nb] : 0;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (t0 + u < l.tiles) c[(t0 + u) * nb] = x;
+                    x += y[u];
+                }
+            }
+        }
         const int sum = block_scan(x, of_warp);
         if (n < nb) l.base[bh * (nb + 1) + n] = entries + sum - x;
         const int mine = (int)(((int64_t)x * G + rows_per_item - 1) / rows_per_item);
@@ -168,7 +183,7 @@ int check_selected(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int 
 
 size_t sel_lists_bytes(int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk) {
     const int64_t tiles = (S + kTile - 1) / kTile, bh = B * Hkv;
-    return sel_align((size_t)bh * nb * tiles * 4) + sel_align((size_t)bh * nb * 4) + sel_align((size_t)bh * (nb + 1) * 4) +
+    return sel_align((size_t)bh * nb * tiles * 4) + sel_align((size_t)bh * (nb + 1) * 4) +
            sel_align((size_t)bh * S * topk * 4);
 }
 
@@ -178,7 +193,6 @@ SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, i
     const int64_t bh = B * Hkv;
     char *at = (char *)ws;
     l.counts = (int32_t *)at; at += sel_align((size_t)bh * nb * l.tiles * 4);
-    l.totals = (int32_t *)at; at += sel_align((size_t)bh * nb * 4);
     l.base = (int32_t *)at;   at += sel_align((size_t)bh * (nb + 1) * 4);
     l.entry = (int32_t *)at;
     return l;
@@ -187,11 +201,11 @@ SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, i
 int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item) {
     const unsigned bh = (unsigned)(p.B * p.Hkv);
     const dim3 grid((unsigned)l.tiles, (unsigned)((p.nb + kRange - 1) / kRange), bh);
-    lists_kernel<false><<<grid, kTile, 0, p.stream>>>(p, l);
-    const int64_t rows = (int64_t)bh * p.nb;
-    launch_after(lists_offsets_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, p.stream, l, rows);
+    lists_count_kernel<<<grid, kTile, 0, p.stream>>>(p, l);
     launch_after(lists_base_kernel, dim3(bh), dim3(1024), 0, p.stream, l, p.nb, (int)(p.H / p.Hkv), items, item_base, max_items, rows_per_item);
-    launch_after(lists_kernel<true>, grid, dim3(kTile), 0, p.stream, p, l);
+    const size_t smem = (kRange * (kTile / 32 + 1) + kTile * (kStage + 1)) * sizeof(int);
+    if (int rc = ensure_dynamic_smem((const void *)lists_fill_kernel, smem, "shared memory of the lists of a block selection")) return rc;
+    launch_after(lists_fill_kernel, grid, dim3(kTile), smem, p.stream, p, l);
     return launched("launching the lists of a block selection");
 }
 

@@ -23,8 +23,7 @@ struct SelProblem {
 // [base[bh * (nb + 1) + n], base[bh * (nb + 1) + n + 1]) of entry[bh * S * topk + ...], ascending, each
 // query * topk + the place of the block in the query's list.
 struct SelLists {
-    int32_t *counts;   // [bh][nb][tiles] queries of a tile that chose a block, then their offset within the block's list
-    int32_t *totals;   // [bh][nb]
+    int32_t *counts;   // [bh][tiles][nb] queries of a tile that chose a block, then their offset within the block's list
     int32_t *base;     // [bh][nb + 1]
     int32_t *entry;    // [bh][S * topk]
     int64_t tiles;

@@ -274,7 +274,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
 }
 
 // Joins a row's partials in the order of its list: LPR lanes of 4 columns per row.  The lanes first look at LPR entries
-// of the list together (which count, and with what weight), then read the partials of those that do, four at a time.
+// of the list together (which count, and with what weight), then read the partials of those that do, eight at a time.
 // BWD: the sum of a row's shares of dq.
 template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t) {
     const uint32_t x0 = (blockIdx.x * 128u + threadIdx.x) / LPR, G = t.G;                       // (i, g) of the pair
@@ -327,7 +327,7 @@ template <typename T, int LPR, bool BWD> __global__ void __launch_bounds__(128) 
             acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
         }
         const int cnt = min(LPR, T_ - s0);
-#pragma unroll 4
+#pragma unroll 8
         for (int y = 0; y < cnt; ++y) {
             const int use = __shfl_sync(0xffffffffu, uses, y, LPR);
             const float f = __shfl_sync(0xffffffffu, w, y, LPR);
