@@ -275,24 +275,46 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
             }
         }
     };
+    // this lane's 16 bytes of every row it copies; a lane past D copies zeros
+    constexpr int RS = 32 / CH > 0 ? 32 / CH : 1;        // rows a warp copies at a time
+    const int r0 = lane / CH, col = lane % CH * 8, bytes = col < D ? 16 : 0;
+    const int64_t k_lane = col < D ? r0 * a.c.k_tok + h * a.c.k_head + col : 0, v_lane = col < D ? r0 * a.c.v_tok + h * a.c.v_head + col : 0;
+    const int64_t k_step = col < D ? RS * a.c.k_tok : 0, v_step = col < D ? RS * a.c.v_tok : 0;
+    const uint32_t lane_dst = ptx::smem_u32(ring + r0 * PITCH + col);
+    int fill = 0;                                        // place of the ring that the next load goes to
     auto load = [&](int x) {                             // tile x into its place of the ring
         const int phys = __shfl_sync(0xffffffffu, phys_of, x % 32), pos = __shfl_sync(0xffffffffu, pos_of, x % 32);
         if (x < mine) {
-            T *dst = ring + x % NS * 2 * TILE;
+            uint32_t dst = lane_dst + fill * (2 * TILE * (int)sizeof(T));
             const int64_t slot = pos & ((1 << a.c.page_shift) - 1);
-            const T *k = (const T *)a.c.k + (phys < 0 ? 0 : phys * a.c.k_page + slot * a.c.k_tok + h * a.c.k_head);
-            const T *v = (const T *)a.c.v + (phys < 0 ? 0 : phys * a.c.v_page + slot * a.c.v_tok + h * a.c.v_head);
             const int lo = (int)(row.lo - pos), hi = phys < 0 ? 0 : (int)(row.len - pos < 16 ? row.len - pos : 16);
+            const T *k = (const T *)a.c.k, *v = (const T *)a.c.v;
+            if (phys >= 0) {
+                k += phys * a.c.k_page + slot * a.c.k_tok;
+                v += phys * a.c.v_page + slot * a.c.v_tok;
+            }
+            if (lo <= 0 && hi == 16) {                   // all but the ends of a row
+                k += k_lane;
+                v += v_lane;
 #pragma unroll
-            for (int c = lane; c < 16 * CH; c += 32) {
-                const int r = c / CH, col = c % CH * 8;
-                // rows outside the sequence and columns past D arrive as zeros: a weight of zero would not silence what
-                // such a row holds
-                const bool in = r >= lo && r < hi && col < D;
-                cp_async16(dst + r * PITCH + col, in ? k + r * a.c.k_tok + col : (const T *)a.c.k, in);
-                cp_async16(dst + TILE + r * PITCH + col, in ? v + r * a.c.v_tok + col : (const T *)a.c.v, in);
+                for (int i = 0; i < 16 / RS; ++i) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(k), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE * (int)sizeof(T)), "l"(v), "r"(bytes) : "memory");
+                    dst += RS * PITCH * sizeof(T);
+                    k += k_step;
+                    v += v_step;
+                }
+            } else {
+                // rows outside the sequence arrive as zeros: a weight of zero would not silence what such a row holds
+                T *at = ring + fill * 2 * TILE;
+                for (int r = r0; r < 16; r += RS) {
+                    const bool in = r >= lo && r < hi && col < D;
+                    cp_async16(at + r * PITCH + col, in ? k + r * a.c.k_tok + h * a.c.k_head + col : k, in);
+                    cp_async16(at + TILE + r * PITCH + col, in ? v + r * a.c.v_tok + h * a.c.v_head + col : v, in);
+                }
             }
         }
+        fill = fill == NS - 1 ? 0 : fill + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
@@ -303,13 +325,15 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
     int phys_now = phys_of, pos_now = pos_of;            // of the batch being computed; loads may be a batch ahead
 #pragma unroll
     for (int x = 0; x < NS - 1; ++x) load(x);
+    int place = 0;
     for (int x = 0; x < mine; ++x) {
         if (x % 32 == 0) { phys_now = phys_of; pos_now = pos_of; }
         if ((x + NS - 1) % 32 == 0) look_up((x + NS - 1) / 32);
         load(x + NS - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
         __syncwarp();
-        const T *k = ring + x % NS * 2 * TILE, *v = k + TILE;
+        const T *k = ring + place * 2 * TILE, *v = k + TILE;
+        place = place == NS - 1 ? 0 : place + 1;
         const int phys = __shfl_sync(0xffffffffu, phys_now, x % 32), pos = __shfl_sync(0xffffffffu, pos_now, x % 32);
         if (phys >= 0) {
             float s[2][4] = {};
