@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, in
 // counts: any value between the topk-th and the next will do), the border again in 64 bits where it is too close.
 // 65536 rows of up to 128 blocks: TOPKW_US us; 64 steps over 64-bit keys took 65.
 template <int PER, typename T>
-__global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *bounds, const float *scores, const float *q_norms, const float *block_norms,
+__global__ void __launch_bounds__(128, PER <= 4 ? 8 : 1) select_rows_kernel(const T *q, const T *bounds, const float *scores, const float *q_norms, const float *block_norms,
                                                           int32_t *out, int64_t rows, int topk, int64_t H, int64_t D, RowsOfBlocks of) {
     const uint32_t r = blockIdx.x * 4 + threadIdx.x / 32;
     pdl_trigger();
@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *b
     const int64_t s = of.query(r), b = bh / of.Hkv, h = bh - b * of.Hkv;
     const int own = (int)s / of.block, n = of.causal ? own + 1 : of.nb, k = topk < n ? topk : n;
     const float *row = scores + (int64_t)r * of.nb;
+    const float q_norm = q_norms[r];
     uint32_t key[PER];
     float size = 0.f;
     bool odd = false;
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(128) select_rows_kernel(const T *q, const T *b
             odd = __any_sync(0xffffffffu, odd);
             // A product step adds 16 products to the accumulator; aligned to the largest and cut at 24 bits, each of the
             // 17 terms may lose 2^-23 of the largest: 2.1e-6 of the terms' size per step.
-            const float eps = (float)(2 * G * ((D + 15) / 16) + 1) * 2.1e-6f * q_norms[r] * size + 1e-42f;
+            const float eps = (float)(2 * G * ((D + 15) / 16) + 1) * 2.1e-6f * q_norm * size + 1e-42f;
             // the least that is taken and the most that is not
             uint32_t in = 0xffffffffu, not_in = 0;
 #pragma unroll
@@ -571,7 +572,8 @@ __global__ void __launch_bounds__(THREADS) topk_block_kernel(const uint64_t *key
 // 1. Every thread takes the largest fp32 score of its share of the pages; the (topk - 1)-th largest of those maxima is
 //    a floor under the (topk - 1)-th largest score (the token's own page is taken anyway), so no page more than 2 eps
 //    below it can be chosen.  With 256 or 1024 threads and few pages wanted, little more than topk pages remain.
-// 2. The remaining pages, up to kCandidates, are scored again in 64 bits, one warp each.
+// 2. Of the remaining pages, up to kCandidates, those more than 2 eps above or below the wanted rank's score are decided;
+//    the others, where there are more of them than places, are scored again in 64 bits, one warp each.
 // 3. Each candidate counts the candidates that beat it; the winners count the winners before them: their place.
 // Rows where more remain (many equal pages; topk above the number of threads) are scored in 64 bits throughout, by the
 // same warps, and searched bit by bit.
@@ -587,7 +589,9 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
     __shared__ double up[256], down[256];
     __shared__ uint64_t key[kCandidates];
     __shared__ int page_of[kCandidates];
+    __shared__ float score_of[kCandidates], s_kth;
     __shared__ int of_warp[32], tied_of[32], s_count;
+    __shared__ uint32_t s_cut;
     __shared__ float f_warp[32];
     pdl_trigger();
     pdl_wait();
@@ -632,18 +636,40 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
     for (int x = 16; x > 0; x >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, x));
     // a lane adds up to 32 products, the lanes 5 times; the weights are rounded (G times): 2^-24 each of the terms' sizes
     const float eps = (float)(64 + G) * 5.9604645e-8f * size + 1e-42f;
-    // the want-th largest of the threads' maxima, bit by bit
-    uint32_t cut = 0;
-    if (want > 0 && want <= THREADS) {
-        const uint32_t k32 = tid < others ? key32_of(best) : 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t x = cut | (1u << bit);
-            const int cnt = block_sum<THREADS>(k32 >= x, of_warp);
-            if (cnt >= want) cut = x;
-            if (cnt == want) break;
+    // The want-th largest of the threads' maxima, by one warp halving their interval: counts without a barrier (16 warps
+    // that searched bit by bit waited at 64 barriers, a quarter of the kernel).
+    uint32_t *maxima = reinterpret_cast<uint32_t *>(page_of);        // THREADS of them
+    maxima[tid] = tid < others ? key32_of(best) : 0;
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t k32[THREADS / 32], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+        for (int j = 0; j < THREADS / 32; ++j) {
+            k32[j] = maxima[j * 32 + lane];
+            if (k32[j]) { lo = min(lo, k32[j]); hi = max(hi, k32[j]); }
         }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi) + 1;
+        // count(>= hi) = 0; count(>= lo) is the number of maxima: a search is of use where that reaches want
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < THREADS / 32; ++j) c += k32[j] > 0;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (want < 1 || c < want) lo = 0;
+        else
+            while (hi - lo > 1 && c != want) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                int x = 0;
+#pragma unroll
+                for (int j = 0; j < THREADS / 32; ++j) x += k32[j] >= mid;
+                x = __reduce_add_sync(0xffffffffu, x);
+                if (x >= want) { lo = mid; c = x; } else hi = mid;
+            }
+        if (lane == 0) s_cut = lo;
     }
-    // cut 0: fewer maxima than wanted.  An early end leaves cut at or below the want-th maximum: a lower floor.
+    __syncthreads();
+    const uint32_t cut = s_cut;
+    // cut 0: fewer maxima than wanted.  cut is at or below the want-th maximum: at worst a lower floor.
     const float floor = cut == 0 || odd ? -INFINITY : of_key32(cut) - 2.f * eps;
     // 64-bit score of a page, by a warp
     auto exact = [&](int p) {
@@ -665,18 +691,43 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
     };
     if (want > 0)
         for (int i = tid; i < others; i += THREADS)
-            if (odd || mine[i].x >= floor) {
+            if (const float x = mine[i].x; odd || x >= floor) {
                 const int at = atomicAdd(&s_count, 1);       // the order in the list does not matter: ranks are counted
-                if (at < kCandidates) page_of[at] = i;
+                if (at < kCandidates) { page_of[at] = i; score_of[at] = x; }
             }
     __syncthreads();
     const int m = s_count;
     if (m <= kCandidates) {
-        for (int i = warp; i < m; i += THREADS / 32) {
-            const uint64_t k = exact(page_of[i]);
-            if (lane == 0) key[i] = k;
-        }
+        // the score at the wanted rank, in fp32
+        if (!odd)
+            for (int i = tid; i < m; i += THREADS) {
+                const float x = score_of[i];
+                const int p = page_of[i];
+                int before = 0;
+                for (int j = 0; j < m; ++j) before += score_of[j] > x || (score_of[j] == x && page_of[j] < p);
+                if (before == want - 1) s_kth = x;
+            }
         __syncthreads();
+        const float kth = odd || m == 0 ? 0.f : s_kth;
+        int sure = 0, near = 0;
+        for (int i = tid; i < m; i += THREADS) {
+            const float x = score_of[i];
+            const bool above = !odd && x > kth + 2.f * eps, below = !odd && x < kth - 2.f * eps;
+            sure += above;
+            near += !above && !below;
+            key[i] = above ? kOwnKey : below ? 0 : kOwnKey - 1;
+        }
+        sure = block_sum<THREADS>(sure, of_warp);
+        near = block_sum<THREADS>(near, of_warp);
+        __syncthreads();
+        if (sure + near > want) {
+            for (int i = warp; i < m; i += THREADS / 32) {
+                if (key[i] != kOwnKey - 1) continue;
+                const uint64_t k = exact(page_of[i]);
+                if (lane == 0) key[i] = k;
+            }
+            __syncthreads();
+        }
         // rank of each candidate, then (marked by a set sign of its page) its place among the winners
         bool wins[(kCandidates + THREADS - 1) / THREADS];
 #pragma unroll

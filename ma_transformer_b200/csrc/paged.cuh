@@ -3,6 +3,7 @@
 #pragma once
 
 #include "mat_common.cuh"
+#include "ptx.cuh"
 
 namespace mat {
 
@@ -48,26 +49,21 @@ template <> struct Vec16<float> {
         return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
     }
 };
-template <typename T, typename T2> struct Vec16Half {
+template <typename T> struct Vec16Half {
     static constexpr int N = 8;
-    static __device__ __forceinline__ uint32_t two(float a, float b) {
-        T lo = Elem<T>::from_f(a), hi = Elem<T>::from_f(b);
-        return (uint32_t)*reinterpret_cast<uint16_t *>(&lo) | ((uint32_t)*reinterpret_cast<uint16_t *>(&hi) << 16);
-    }
-    static __device__ __forceinline__ float one(uint16_t x) { return Elem<T>::to_f(*reinterpret_cast<T *>(&x)); }
     static __device__ __forceinline__ void unpack(const uint4 &u, float *f) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            f[2 * i] = one((uint16_t)(w[i] & 0xffffu));
-            f[2 * i + 1] = one((uint16_t)(w[i] >> 16));
+            f[2 * i] = ptx::Mma<T>::lo(w[i]);
+            f[2 * i + 1] = ptx::Mma<T>::hi(w[i]);
         }
     }
     static __device__ __forceinline__ uint4 pack(const float *f) {
-        return make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7]));
+        return make_uint4(ptx::Mma<T>::pack(f[0], f[1]), ptx::Mma<T>::pack(f[2], f[3]), ptx::Mma<T>::pack(f[4], f[5]), ptx::Mma<T>::pack(f[6], f[7]));
     }
 };
-template <> struct Vec16<__nv_bfloat16> : Vec16Half<__nv_bfloat16, __nv_bfloat162> {};
-template <> struct Vec16<__half> : Vec16Half<__half, __half2> {};
+template <> struct Vec16<__nv_bfloat16> : Vec16Half<__nv_bfloat16> {};
+template <> struct Vec16<__half> : Vec16Half<__half> {};
 
 }  // namespace mat

@@ -132,12 +132,20 @@ template <int W> struct Unit {
 
 // x: the 2 W values of a unit; c, s: cosine and sine of its pairs
 template <int W> __device__ __forceinline__ void turn(float *x, const float *c, const float *s, bool interleaved) {
+    if (interleaved) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-        const int p = interleaved ? 2 * i : i, q = interleaved ? 2 * i + 1 : W + i;
-        const float a = x[p], b = x[q];
-        x[p] = a * c[i] - b * s[i];
-        x[q] = b * c[i] + a * s[i];
+        for (int i = 0; i < W; ++i) {
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = a * c[i] - b * s[i];
+            x[2 * i + 1] = b * c[i] + a * s[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float a = x[i], b = x[W + i];
+            x[i] = a * c[i] - b * s[i];
+            x[W + i] = b * c[i] + a * s[i];
+        }
     }
 }
 
@@ -146,7 +154,7 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) append
     __shared__ int starts[kKnownStarts + 1];         // first rows of the sequences
     __shared__ int pos_of[64];
     __shared__ int64_t k_of[64], v_of[64];
-    extern __shared__ float turns[];                 // [tile][rot / 2] cosines, then sines
+    extern __shared__ __align__(16) float turns[];                 // [tile][rot / 2] cosines, then sines
     pdl_trigger();
     const int tid = threadIdx.x, D = (int)a.D, half = a.rot / 2;
     const int64_t n0 = (int64_t)blockIdx.x * a.tile;
@@ -230,10 +238,19 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) append
                 if (to[y] < 0) continue;
                 T *out = dst + to[y];
                 if (turned) {
-                    float x[2 * W], c[W], s[W];
+                    float x[2 * W];
+                    __align__(16) float c[W >= 4 ? W : 4], s[W >= 4 ? W : 4];
                     const int first = (t0 + y * lanes) * half + u.pair;
+                    if (VEC) {
 #pragma unroll
-                    for (int i = 0; i < W; ++i) { c[i] = cosines[first + i]; s[i] = sines[first + i]; }
+                        for (int i = 0; i < W; i += 4) {      // a unit's pairs start on 16 bytes: rot is a multiple of 2 W
+                            *reinterpret_cast<float4 *>(c + i) = *reinterpret_cast<const float4 *>(cosines + first + i);
+                            *reinterpret_cast<float4 *>(s + i) = *reinterpret_cast<const float4 *>(sines + first + i);
+                        }
+                    } else {
+                        c[0] = cosines[first];
+                        s[0] = sines[first];
+                    }
                     if (VEC) {
                         Vec16<T>::unpack(raw[y][0], x);
                         Vec16<T>::unpack(raw[y][1], x + W);
