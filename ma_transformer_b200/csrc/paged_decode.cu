@@ -49,16 +49,22 @@ struct RowTokens {
         } else if (a.pages) {
             list = a.pages + (b * a.Hkv + h) * a.n_sel;
             n = a.n_sel << a.c.page_shift;
-        } else if (a.left < 0) {
-            n = len;
         } else {
-            dil = a.dilation;
-            const int64_t back = dil == 1 ? len - 1 : (len - 1) / dil;
-            n = (a.left < back ? a.left : back) + 1;
-            first = lo = len - 1 - (n - 1) * dil;
-            if (a.aligned) {
-                first = lo / 16 * 16;
-                n += lo - first;
+            // tokens past the end of the table are absent
+            const int64_t cap = a.c.width << a.c.page_shift;
+            if (len > cap && threadIdx.x == 0) atomicOr(a.status, kPagedOutside);
+            if (a.left < 0) {
+                n = len < cap ? len : cap;
+            } else {
+                dil = a.dilation;
+                const int64_t back = dil == 1 ? len - 1 : (len - 1) / dil;
+                n = (a.left < back ? a.left : back) + 1;
+                first = lo = len - 1 - (n - 1) * dil;
+                if (len > cap) n = first < cap ? (cap - first + dil - 1) / dil : 0;
+                if (a.aligned) {
+                    first = lo / 16 * 16;
+                    n += n > 0 ? lo - first : 0;
+                }
             }
         }
     }

@@ -318,9 +318,27 @@ def test_pages_outside_the_cache_count_as_absent_and_are_reported():
     keep = [i for i in range(100) if i // 16 not in (2, 4)]
     o, A, E = attend(q[0], logical[0][0][keep], logical[0][1][keep], 1 / 8)
     assert ((out[0] - o).abs() <= allowance(o, A, E, D, dtype)).all()
-    n.fill_(100 + 16 * 50)                            # longer than the table is wide
-    paged.decode(q.cuda(), cache, table.cuda(), n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("spec, first", [(None, 0), (PatternSpec.causal_window(50), 249 - 49), (PatternSpec.causal_window(40, 2), 249 - 78),
+                                         (PatternSpec.causal_window(3), 249 - 2)])
+def test_a_length_past_the_table_reads_what_the_table_holds(dtype, spec, first):
+    """A sequence of 250 tokens whose table stops after 208, and the largest length there is."""
+    k, v, _, table, logical = make_cache([208], 16, 2, 64, dtype)
+    cache = mt.PagedKVCache.from_tensors(k.cuda(), v.cuda())
+    q = torch.randn(1, 4, 64).to(dtype)
+    n = torch.tensor([250], dtype=torch.int32, device="cuda")
+    step = spec.dilation if spec else 1
+    pos = [p for p in range(first, 208) if (p - first) % step == 0]
+    out = paged.decode(q.cuda(), cache, table.cuda(), n, spec=spec).cpu().double()
     assert nat.device_status() == 2
+    o, A, E = attend(q[0], logical[0][0][pos], logical[0][1][pos], 1 / 8)
+    assert ((out[0] - o).abs() <= allowance(o, A, E, 64, dtype)).all()
+    n.fill_(2 ** 31 - 1)
+    out = paged.decode(q.cuda(), cache, table.cuda(), n, spec=spec)
+    assert nat.device_status() == 2 and (spec is None or not out.any())
 
 
 @pytest.mark.gpu

@@ -179,18 +179,42 @@ def test_selection_of_equal_scores_takes_the_lower_block():
 
 
 @pytest.mark.gpu
-def test_selection_of_many_blocks():
-    """More blocks than one warp's registers hold, more score rows than are held at a time."""
-    q, k, _, _ = inputs(1, 20000, 2, 1, 8, torch.float32)
-    got = sel.select_blocks(q.cuda(), k.cuda(), 16, 7, True).cpu()
-    for s in (0, 15, 16, 5000, 16399, 19999):
-        qs, ks = q[:, s // 16 * 16:s // 16 * 16 + 16], k[:, :s // 16 * 16 + 16]
-        lo, hi = (f(ks.double().view(-1, 16, 8), 1) for f in (torch.amin, torch.amax))
-        row = q[0, s].double()
-        score = (row.clamp(min=0).sum(0) * hi + row.clamp(max=0).sum(0) * lo).sum(-1)
-        own = s // 16
-        rank = sorted(range(own + 1), key=lambda n: (n != own, -float(score[n]), n))[:7]
-        assert got[0, s, 0].tolist() == sorted(rank) + [-1] * (7 - len(rank))
+@pytest.mark.parametrize("S, Hkv, dtype", [(20000, 1, torch.float32), (20000, 1, torch.bfloat16), (16384, 4, torch.bfloat16), (6000, 2, torch.float16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_selection_of_many_blocks(S, Hkv, dtype, causal):
+    """More blocks than one warp's registers hold, more score rows than are held at a time, every width of row."""
+    q, k, _, _ = inputs(1, S, 2 * Hkv, Hkv, 16, dtype)
+    got = sel.select_blocks(q.cuda(), k.cuda(), 16, 7, causal).cpu()
+    nb = S // 16
+    kb = k[0].double().view(nb, 16, Hkv, 16)
+    lo, hi = kb.amin(1), kb.amax(1)
+    for s in (0, 15, 16, 111, 112, 2047, 2048, 5000, 5999, S // 2, S - 17, S - 1):
+        if s >= S:
+            continue
+        for h in range(Hkv):
+            row = q[0, s, 2 * h:2 * h + 2].double()
+            score = (row.clamp(min=0).sum(0) * hi[:, h] + row.clamp(max=0).sum(0) * lo[:, h]).sum(-1)
+            own = s // 16
+            last = own + 1 if causal else nb
+            rank = sorted(range(last), key=lambda n: (n != own, -float(score[n]), n))[:7]
+            assert got[0, s, h].tolist() == sorted(rank) + [-1] * (7 - len(rank)), (s, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scores_nearer_than_their_fp32_error_are_ordered_in_64_bits(dtype):
+    """Blocks whose bounds differ in one column's last bit: fp32 sums cannot tell most of them apart."""
+    S, block, D = 1280, 16, 64
+    g = torch.Generator().manual_seed(11)
+    k = torch.randn(1, 1, 1, D, generator=g).to(dtype).expand(1, S, 1, D).contiguous() * 8
+    for n in range(S // block):                           # one element of a block a step larger, another column each
+        c = (n * 7) % D
+        x = k[0, n * block, 0, c].float()
+        k[0, n * block, 0, c] = (x + x.abs() * torch.finfo(dtype).eps).to(dtype)
+    q = torch.randn(1, S, 2, D, generator=g).to(dtype) * 1e-3
+    q[..., 0] = 30
+    got = sel.select_blocks(q.cuda(), k.cuda(), block, 9, True).cpu()
+    assert torch.equal(got, plain_select(q, k, block, 9, True))
 
 
 # ---- attention and gradients --------------------------------------------------------------------------------
