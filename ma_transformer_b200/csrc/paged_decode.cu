@@ -30,6 +30,7 @@ struct DecodeArgs {
     int64_t n_sel;
     float scale_log2;
     int G, nsplit, min_chunk, tiles;   // tiles: groups of query heads per key head
+    int cluster;                    // the chunks of a row are one cluster
     int aligned;                    // the kernel reads 16 neighbouring positions at a time: first is a multiple of 16
     float2 *stats;                  // [B, H, nsplit] (maximum, sum)
     float *part;                    // [B, H, nsplit, D]
@@ -84,10 +85,61 @@ struct RowTokens {
     }
 };
 
+// Rows of few chunks: the chunks' CTAs form a cluster and join through each other's shared memory, without a workspace
+// and a second launch (8 rows of 777 tokens: a call of CLUSTER_US us against 15.2).  Every CTA of the cluster stays to the end,
+// so this is for launches that fit the GPU at once.  `mine`: [heads][cols + 4] unnormalised outputs, then maximum and sum
+// in the last columns; the CTAs share the (head, 4 columns) items.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(const void *p, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(ptx::smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float4 peer_load(uint32_t a) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(a) : "memory");
+    return x;
+}
+template <typename T> __device__ __forceinline__ void cluster_join(const DecodeArgs &a, const float *mine, int heads, int pitch, int64_t head0) {
+    __syncthreads();
+    cluster_sync();
+    const int vecs = (int)a.D / 4, n = a.nsplit;
+    for (int x = blockIdx.y * 128 + threadIdx.x; x < heads * vecs; x += n * 128) {
+        const int g = x / vecs, col = x % vecs * 4;
+        const float *row = mine + g * pitch;
+        float4 st[8], u[8];
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < n) {
+                st[r] = peer_load(peer_smem(row + pitch - 4, r));
+                u[r] = peer_load(peer_smem(row + col, r));
+                top = fmaxf(top, st[r].x);
+            }
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < n) {
+                const float e = exp2f(st[r].x - ref);
+                sum += st[r].y * e;
+                y.x = fmaf(u[r].x, e, y.x); y.y = fmaf(u[r].y, e, y.y); y.z = fmaf(u[r].z, e, y.z); y.w = fmaf(u[r].w, e, y.w);
+            }
+        const float f = sum == 0.f ? 0.f : 1.f / sum;
+        T *o = (T *)a.o + (head0 + g) * a.D + col;
+        o[0] = Elem<T>::from_f(y.x * f); o[1] = Elem<T>::from_f(y.y * f); o[2] = Elem<T>::from_f(y.z * f); o[3] = Elem<T>::from_f(y.w * f);
+    }
+    __syncthreads();
+    cluster_sync();                                  // nobody leaves while its shared memory is read
+}
+
 // ---- one warp per few keys, fp32 arithmetic: any type ---------------------------------------------------------------
 // LPK lanes hold one key's columns, NV 16-byte vectors each (lanes past D idle); a warp scores 32 / LPK keys at a time,
 // U times unrolled so that their loads are in flight together.  GT query heads per CTA.
-template <typename T, int LPK, int NV, int GT, int U>
+template <typename T, int LPK, int NV, int GT, int U, bool CLUSTER>
 __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     constexpr int W = Vec16<T>::N, KPW = 32 / LPK, C = NV * W;
     const int64_t b = blockIdx.z, h = blockIdx.x / (unsigned)a.tiles, g0 = (int64_t)(blockIdx.x % (unsigned)a.tiles) * GT;
@@ -97,7 +149,7 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a), t0 = blockIdx.y * chunk;
     const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
-    if (t0 >= row.n && blockIdx.y > 0) return;
+    if (!CLUSTER && t0 >= row.n && blockIdx.y > 0) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, part = lane % LPK, key = lane / LPK;
 
     float q[GT][C], acc[GT][C], m[GT], l[GT];
@@ -183,7 +235,7 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
         }
     }
     // join the key lanes of a warp, then the warps
-    extern __shared__ float sm[];        // [4][GT][D + 2]
+    extern __shared__ __align__(16) float sm[];        // [4][GT][D + 2], then for a cluster [GT][D + 4]
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
 #pragma unroll
@@ -220,11 +272,14 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
         for (int d = threadIdx.x; d < D; d += 128) {
             float x = 0.f;
             for (int i = 0; i < 4; ++i) x += w[i * stride + 2 + d] * e[i];
-            if (whole) ((T *)a.o)[head * D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x * inv);
+            if (CLUSTER) sm[4 * GT * (D + 2) + g * (D + 4) + d] = x;
+            else if (whole) ((T *)a.o)[head * D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x * inv);
             else a.part[(head * a.nsplit + blockIdx.y) * D + d] = x;
         }
-        if (!whole && threadIdx.x == 0) a.stats[head * a.nsplit + blockIdx.y] = make_float2(top, sum);
+        if (CLUSTER && threadIdx.x < 2) sm[4 * GT * (D + 2) + g * (D + 4) + D + threadIdx.x] = threadIdx.x ? sum : top;
+        else if (!whole && threadIdx.x == 0) a.stats[head * a.nsplit + blockIdx.y] = make_float2(top, sum);
     }
+    if (CLUSTER) cluster_join<T>(a, sm + 4 * GT * (D + 2), (int)(G - g0 < GT ? G - g0 : GT), D + 4, b * a.H + h * G + g0);
 }
 
 // ---- 16-bit types on the tensor cores ---------------------------------------------------------------------------------
@@ -238,7 +293,7 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) 
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) decode_mma_kernel(const DecodeArgs a) {
+template <typename T, int DP, int NS, bool CLUSTER> __global__ void __launch_bounds__(128) decode_mma_kernel(const DecodeArgs a) {
     constexpr int PITCH = DP + 8, TILE = 16 * PITCH, CH = DP / 8;
     const int64_t b = blockIdx.z, h = blockIdx.x / (unsigned)a.tiles, G = a.G;
     const int g0 = (int)(blockIdx.x % (unsigned)a.tiles) * 16, heads = min(16, (int)G - g0);
@@ -247,7 +302,7 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a), t0 = blockIdx.y * chunk;
     const int64_t t1 = t0 + chunk < row.n ? t0 + chunk : row.n;
-    if (t0 >= row.n && blockIdx.y > 0) return;
+    if (!CLUSTER && t0 >= row.n && blockIdx.y > 0) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     extern __shared__ __align__(16) char smem[];
     T *ring = (T *)smem + warp * NS * 2 * TILE;          // NS x (16 keys, 16 values)
@@ -436,7 +491,11 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
             y.x = fmaf(u.x, e, y.x); y.y = fmaf(u.y, e, y.y); y.z = fmaf(u.z, e, y.z); y.w = fmaf(u.w, e, y.w);
         }
         const int64_t head = b * a.H + h * G + g0 + g;
-        if (whole) {
+        if (CLUSTER) {
+            float *mine_row = ls + 64 + g * (DP + 4);
+            *reinterpret_cast<float4 *>(mine_row + col) = y;
+            if (col == 0) *reinterpret_cast<float4 *>(mine_row + DP) = make_float4(top, sum, 0.f, 0.f);
+        } else if (whole) {
             const float f = sum == 0.f ? 0.f : 1.f / sum;
             T z[4] = {Elem<T>::from_f(y.x * f), Elem<T>::from_f(y.y * f), Elem<T>::from_f(y.z * f), Elem<T>::from_f(y.w * f)};
             *reinterpret_cast<uint2 *>((T *)a.o + head * D + col) = *reinterpret_cast<uint2 *>(z);
@@ -445,6 +504,7 @@ template <typename T, int DP, int NS> __global__ void __launch_bounds__(128) dec
             if (col == 0) a.stats[head * a.nsplit + blockIdx.y] = make_float2(top, sum);
         }
     }
+    if (CLUSTER) cluster_join<T>(a, ls + 64, heads, DP + 4, b * a.H + h * G + g0);
 }
 
 // ---- joining the chunks of a row -------------------------------------------------------------------------------------
@@ -545,14 +605,29 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
     o[0] = Elem<T>::from_f(x.x * f); o[1] = Elem<T>::from_f(x.y * f); o[2] = Elem<T>::from_f(x.z * f); o[3] = Elem<T>::from_f(x.w * f);
 }
 
+int launch_rows(void (*kernel)(const DecodeArgs), const DecodeArgs &a, size_t smem, cudaStream_t s) {
+    if (int rc = ensure_dynamic_smem((const void *)kernel, smem, "shared memory of the paged decode")) return rc;
+    cudaLaunchConfig_t cfg = {};
+    // heads fastest: the CTAs that read neighbouring rows of a page run side by side
+    cfg.gridDim = dim3((unsigned)(a.Hkv * a.tiles), (unsigned)a.nsplit, (unsigned)a.B);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)a.nsplit;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode");
+}
+
 template <typename T, int LPK, int NV, int GT> int launch_simt(const DecodeArgs &a, cudaStream_t s) {
     constexpr int U = NV == 1 ? 4 : 2;
-    // heads fastest: the CTAs that read neighbouring rows of a page run side by side
-    dim3 grid((unsigned)(a.Hkv * a.tiles), (unsigned)a.nsplit, (unsigned)a.B);
-    const size_t smem = 4 * GT * (a.D + 2) * sizeof(float);
-    decode_simt_kernel<T, LPK, NV, GT, U><<<grid, 128, smem, s>>>(a);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode");
+    const size_t smem = (4 * GT * (a.D + 2) + (a.cluster ? GT * (a.D + 4) : 0)) * sizeof(float);
+    return launch_rows(a.cluster ? decode_simt_kernel<T, LPK, NV, GT, U, true> : decode_simt_kernel<T, LPK, NV, GT, U, false>, a, smem, s);
 }
 
 template <typename T, int LPK, int NV> int launch_simt_heads(const DecodeArgs &a, int gt, cudaStream_t s) {
@@ -564,14 +639,8 @@ template <typename T, int LPK, int NV> int launch_simt_heads(const DecodeArgs &a
 }
 
 template <typename T, int DP, int NS> int launch_mma(const DecodeArgs &a, cudaStream_t s) {
-    const size_t ring = 4 * NS * 2 * 16 * (DP + 8) * sizeof(T), res = (4 * 16 * (DP + 4) + 128) * sizeof(float);
-    const size_t smem = ring > res ? ring : res;
-    if (int rc = ensure_dynamic_smem((const void *)decode_mma_kernel<T, DP, NS>, smem, "shared memory of the paged decode")) return rc;
-    // heads fastest: the CTAs that read neighbouring rows of a page run side by side
-    dim3 grid((unsigned)(a.Hkv * a.tiles), (unsigned)a.nsplit, (unsigned)a.B);
-    decode_mma_kernel<T, DP, NS><<<grid, 128, smem, s>>>(a);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode");
+    const size_t ring = 4 * NS * 2 * 16 * (DP + 8) * sizeof(T), res = ((a.cluster ? 5 : 4) * 16 * (DP + 4) + 128) * sizeof(float);
+    return launch_rows(a.cluster ? decode_mma_kernel<T, DP, NS, true> : decode_mma_kernel<T, DP, NS, false>, a, ring > res ? ring : res, s);
 }
 
 template <typename T> int run_simt(DecodeArgs &a, cudaStream_t s) {
@@ -592,7 +661,7 @@ template <> int run_mma<float>(DecodeArgs &a, cudaStream_t s) { return run_simt<
 
 template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
     const int rc = a.aligned ? run_mma<T>(a, s) : run_simt<T>(a, s);
-    if (rc || a.nsplit == 1) return rc;
+    if (rc || a.nsplit == 1 || a.cluster) return rc;
     const cudaError_t e = a.nsplit <= 32 ? launch_after(join_few_kernel<T>, dim3((unsigned)((a.H * a.B + 3) / 4)), dim3(128), 0, s, a)
                                          : launch_after(join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B), dim3(256), 0, s, a);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode's join");
@@ -600,22 +669,30 @@ template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
 
 // How many chunks a row may have, and their least size.  The lengths are on the device, so both come from the page
 // table's width; the kernels shorten the chunks' number, not their size, for shorter rows.
-void plan(const mat_paged_cache *c, int64_t B, int64_t H, int64_t width, int64_t left, int64_t n_sel, bool list,
-          int &nsplit, int &min_chunk) {
+struct DecodePlan { int nsplit, min_chunk, cluster; };
+
+DecodePlan plan(const mat_paged_cache *c, int64_t B, int64_t width, int64_t left, int64_t n_sel) {
     int64_t most = width * c->page_size;
-    if (list) most = n_sel * c->page_size;
+    if (n_sel > 0) most = n_sel * c->page_size;
     else if (left >= 0 && left + 16 < most) most = left + 16;   // up to 15 tokens before the window's first
     const int64_t rows = B * c->H_kv;
+    DecodePlan p;
+    if (rows * 8 <= kSms && most <= 8192) {       // one cluster of at most eight chunks per row, all of them resident
+        p.min_chunk = 64;
+        p.nsplit = (int)(most >= 8 * 64 ? 8 : (most + 63) / 64);
+        p.cluster = p.nsplit > 1;
+        return p;
+    }
     // Every CTA pays some 4 us to look up its pages, fill its rings and write its result.  64 sequences of up to 8192
     // tokens x 8 key heads of 128: 172 us with chunks of 512 tokens and more, 163 with 1024, 159 with 2048; 32 x 2048
-    // chosen tokens x 8: 78, 61, 53 us.  Few rows need the shorter chunks to fill the GPU: one sequence of 777 tokens x
-    // 8 heads has 7 x 8 CTAs with chunks of 128.
-    min_chunk = rows >= kSms ? 2048 : rows >= 16 ? 512 : 128;
+    // chosen tokens x 8: 78, 61, 53 us.  Few rows need the shorter chunks to fill the GPU.
+    p.min_chunk = rows >= kSms ? 2048 : rows >= 16 ? 512 : 128;
     int64_t cap = 16 * kSms / rows;
     if (cap < 8) cap = 8;
-    int64_t n = (most + min_chunk - 1) / min_chunk;
-    nsplit = (int)(n < 1 ? 1 : n > cap ? cap : n);
-    (void)H;
+    const int64_t n = (most + p.min_chunk - 1) / p.min_chunk;
+    p.nsplit = (int)(n < 1 ? 1 : n > cap ? cap : n);
+    p.cluster = p.nsplit > 1 && p.nsplit <= 8 && rows * p.nsplit <= kSms;
+    return p;
 }
 
 int check_decode(const mat_paged_cache *c, int64_t B, int64_t H, int64_t left, int64_t n_sel) {
@@ -636,10 +713,9 @@ using namespace mat;
 extern "C" size_t mat_paged_decode_workspace_bytes(const mat_paged_cache *cache, int64_t B, int64_t H, int64_t table_width,
                                                    int64_t left, int64_t n_sel) {
     if (check_paged_cache(cache) || B < 1 || H < 1 || table_width < 1 || check_decode(cache, B, H, left, n_sel)) return 0;
-    int nsplit, min_chunk;
-    plan(cache, B, H, table_width, left, n_sel, n_sel > 0, nsplit, min_chunk);
-    if (nsplit == 1) return 0;
-    return align256((size_t)B * H * nsplit * sizeof(float2)) + (size_t)B * H * nsplit * cache->D * sizeof(float);
+    const DecodePlan p = plan(cache, B, table_width, left, n_sel);
+    if (p.nsplit == 1 || p.cluster) return 0;
+    return align256((size_t)B * H * p.nsplit * sizeof(float2)) + (size_t)B * H * p.nsplit * cache->D * sizeof(float);
 }
 
 extern "C" int mat_paged_decode(const mat_paged_cache *cache, const void *q, int64_t q_stride, void *o, int64_t B, int64_t H,
@@ -666,7 +742,8 @@ extern "C" int mat_paged_decode(const mat_paged_cache *cache, const void *q, int
     a.lengths = lengths; a.left = left; a.dilation = dilation;
     a.pages = pages; a.n_sel = n_sel;
     a.scale_log2 = (scale > 0.f ? scale : 1.0f / std::sqrt((float)cache->D)) * 1.4426950408889634f;
-    plan(cache, B, H, table_width, left, n_sel, pages != nullptr, a.nsplit, a.min_chunk);
+    const DecodePlan w = plan(cache, B, table_width, left, pages ? n_sel : 0);
+    a.nsplit = w.nsplit; a.min_chunk = w.min_chunk; a.cluster = w.cluster;
     a.stats = (float2 *)workspace;
     a.part = (float *)((char *)workspace + align256((size_t)B * H * a.nsplit * sizeof(float2)));
     if (!(a.status = paged_status_word())) return fail(MAT_ERR_CUDA, "no device status word");
