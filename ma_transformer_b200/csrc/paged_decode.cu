@@ -86,7 +86,7 @@ struct RowTokens {
 };
 
 // Rows of few chunks: the chunks' CTAs form a cluster and join through each other's shared memory, without a workspace
-// and a second launch (8 rows of 777 tokens: a call of CLUSTER_US us against 15.2).  Every CTA of the cluster stays to the end,
+// and a second launch (8 rows of 777 tokens: a call of 10.6 us against 15.2).  Every CTA of the cluster stays to the end,
 // so this is for launches that fit the GPU at once.  `mine`: [heads][cols + 4] unnormalised outputs, then maximum and sum
 // in the last columns; the CTAs share the (head, 4 columns) items.
 __device__ __forceinline__ void cluster_sync() {
