@@ -5,11 +5,11 @@
 //     sum_g sum_d max(q_gd lo_d, q_gd hi_d) = sum_d up_d hi_d + down_d lo_d,
 //     up_d = sum_g max(q_gd, 0), down_d = sum_g min(q_gd, 0):
 // one dot product of 2 D terms whatever G is, and an upper bound of the group's summed q . k over the block's keys.
-// Bounds are exact in the keys' type, and scores are formed and compared in 64 bits, so a selection does not depend on
-// how the sums are split: two blocks change places only where their true scores agree to about 1e-15.
+// Bounds are exact in the keys' type, and a selection is the one that scores in 64 bits give, so it does not depend on how
+// sums are split: two blocks change places only where their true scores agree to about 1e-15.
 //
-// 64-bit scores of everything would be the whole cost (conversions and 64-bit adds at an eighth of the fp32 rate), and
-// few of them matter.  So scores are first formed in fp32 with a bound eps on their error; what lies more than 2 eps
+// Few scores are needed to 64 bits, and all of them in 64 bits cost more than the rest of a selection (159 us of 221 for
+// 65536 rows of up to 128 blocks of 64-column keys, where fp32 takes 22).  So scores are first formed in fp32 with a bound eps on their error; what lies more than 2 eps
 // above or below the topk-th largest is decided by that, and the rest is scored again in 64 bits.  Where the two scores
 // at the border are nearer than 2 eps to many others (equal keys, say), all of those are scored again: slower, not
 // different.  A 64-bit score becomes a key whose order as an integer is the score's (NaN lowest, the query's own block
@@ -239,6 +239,9 @@ __global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float
 }
 
 // ---- scores of a cache's pages ---------------------------------------------------------------------------------------
+// Bound by latency at the sizes that occur: 16 us for 15625 pages x 8 heads of 64 (32 MB: 5 us), most of it the chain
+// length -> table -> bounds -> sum over lanes.
+//
 // LP lanes share a page: a lane holds the weights of its NV vectors (of the 2 D bounds: smallest keys, then largest) in
 // registers and reads four pages' vectors at once.  Leaves (score, sum of the terms' absolute values) in fp32 for pages
 // first, first + step, ... of a row; `threads` threads take part.
@@ -389,7 +392,8 @@ __global__ void __launch_bounds__(128) topk_warp_kernel(const uint64_t *keys, in
 
 // One warp per row over fp32 scores: the topk-th largest by halving the interval of the scores' integers (about ten
 // counts: any value between the topk-th and the next will do), the border again in 64 bits where it is too close.
-// 65536 rows of up to 128 blocks: TOPKW_US us; 64 steps over 64-bit keys took 65.
+// 65536 rows of up to 128 blocks: 60 us, 640 instructions a row at 2.5 a clock (64 steps over 64-bit keys: 65 us, behind
+// scores that took 159 us in 64 bits where these take 22).
 template <int PER, typename T>
 __global__ void __launch_bounds__(128, PER <= 4 ? 8 : 1) select_rows_kernel(const T *q, const T *bounds, const float *scores, const float *q_norms, const float *block_norms,
                                                           int32_t *out, int64_t rows, int topk, int64_t H, int64_t D, RowsOfBlocks of) {

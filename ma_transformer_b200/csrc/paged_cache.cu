@@ -6,9 +6,9 @@
 // before it is rounded to fp32 (an fp32 product would be off by p * f * 2^-24: 0.06 rad at position 10^6).
 //
 // append_rows_kernel streams: a CTA takes a tile of tokens with all their heads, finds each token's sequence, page and
-// angles once (a chain of five dependent reads), and then moves 2 x 16 bytes per thread and step.  One CTA per page and
-// key head paid that chain per 10 KB and took 177 us (100 us with 8-byte vectors and more CTAs) where this takes
-// PROMPTS_US us: 7 prompts, 32768 tokens x (12 + 2 * 4) heads of 64 in fp16, 172 MB, 27 us at the copy rate.
+// angles once (a chain of five dependent reads), and then moves 2 x 16 bytes per thread and step.  7 prompts, 32768
+// tokens x (12 + 2 * 4) heads of 64 in fp16, 172 MB, 27 us at the copy rate: 33 us (46 us a call with the bounds).  One
+// CTA per page and key head paid that chain per 10 KB: 177 us, 100 us with 8-byte vectors and more CTAs.
 //
 // page_bounds_kernel follows where the cache keeps bounds: one warp owns one page and head and takes its bounds from all
 // filled slots (the new ones come from L2), so there are no atomics, and a cache that was rolled back and written again

