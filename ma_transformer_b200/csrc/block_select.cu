@@ -276,7 +276,7 @@ __device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds,
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int p = p0 + u * step + threadIdx.x / LP;
-            next[u] = p < n ? (int)physical_page(c, b, p, status) : -1;
+            next[u] = p < n ? table_entry(c, b, p) : -1;
         }
     };
     look_up(first);
@@ -284,7 +284,7 @@ __device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds,
         uint4 x[U][NV];
         int64_t phys[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) phys[u] = next[u];
+        for (int u = 0; u < U; ++u) phys[u] = next[u] < c.n_pages ? next[u] : -1;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -310,7 +310,7 @@ __device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds,
                 size += __shfl_xor_sync(0xffffffffu, size, o);
             }
             const int p = p0 + u * step + threadIdx.x / LP;
-            // a page outside the cache is no number: it sends its row to the 64-bit scores, where it ranks last
+            // a page outside the cache is no number: it sends its row to the 64-bit scores, which report it and rank it last
             if (part == 0 && p < n) scores[p] = make_float2(phys[u] < 0 ? -INFINITY : s, size);
         }
     }
@@ -708,6 +708,7 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
                 const float x = score_of[i];
                 const int p = page_of[i];
                 int before = 0;
+#pragma unroll 8
                 for (int j = 0; j < m; ++j) before += score_of[j] > x || (score_of[j] == x && page_of[j] < p);
                 if (before == want - 1) s_kth = x;
             }
@@ -742,6 +743,7 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
                 const uint64_t k = key[i];
                 const int p = page_of[i];
                 int before = 0;
+#pragma unroll 8
                 for (int j = 0; j < m; ++j) before += key[j] > k || (key[j] == k && page_of[j] < p);
                 wins[y] = before < want;
             }
@@ -759,6 +761,7 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, cons
             if (i < m && wins[y]) {
                 const int p = page_of[i];
                 int before = 0;
+#pragma unroll 8
                 for (int j = 0; j < m; ++j) before += page_of[j] < p;
                 o[before] = p;
             }

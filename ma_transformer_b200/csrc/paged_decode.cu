@@ -173,13 +173,19 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     for (int64_t base = t0 + warp * (KPW * U); base < t1; base += 4 * KPW * U) {
         uint4 kv[U][NV], vv[U][NV];
         bool ok[U];
+        int64_t at[U];
+        int32_t entry[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t t = base + u * KPW + key;
-            const int64_t pos = t < t1 ? row.position(a, t) : -1;
-            const int64_t phys = pos >= 0 ? physical_page(a.c, b, pos >> a.c.page_shift, a.status) : -1;
-            ok[u] = phys >= 0;
-            const int64_t slot = pos & ((1 << a.c.page_shift) - 1);
+            at[u] = t < t1 ? row.position(a, t) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) entry[u] = at[u] >= 0 ? table_entry(a.c, b, at[u] >> a.c.page_shift) : -1;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ok[u] = entry[u] >= 0 && entry[u] < a.c.n_pages;
+            const int64_t phys = entry[u], slot = at[u] & ((1 << a.c.page_shift) - 1);
             const T *kr = (const T *)a.c.k + phys * a.c.k_page + slot * a.c.k_tok + h * a.c.k_head;
             const T *vr = (const T *)a.c.v + phys * a.c.v_page + slot * a.c.v_tok + h * a.c.v_head;
 #pragma unroll
@@ -190,6 +196,9 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
                 vv[u][i] = in ? __ldg(reinterpret_cast<const uint4 *>(vr + col)) : make_uint4(0, 0, 0, 0);
             }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (at[u] >= 0) entry_inside(a.c, entry[u], a.status);
         float s[U][GT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
