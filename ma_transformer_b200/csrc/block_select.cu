@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float
 template <typename T, int LP, int NV>
 __device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds, const T *q, int64_t H, int64_t Hkv, int64_t D, int64_t b, int64_t h,
                                             int n, int first, int step, float2 *scores, int *status) {
-    constexpr int W = Vec16<T>::N, U = NV >= 4 ? 2 : 4;
+    constexpr int W = Vec16<T>::N, U = NV >= 4 ? 1 : NV == 2 ? 2 : 4;
     const int64_t G = H / Hkv;
     const int part = threadIdx.x % LP, vecs = (int)D / W;
     float w[NV][W];
@@ -585,7 +585,7 @@ constexpr int kCandidates = 1024;
 
 // LP > 0: the CTA scores its row's pages itself first (rows enough to fill the GPU with one CTA each).
 template <typename T, int THREADS, int LP, int NV>
-__global__ void __launch_bounds__(THREADS) select_pages_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1) select_pages_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
                                                                const int32_t *lengths, float2 *scores, int32_t *out, int topk, int *status) {
     constexpr int W = Vec16<T>::N;
     const int64_t b = blockIdx.y, h = blockIdx.x, G = H / Hkv, row = b * Hkv + h;
@@ -901,15 +901,15 @@ template <typename T>
 int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, int64_t q_stride, int64_t B, int64_t H, const int32_t *lengths,
                      int64_t topk, int32_t *pages, float2 *scores, int *status, cudaStream_t s) {
     const int vecs = 2 * (int)c->D / Vec16<T>::N;            // of one page and head
-    const int lp = vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32;
+    const int lp = vecs <= 8 ? 8 : vecs <= 32 ? 16 : 32;
     const T *bounds = (const T *)c->key_bounds;
     const dim3 rows((unsigned)c->H_kv, (unsigned)B);
     cudaError_t e;
     if (B * c->H_kv >= 148) {
 #define SELECT_PAGES(LP, NV) select_pages_kernel<T, 512, LP, NV><<<rows, 512, 0, s>>>(v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, pages, (int)topk, status)
         if (lp == 8) SELECT_PAGES(8, 1);
-        else if (lp == 16) SELECT_PAGES(16, 1);
-        else if (vecs <= 32) SELECT_PAGES(32, 1);
+        else if (vecs <= 16) SELECT_PAGES(16, 1);
+        else if (vecs <= 32) SELECT_PAGES(16, 2);
         else if (vecs <= 64) SELECT_PAGES(32, 2);
         else SELECT_PAGES(32, 4);
 #undef SELECT_PAGES
@@ -922,8 +922,8 @@ int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, i
     const dim3 grid((unsigned)gx, (unsigned)c->H_kv, (unsigned)B);
 #define PAGE_SCORES(LP, NV) page_scores_kernel<T, LP, NV><<<grid, 256, 0, s>>>(v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, status)
     if (lp == 8) PAGE_SCORES(8, 1);
-    else if (lp == 16) PAGE_SCORES(16, 1);
-    else if (vecs <= 32) PAGE_SCORES(32, 1);
+    else if (vecs <= 16) PAGE_SCORES(16, 1);
+    else if (vecs <= 32) PAGE_SCORES(16, 2);
     else if (vecs <= 64) PAGE_SCORES(32, 2);
     else PAGE_SCORES(32, 4);
 #undef PAGE_SCORES
