@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
     if ((int)blockIdx.x >= t.item_base[(int64_t)bh * (p.nb + 1) + p.nb]) return;
     const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
     const int n = item.x, e0 = t.l.base[(int64_t)bh * (p.nb + 1) + n], D = (int)p.D, pitch = D + 4, T_ = (int)p.topk, vecs = D / 4;
-    const int rows_all = (t.l.base[(int64_t)bh * (p.nb + 1) + n + 1] - e0) * t.G, r_end = min(item.y + kF32Rows, rows_all);
+    const int rows_all = (t.l.base[(int64_t)bh * (p.nb + 1) + n + 1] - e0) * t.G, r_end = min(item.y + kF32BwdRows, rows_all);
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
     const int keys = min((int)p.block - sub * 64, 64), held = (int)max((int64_t)0, min((int64_t)keys, p.S - j0));
     if (held == 0) return;                                   // the sequence ends before this half
