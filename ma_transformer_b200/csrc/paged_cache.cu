@@ -398,6 +398,7 @@ extern "C" int mat_paged_append(const mat_paged_cache *cache, const void *k_new,
     if (!k_new || !v_new || !start) return fail(MAT_ERR_INVALID, "k_new, v_new and start must be non-NULL");
     if ((q == nullptr) != (q_out == nullptr)) return fail(MAT_ERR_INVALID, "q and q_out come together");
     const int64_t D = cache->D, Hkv = cache->H_kv, vec = 16 / (int64_t)dtype_size(cache->dtype);
+    if (q && H > 65535) return fail(MAT_ERR_UNSUPPORTED, "at most 65535 query heads");
     if (q && (H < Hkv || H % Hkv)) return fail(MAT_ERR_INVALID, "H = %lld query heads do not divide over H_kv = %lld key heads", (long long)H, (long long)Hkv);
     if (rot < 0 || rot > D || rot % 2) return fail(MAT_ERR_INVALID, "the rotated width must be even and at most D, got %lld", (long long)rot);
     if (rot > 0 && !inv_freq) return fail(MAT_ERR_INVALID, "a rotation needs its frequencies");

@@ -145,7 +145,7 @@ def test_decode_refusals(change, code):
 
 @pytest.mark.parametrize("change", [
     dict(N=-1), dict(N=3), dict(N=1 << 31, cu=16), dict(kn=None), dict(vn=None), dict(start=None), dict(table=None), dict(B=0, N=0),
-    dict(q=16), dict(q=16, qo=16, H=3), dict(rot=3, f=16), dict(rot=66, f=16), dict(rot=2), dict(rot=-2), dict(kts=4), dict(vts=-8),
+    dict(q=16), dict(q=16, qo=16, H=3), dict(q=16, qo=16, H=1 << 17, qts=256), dict(rot=3, f=16), dict(rot=66, f=16), dict(rot=2), dict(rot=-2), dict(kts=4), dict(vts=-8),
     dict(q=16, qo=16, H=4, qts=4), dict(kn=8), dict(q=24, qo=16, H=4, qts=256)])
 def test_append_refusals(change):
     s, base = _struct()
