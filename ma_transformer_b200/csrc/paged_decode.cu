@@ -141,7 +141,9 @@ template <typename T> __device__ __forceinline__ void cluster_join(const DecodeA
 // U times unrolled so that their loads are in flight together.  GT query heads per CTA.
 template <typename T, int LPK, int NV, int GT, int U, bool CLUSTER>
 __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
-    constexpr int W = Vec16<T>::N, KPW = 32 / LPK, C = NV * W;
+    constexpr int W = Vec16<T>::N, KPW = 32 / LPK, C = NV * W, NVAL = U * GT;
+    constexpr int NR = NVAL > LPK ? NVAL / LPK : 1;                  // scores a lane is left with
+    constexpr int ULANE = LPK / U;                                   // lowest lane bit that tells keys apart
     const int64_t b = blockIdx.z, h = blockIdx.x / (unsigned)a.tiles, g0 = (int64_t)(blockIdx.x % (unsigned)a.tiles) * GT;
     const int64_t G = a.G;
     const int D = (int)a.D;
@@ -152,10 +154,14 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     if (!CLUSTER && t0 >= row.n && blockIdx.y > 0) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, part = lane % LPK, key = lane / LPK;
 
-    float q[GT][C], acc[GT][C], m[GT], l[GT];
+    const int group0 = lane - part;
+    const int first_value = part * NVAL / LPK;                       // of the scores this lane is left with
+    auto lane_of = [](int value) { return value * LPK / NVAL; };     // lane of a group that is left with it
+    float q[GT][C], acc[GT][C], m[NR], l[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
-        m[g] = -INFINITY; l[g] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int col = (i * LPK + part) * W;
@@ -170,11 +176,10 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
         for (int j = 0; j < C; ++j) { q[g][j] *= a.scale_log2; acc[g][j] = 0.f; }
     }
 
-    for (int64_t base = t0 + warp * (KPW * U); base < t1; base += 4 * KPW * U) {
-        uint4 kv[U][NV], vv[U][NV];
-        bool ok[U];
-        int64_t at[U];
-        int32_t entry[U];
+    // positions and table entries of the next keys are read while the present ones are worked on
+    int64_t at[U];
+    int32_t entry[U];
+    auto look_up = [&](int64_t base) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t t = base + u * KPW + key;
@@ -182,6 +187,11 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) entry[u] = at[u] >= 0 ? table_entry(a.c, b, at[u] >> a.c.page_shift) : -1;
+    };
+    look_up(t0 + warp * (KPW * U));
+    for (int64_t base = t0 + warp * (KPW * U); base < t1; base += 4 * KPW * U) {
+        uint4 kv[U][NV], vv[U][NV];
+        bool ok[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             ok[u] = entry[u] >= 0 && entry[u] < a.c.n_pages;
@@ -198,8 +208,12 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (at[u] >= 0) entry_inside(a.c, entry[u], a.status);
-        float s[U][GT];
+            if (at[u] >= 0 && !ok[u]) atomicOr(a.status, kPagedOutside);
+        look_up(base + 4 * KPW * U);
+        // Scores of U keys x GT heads, NV values per group of lanes.  Halving the set at every step of the sum over lanes
+        // takes NV - 1 exchanges instead of NV log2(LPK), and leaves each lane with its own NR scores: one exponential
+        // per score instead of one per lane, and the weights go back by a shuffle each.
+        float s[NVAL];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float k[C];
@@ -210,26 +224,49 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
                 float d = 0.f;
 #pragma unroll
                 for (int j = 0; j < C; ++j) d = fmaf(q[g][j], k[j], d);
-#pragma unroll
-                for (int o = LPK / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-                s[u][g] = ok[u] ? d : -INFINITY;
+                s[u * GT + g] = d;
             }
         }
+        int left = NVAL;
 #pragma unroll
-        for (int g = 0; g < GT; ++g) {
-            float top = m[g];
+        for (int o = LPK / 2; o > 0; o >>= 1) {
+            if (left > 1) {
+                left /= 2;
 #pragma unroll
-            for (int u = 0; u < U; ++u) top = fmaxf(top, s[u][g]);
+                for (int i = 0; i < NVAL / 2; ++i)
+                    if (i < left) {
+                        const float send = lane & o ? s[i] : s[i + left], keep = lane & o ? s[i + left] : s[i];
+                        s[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                    }
+            } else {
+                s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+            }
+        }
+        uint32_t seen = 0;                               // keys of this group's U that count
+#pragma unroll
+        for (int u = 0; u < U; ++u) seen |= (ok[u] ? 1u : 0u) << u;
+        bool moved = false;
+        float keep[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            if (!(seen >> ((first_value + i) / GT) & 1)) s[i] = -INFINITY;
+            float top = s[i];
+#pragma unroll
+            for (int o = ULANE; o < LPK; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));   // over the keys
+            top = fmaxf(top, m[i]);
             const float ref = top == -INFINITY ? 0.f : top;   // nothing seen yet: every weight below is 2^-inf = 0
-            const float keep = exp2f(m[g] - ref);
-            m[g] = top;
-            l[g] *= keep;
+            keep[i] = exp2f(m[i] - ref);
+            moved |= top != m[i];
+            m[i] = top;
+            s[i] = exp2f(s[i] - ref);
+            l[i] = l[i] * keep[i] + s[i];
+        }
+        if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-            for (int j = 0; j < C; ++j) acc[g][j] *= keep;
+            for (int g = 0; g < GT; ++g) {
+                const float f = __shfl_sync(0xffffffffu, keep[g % NR], group0 + lane_of(g));
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                s[u][g] = exp2f(s[u][g] - ref);
-                l[g] += s[u][g];
+                for (int j = 0; j < C; ++j) acc[g][j] *= f;
             }
         }
 #pragma unroll
@@ -238,10 +275,23 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) Vec16<T>::unpack(vv[u][i], v + i * W);
 #pragma unroll
-            for (int g = 0; g < GT; ++g)
+            for (int g = 0; g < GT; ++g) {
+                const float w = __shfl_sync(0xffffffffu, s[(u * GT + g) % NR], group0 + lane_of(u * GT + g));
 #pragma unroll
-                for (int j = 0; j < C; ++j) acc[g][j] = fmaf(s[u][g], v[j], acc[g][j]);
+                for (int j = 0; j < C; ++j) acc[g][j] = fmaf(w, v[j], acc[g][j]);
+            }
         }
+    }
+    // every lane: maximum and sum of every head of its group
+    float m_all[GT], l_all[GT];
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int o = ULANE; o < LPK; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+        m_all[g] = __shfl_sync(0xffffffffu, m[g % NR], group0 + lane_of(g));
+        l_all[g] = __shfl_sync(0xffffffffu, l[g % NR], group0 + lane_of(g));
     }
     // join the key lanes of a warp, then the warps
     extern __shared__ __align__(16) float sm[];        // [4][GT][D + 2], then for a cluster [GT][D + 4]
@@ -249,11 +299,11 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
     for (int g = 0; g < GT; ++g) {
 #pragma unroll
         for (int o = LPK; o < 32; o <<= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m[g], o), l2 = __shfl_xor_sync(0xffffffffu, l[g], o);
-            const float top = fmaxf(m[g], m2), ref = top == -INFINITY ? 0.f : top;
-            const float e1 = exp2f(m[g] - ref), e2 = exp2f(m2 - ref);
-            l[g] = l[g] * e1 + l2 * e2;
-            m[g] = top;
+            const float m2 = __shfl_xor_sync(0xffffffffu, m_all[g], o), l2 = __shfl_xor_sync(0xffffffffu, l_all[g], o);
+            const float top = fmaxf(m_all[g], m2), ref = top == -INFINITY ? 0.f : top;
+            const float e1 = exp2f(m_all[g] - ref), e2 = exp2f(m2 - ref);
+            l_all[g] = l_all[g] * e1 + l2 * e2;
+            m_all[g] = top;
 #pragma unroll
             for (int j = 0; j < C; ++j) acc[g][j] = acc[g][j] * e1 + __shfl_xor_sync(0xffffffffu, acc[g][j], o) * e2;
         }
@@ -264,7 +314,7 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
 #pragma unroll
                 for (int j = 0; j < W; ++j)
                     if ((i * LPK + part) * W < D) w[2 + (i * LPK + part) * W + j] = acc[g][i * W + j];
-            if (part == 0) { w[0] = m[g]; w[1] = l[g]; }
+            if (part == 0) { w[0] = m_all[g]; w[1] = l_all[g]; }
         }
     }
     __syncthreads();
@@ -555,13 +605,14 @@ template <typename T> __global__ void __launch_bounds__(128) join_few_kernel(con
     }
 }
 
-// More: one CTA per (sequence, query head), the chunks' weights first, then the sum.  D / 4 lanes of four columns, the other
-// threads take every k-th chunk, and their sums are added in a fixed order.
+// More: CTAs of 32 columns of a (sequence, query head), the chunks' weights first, then the sum; the threads' sums are
+// added in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) join_kernel(const DecodeArgs a) {
+    constexpr int vecs = 8, lanes = 32;             // 32 columns a CTA, every 32nd chunk a thread
     __shared__ float4 acc[256];
     __shared__ float red[8], weight[256];
     const int64_t b = blockIdx.y, head = b * a.H + blockIdx.x, h = blockIdx.x / (unsigned)a.G;
-    const int tid = threadIdx.x, D = (int)a.D, vecs = D / 4, lanes = 256 / vecs, v = tid % vecs, k = tid / vecs;
+    const int tid = threadIdx.x, D = (int)a.D, v = blockIdx.z * vecs + tid % vecs, k = tid / vecs;
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a);
     pdl_wait();
@@ -589,7 +640,7 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
         weight[tid] = w0;
         __syncthreads();
         const int m = min(256, n - i0);
-        if (k < lanes)
+        if (v * 4 < D)
 #pragma unroll 4
             for (int i = k; i < m; i += lanes) {
                 const float4 y = *reinterpret_cast<const float4 *>(part + (int64_t)(i0 + i) * D + v * 4);
@@ -603,12 +654,12 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
     __syncthreads();
     if (tid % 32 == 0) red[tid / 32] = sum;
     __syncthreads();
-    if (k > 0) return;
+    if (k > 0 || v * 4 >= D) return;
     sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += red[i];
     for (int i = 1; i < lanes; ++i) {
-        const float4 y = acc[i * vecs + v];
+        const float4 y = acc[i * vecs + tid];
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
@@ -666,7 +717,7 @@ template <typename T> int run_simt(DecodeArgs &a, cudaStream_t s) {
 
 template <typename T> int run_mma(DecodeArgs &a, cudaStream_t s) {
     a.tiles = (int)((a.H / a.Hkv + 15) / 16);
-    return a.D <= 64 ? launch_mma<T, 64, 5>(a, s) : a.D <= 128 ? launch_mma<T, 128, 3>(a, s) : launch_mma<T, 256, 2>(a, s);
+    return a.D <= 64 ? launch_mma<T, 64, 3>(a, s) : a.D <= 128 ? launch_mma<T, 128, 3>(a, s) : launch_mma<T, 256, 2>(a, s);
 }
 template <> int run_mma<float>(DecodeArgs &a, cudaStream_t s) { return run_simt<float>(a, s); }
 
@@ -674,7 +725,7 @@ template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
     const int rc = a.aligned ? run_mma<T>(a, s) : run_simt<T>(a, s);
     if (rc || a.nsplit == 1 || a.cluster) return rc;
     const cudaError_t e = a.nsplit <= 32 ? launch_after(join_few_kernel<T>, dim3((unsigned)((a.H * a.B + 3) / 4)), dim3(128), 0, s, a)
-                                         : launch_after(join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B), dim3(256), 0, s, a);
+                                         : launch_after(join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B, (unsigned)((a.D + 31) / 32)), dim3(256), 0, s, a);
     return e == cudaSuccess ? MAT_OK : cuda_fail(e, "launching the paged decode's join");
 }
 
@@ -697,7 +748,7 @@ DecodePlan plan(const mat_paged_cache *c, int64_t B, int64_t width, int64_t left
     // Every CTA pays some 4 us to look up its pages, fill its rings and write its result.  64 sequences of up to 8192
     // tokens x 8 key heads of 128: 172 us with chunks of 512 tokens and more, 163 with 1024, 159 with 2048; 32 x 2048
     // chosen tokens x 8: 78, 61, 53 us.  Few rows need the shorter chunks to fill the GPU.
-    p.min_chunk = rows >= kSms ? 2048 : rows >= 16 ? 512 : 128;
+    p.min_chunk = rows >= kSms ? 2048 : rows >= 16 || most > 65536 ? 512 : 128;
     int64_t cap = 16 * kSms / rows;
     if (cap < 8) cap = 8;
     const int64_t n = (most + p.min_chunk - 1) / p.min_chunk;
