@@ -696,6 +696,7 @@ template <typename T, int LPK, int NV> int launch_simt_heads(const DecodeArgs &a
     switch (gt) {
         case 1: return launch_simt<T, LPK, NV, 1>(a, s);
         case 2: return launch_simt<T, LPK, NV, 2>(a, s);
+        case 8: if constexpr (sizeof(T) == 4 && NV == 1) return launch_simt<T, LPK, NV, 8>(a, s);
         default: return launch_simt<T, LPK, NV, 4>(a, s);
     }
 }
@@ -707,9 +708,11 @@ template <typename T, int DP, int NS> int launch_mma(const DecodeArgs &a, cudaSt
 
 template <typename T> int run_simt(DecodeArgs &a, cudaStream_t s) {
     const int64_t G = a.H / a.Hkv;
-    const int gt = G >= 4 ? 4 : (G >= 2 ? 2 : 1);
-    a.tiles = (int)((G + gt - 1) / gt);
     const int vecs = (int)(a.D * sizeof(T) / 16);
+    // eight heads a CTA where the registers allow it: 306 us against 362 for 32 fp32 sequences of up to 8192 tokens with 64
+    // heads on 8 of 128 columns
+    const int gt = G >= 8 && sizeof(T) == 4 && vecs <= 32 ? 8 : G >= 4 ? 4 : (G >= 2 ? 2 : 1);
+    a.tiles = (int)((G + gt - 1) / gt);
     return vecs <= 8 ? launch_simt_heads<T, 8, 1>(a, gt, s)
          : vecs <= 16 ? launch_simt_heads<T, 16, 1>(a, gt, s)
          : vecs <= 32 ? launch_simt_heads<T, 32, 1>(a, gt, s) : launch_simt_heads<T, 32, 2>(a, gt, s);

@@ -196,6 +196,12 @@ DECODE = [
     ([66, 1], 64, 1, 128, 16, torch.bfloat16),
     ([8191, 4097, 1], 32, 8, 128, 64, torch.bfloat16),
     ([20000], 2, 1, 64, 64, torch.float16),
+    ([300, 17, 0, 5000], 16, 2, 64, 16, torch.float32),
+    ([700, 33], 24, 2, 128, 32, torch.float32),
+    ([90], 9, 1, 8, 8, torch.float32),
+    ([400, 1200], 8, 1, 32, 8, torch.bfloat16),
+    ([9000, 100], 4, 4, 128, 64, torch.bfloat16),
+    ([2500] * 40, 8, 8, 64, 64, torch.float16),
 ]
 
 
@@ -238,7 +244,7 @@ def test_decode(case):
 @pytest.mark.gpu
 @pytest.mark.parametrize("spec", [PatternSpec.causal_window(1), PatternSpec.causal_window(64, 2), PatternSpec.causal_window(200),
                                   PatternSpec.sliding_window(7), PatternSpec.causal_window(5000, 3)], ids=str)
-@pytest.mark.parametrize("case", [DECODE[1], DECODE[3], DECODE[7]], ids=str)
+@pytest.mark.parametrize("case", [DECODE[1], DECODE[3], DECODE[7], DECODE[15], DECODE[18]], ids=str)
 def test_decode_of_a_window(case, spec):
     run_decode(case, spec=spec)
 
@@ -247,7 +253,9 @@ def test_decode_of_a_window(case, spec):
 def test_decode_with_other_strides_widths_and_scale():
     run_decode(DECODE[3], heads_first=True, strided=True, scale=0.3)
     run_decode(DECODE[7], heads_first=True)
-    run_decode(DECODE[3], extra_width=20000)          # a table for far longer sequences than there are
+    for case in (DECODE[3], DECODE[15]):              # a table for far longer sequences than there are
+        run_decode(case, extra_width=20000)
+        run_decode(case, extra_width=2000)
     run_decode(([5] * 700, 2, 1, 64, 8, torch.bfloat16))
 
 
