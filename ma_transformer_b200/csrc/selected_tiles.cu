@@ -38,6 +38,7 @@ struct SelTile {                     // what the kernels need beside SelProblem
     float *part;                     // [group rows][slots][D]
     float *kv_part;                  // [group bh][max_items][nsub][2][64][D]
     const float *delta;
+    float *delta_part;               // [group rows][slots][nsub]: shares of delta (few keys a row)
     int64_t bh0;                     // first (batch, key head) of the group
     int G, nsub;
     float scale_log2;
@@ -367,11 +368,15 @@ template <typename T, int LPR, int AHEAD, bool BWD> __global__ void __launch_bou
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // A tile is 64 rows against up to NKP keys of one (sub-)block.  Warp w scores rows 16 w .. 16 w + 15 and writes their
 // share of dq; for dk and dv the weights and dS go through shared memory and warp w owns 16 keys (NKP = 64), or 16 keys
-// and half of the columns (NKP = 32).  Six products of 16 x 64 x 64 per 16 rows (dq counts twice): 240 us at 8192 tokens x
+// and half of the columns (NKP = 32).  Seven products of 16 x 64 x 64 per 16 rows (dq and dk count twice): 250 us at 8192 tokens x
 // 8 heads of 64 x 16 blocks of 64, tensor pipe 41 %, L1 70 % busy (fragments, P and dS, gathered rows), two CTAs a SM by
 // registers.  fp16 gradients want the loss scale that the library's other 16-bit backward kernels want: dS is held in
 // the inputs' type.
-template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, 2) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
+// DELTA: the tile leaves each row's share of delta = sum p dp instead of gradients.  Where a row has few keys its output is
+// as large as a value, and delta taken from the rounded output is off by as much as dS's own rounding: dq and dk of rows
+// of up to 16 keys were 1.8 and 1.7 times as far off as a rounding of the result alone (of 553 rows that see their own
+// block of 128 only, 1.6 times), against 1.1 to 1.4 where rows see two blocks and more.
+template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void __launch_bounds__(128, 2) sel_bwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8, WP = NKP + 8, KW = NKP / 16, CW = 4 / KW, CF = DP / 16 / CW, NBUF = DP == 64 ? 2 : 1;
     const int64_t bhl = blockIdx.z;
     const int bh = (int)t.bh0 + blockIdx.z;
@@ -389,8 +394,8 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
     const int held = (int)max((int64_t)0, min((int64_t)keys, p.S - j0)), n16 = EXACT ? NKP / 16 : (keys + 15) / 16;
     if (held == 0) return;                                                    // the sequence ends before this half
     extern __shared__ __align__(16) char smem[];
-    T *ks = (T *)smem, *vs = ks + NKP * PITCH, *qs = vs + NKP * PITCH, *ps = qs + NBUF * 128 * PITCH, *ds = ps + 64 * WP;
-    int *row_q = (int *)(ds + 64 * WP), *row_at = row_q + kBwdRows;
+    T *ks = (T *)smem, *vs = ks + NKP * PITCH, *qs = vs + NKP * PITCH, *ps = qs + NBUF * 128 * PITCH, *ds = ps + 64 * WP, *dr = ds + 64 * WP;
+    int *row_q = (int *)(dr + 64 * WP), *row_at = row_q + kBwdRows;
     int *row_src = row_at + kBwdRows;
     float *row_lse = (float *)(row_src + kBwdRows), *row_delta = row_lse + kBwdRows;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -409,7 +414,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
             src = i * (int)p.H + g;
             const int64_t row = b * p.S * p.H + h * t.G + src;
             lse = p.lse_in[row] * 1.4426950408889634f;
-            delta = t.delta[row];
+            if (!DELTA) delta = t.delta[row];
         }
         row_q[x] = i; row_at[x] = at; row_src[x] = src; row_lse[x] = lse; row_delta[x] = delta;
     }
@@ -472,6 +477,31 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
                         ptx::Mma<T>::run(dp[2 * c + 1], of, x[2], x[3]);
                     }
             }
+        if constexpr (DELTA) {
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
+                const int col = c * 8 + (lane % 4) * 2;
+                if (col < vis0) sum0 = fmaf(ptx::ex2(fmaf(s[c][0], t.scale_log2, -lse0)), dp[c][0], sum0);
+                if (col + 1 < vis0) sum0 = fmaf(ptx::ex2(fmaf(s[c][1], t.scale_log2, -lse0)), dp[c][1], sum0);
+                if (col < vis1) sum1 = fmaf(ptx::ex2(fmaf(s[c][2], t.scale_log2, -lse1)), dp[c][2], sum1);
+                if (col + 1 < vis1) sum1 = fmaf(ptx::ex2(fmaf(s[c][3], t.scale_log2, -lse1)), dp[c][3], sum1);
+            }
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                sum0 += __shfl_xor_sync(0xffffffffu, sum0, x);
+                sum1 += __shfl_xor_sync(0xffffffffu, sum1, x);
+            }
+            if (lane % 4 == 0) {
+                if (i0 >= 0) t.delta_part[(part0 + row_at[x0]) * t.nsub + sub] = sum0;
+                if (i1 >= 0) t.delta_part[(part0 + row_at[x1]) * t.nsub + sub] = sum1;
+            }
+            if (NBUF == 1) {
+                __syncthreads();
+                if (first + 64 < r_end) stage_rows(qs, first + 64 - item.y);
+            }
+            continue;
+        }
         uint32_t df[NF / 2][4], dl[NF / 2][4];
 #pragma unroll
         for (int c = 0; c < NF; ++c) {
@@ -480,9 +510,10 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
             const float bb = col + 1 < vis0 ? ptx::ex2(fmaf(s[c][1], t.scale_log2, -lse0)) : 0.f;
             const float cc = col < vis1 ? ptx::ex2(fmaf(s[c][2], t.scale_log2, -lse1)) : 0.f;
             const float d = col + 1 < vis1 ? ptx::ex2(fmaf(s[c][3], t.scale_log2, -lse1)) : 0.f;
-            // Weights and dS are rounded to the inputs' type for the products over the rows (dv, dk: one rounding of the
-            // kind the result has).  dq has the rounded output's error in delta beside its own rounding, so dS goes into
-            // it as two halves, rounded value and rest: 1.9e-3 off instead of 2.6e-3 for bf16.
+            // Weights are rounded to the inputs' type for dv, one rounding of the kind the result has.  dq and dk also
+            // have the rounded output's error in delta, so dS goes into them as two halves, rounded value and rest: for
+            // bf16 1.9e-3 off instead of 2.6e-3 (dq), 1.9e-3 instead of 2.4e-3 (dk; 12 us of 350
+            // at 8192 tokens x 8 heads of 64).
             const float ea = col < vis0 ? a * (dp[c][0] - del0) : 0.f, eb = col + 1 < vis0 ? bb * (dp[c][1] - del0) : 0.f;
             const float ec = col < vis1 ? cc * (dp[c][2] - del1) : 0.f, ed = col + 1 < vis1 ? d * (dp[c][3] - del1) : 0.f;
             const uint32_t p0 = ptx::Mma<T>::pack(a, bb), p1 = ptx::Mma<T>::pack(cc, d);
@@ -496,6 +527,8 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
             *reinterpret_cast<uint32_t *>(ps + (row + 8) * WP + col) = p1;
             *reinterpret_cast<uint32_t *>(ds + row * WP + col) = d0;
             *reinterpret_cast<uint32_t *>(ds + (row + 8) * WP + col) = d1;
+            *reinterpret_cast<uint32_t *>(dr + row * WP + col) = dl[c / 2][(c % 2) * 2];
+            *reinterpret_cast<uint32_t *>(dr + (row + 8) * WP + col) = dl[c / 2][(c % 2) * 2 + 1];
         }
         __syncthreads();
         // dq share of this warp's rows, 16 columns at a time
@@ -528,10 +561,11 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
         if (kg < n16)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
-                uint32_t pa[4], da[4];
+                uint32_t pa[4], da[4], ra[4];
                 const int row = kk * 16 + (lane / 16) * 8 + lane % 8, col = kg * 16 + (lane / 8 % 2) * 8;
                 ptx::ldmatrix_x4_trans(pa, ptx::smem_u32(ps + row * WP + col));
                 ptx::ldmatrix_x4_trans(da, ptx::smem_u32(ds + row * WP + col));
+                ptx::ldmatrix_x4_trans(ra, ptx::smem_u32(dr + row * WP + col));
 #pragma unroll
                 for (int c = 0; c < CF; ++c)
                     if (cg * CF + c < d16) {
@@ -543,6 +577,8 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
                         ptx::ldmatrix_x4_trans(x, ptx::smem_u32(qt + (kk * 16 + lane % 16) * PITCH + dc));
                         ptx::Mma<T>::run(dk[c][0], da, x[0], x[1]);
                         ptx::Mma<T>::run(dk[c][1], da, x[2], x[3]);
+                        ptx::Mma<T>::run(dk[c][0], ra, x[0], x[1]);
+                        ptx::Mma<T>::run(dk[c][1], ra, x[2], x[3]);
                     }
             }
         if (NBUF == 1) {
@@ -550,6 +586,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
             if (first + 64 < r_end) stage_rows(qs, first + 64 - item.y);
         }
     }
+    if (DELTA) return;
     float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
     if (kg < n16)
 #pragma unroll
@@ -591,6 +628,27 @@ template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(
         store4((T *)p.dk + at, make_float4(a.x * p.scale, a.y * p.scale, a.z * p.scale, a.w * p.scale));
         store4((T *)p.dv + at, c);
     }
+}
+
+// delta of every row as the sum of its shares, in the order of its list
+__global__ void __launch_bounds__(128) sel_delta_join_kernel(const SelProblem p, const SelTile t, float *delta) {
+    const uint32_t x = blockIdx.x * 128u + threadIdx.x, G = t.G;
+    pdl_trigger();
+    pdl_wait();
+    if (x >= (uint32_t)p.S * G) return;
+    const int i = (int)(x / G), g = (int)(x - i * G), bh = (int)t.bh0 + blockIdx.y, T_ = (int)p.topk;
+    const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
+    const int32_t *list = p.blocks + ((b * p.S + i) * p.Hkv + h) * T_;
+    const int limit = p.causal ? i / (int)p.block + 1 : (int)p.nb;
+    const float *part = t.delta_part + ((int64_t)blockIdx.y * p.S * G + x) * T_ * t.nsub;
+    float sum = 0.f;
+    int prev = -1;
+    for (int s = 0; s < T_; ++s) {
+        if (!sel_entry_counts(list[s], prev, limit)) continue;
+        const int uses = min(t.nsub, (int)((p.S - (int64_t)prev * p.block + 63) / 64));
+        for (int u = 0; u < uses; ++u) sum += part[s * t.nsub + u];
+    }
+    delta[(b * p.S + i) * p.H + h * G + g] = sum;
 }
 
 // delta = dO . O of every row: LPR lanes of 16 bytes
@@ -650,8 +708,11 @@ int launched(const char *what) {
 struct Plan {
     int64_t max_items, group;       // items per (batch, key head); pairs worked off together
     int nsub;
-    size_t lists, items, base, stats, part, kv, delta, total;
+    size_t lists, items, base, stats, part, kv, delta, delta_part, total;
 };
+
+// Rows of so few keys that delta is summed from the tiles (16-bit types); with one block a causal row may see a key or two.
+bool few_keys(int64_t block, int64_t topk) { return topk == 1 || block * topk <= 64; }
 
 int rows_per_item(int dtype, bool bwd) { return dtype == MAT_F32 ? (bwd ? kF32BwdRows : kF32Rows) : bwd ? kBwdRows : kFwdRows; }
 
@@ -673,6 +734,7 @@ Plan plan(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, in
     w.part = take((size_t)w.group * per);
     w.kv = take(bwd ? (size_t)w.group * w.max_items * w.nsub * 2 * 64 * D * 4 : 0);
     w.delta = take(bwd ? (size_t)B * S * H * 4 : 0);
+    w.delta_part = take(bwd && dtype != MAT_F32 && few_keys(block, topk) ? (size_t)w.group * S * G * topk * w.nsub * 4 : 0);
     w.total = at;
     return w;
 }
@@ -687,6 +749,7 @@ int prepare(const SelProblem &p, const Plan &w, void *ws, bool bwd, SelTile &t) 
     t.part = (float *)(at + w.part);
     t.kv_part = (float *)(at + w.kv);
     t.delta = (const float *)(at + w.delta);
+    t.delta_part = (float *)(at + w.delta_part);
     t.G = (int)(p.H / p.Hkv);
     t.nsub = w.nsub;
     t.scale_log2 = p.scale * 1.4426950408889634f;
@@ -714,11 +777,20 @@ template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, 
 }
 
 template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, const Plan &w, SelTile &t) {
-    const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 2 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20;
-    if (int rc = ensure_dynamic_smem((const void *)sel_bwd_mma_kernel<T, DP, NKP, EXACT>, smem, "shared memory of the selected attention's backward")) return rc;
-    launch_delta<T>(p, const_cast<float *>(t.delta));
+    const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 3 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20;
+    const auto grads = sel_bwd_mma_kernel<T, DP, NKP, EXACT, false>, shares = sel_bwd_mma_kernel<T, DP, NKP, EXACT, true>;
+    const bool few = few_keys(p.block, p.topk);
+    if (int rc = ensure_dynamic_smem((const void *)grads, smem, "shared memory of the selected attention's backward")) return rc;
+    if (int rc = few ? ensure_dynamic_smem((const void *)shares, smem, "shared memory of the selected attention's backward") : MAT_OK) return rc;
+    float *delta = const_cast<float *>(t.delta);
+    if (!few) launch_delta<T>(p, delta);
     return over_groups<true, T>(p, w, t, [&](unsigned n) {
-        launch_after(sel_bwd_mma_kernel<T, DP, NKP, EXACT>, dim3((unsigned)w.max_items, (unsigned)w.nsub, n), dim3(128), smem, p.stream, p, t);
+        const dim3 grid((unsigned)w.max_items, (unsigned)w.nsub, n);
+        if (few) {
+            launch_after(shares, grid, dim3(128), smem, p.stream, p, t);
+            launch_after(sel_delta_join_kernel, dim3((unsigned)((p.S * t.G + 127) / 128), n), dim3(128), 0, p.stream, p, t, delta);
+        }
+        launch_after(grads, grid, dim3(128), smem, p.stream, p, t);
     });
 }
 

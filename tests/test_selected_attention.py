@@ -125,6 +125,10 @@ CASES = [
     (3, 64, 2, 2, 96, 64, 1, True, torch.float16),
     (1, 2100, 1, 1, 64, 64, 6, True, torch.bfloat16),
     (1, 700, 16, 1, 72, 64, 3, True, torch.bfloat16),
+    (2, 500, 4, 2, 64, 16, 1, True, torch.bfloat16),
+    (1, 553, 2, 1, 128, 128, 1, True, torch.bfloat16),
+    (1, 400, 6, 2, 40, 32, 2, False, torch.float16),
+    (1, 300, 2, 1, 128, 96, 1, False, torch.float16),
 ]
 
 
