@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
 // more), so its 16 rows share one table lookup, a warp looks up 32 tiles at a time, and rows are stepped through: forming
 // every copy's address took more issue slots than the mathematics (150 us instead of 140).
 // 64 sequences of up to 8192 tokens, 32 heads on 8 of 128 columns, 861 MB: 140 us = 6.15 TB/s, 95 % of the measured copy
-// rate; a call of 155 us with its join over states that L2 does not hold (5.5 TB/s).  4 of up to 131072: 5.8 TB/s.
+// rate; a call of 149 us with its join over states that L2 does not hold (5.8 TB/s).  4 of up to 131072: 6.06 TB/s.
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
