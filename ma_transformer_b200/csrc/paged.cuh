@@ -38,8 +38,8 @@ __device__ __forceinline__ int64_t physical_page(const PagedView &c, int64_t b, 
     return p;
 }
 
-// The table's entry alone, for several pages at once: with the report in between, the reads wait for each other (four of
-// them 2.6 us instead of one's 0.7).
+// The table's entry alone, for several pages at once: with the report in between, the reads wait for each other (a step
+// of four pages took the page scores 2.6 us, 1.8 without).
 __device__ __forceinline__ int32_t table_entry(const PagedView &c, int64_t b, int64_t logical) {
     return logical >= 0 && logical < c.width ? __ldg(c.table + b * c.table_stride + logical) : -1;
 }
