@@ -283,7 +283,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
 // list together (which count, and with what weight) while the first AHEAD partials are on their way.
 // BWD: the sum of a row's shares of dq.
 template <typename T, int LPR, int AHEAD, bool BWD> __global__ void __launch_bounds__(128) sel_join_kernel(const SelProblem p, const SelTile t) {
-    const uint32_t x0 = (blockIdx.x * 128u + threadIdx.x) / LPR, G = t.G;                       // (i, g) of the pair
+    const uint32_t x0 = blockIdx.x * (128u / LPR) + threadIdx.x / LPR, G = t.G;                 // (i, g) of the pair; S G < 2^31
     const int lane = threadIdx.x % LPR, col = lane * 4, D = (int)p.D, T_ = (int)p.topk;
     pdl_trigger();
     pdl_wait();
