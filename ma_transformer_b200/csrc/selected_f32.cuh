@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
     float *ks = (float *)smem, *vs = ks + 64 * pitch, *qs = vs + 64 * pitch, *os = qs + 64 * pitch, *ps = os + 64 * pitch, *ds = ps + 64 * kWPitch;
     __shared__ int row_q[64], row_at[64];
     __shared__ float row_lse[64], row_delta[64];
+    __shared__ OddColumns<128> odd;
     stage_f32(ks, (const float *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, p.Hkv * D, held, 64, D);
     stage_f32(vs, (const float *)p.v + ((b * p.S + j0) * p.Hkv + h) * D, p.Hkv * D, held, 64, D);
     cp_async_commit();
@@ -232,6 +233,8 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
     for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) dk[u][i] = dv[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int ragged_end = p.causal ? (int)(j0 + held) - 1 : 0;        // queries below it see part of the keys
+    bool odd_rows = false;                               // `odd` is in use
     for (int first = item.y; first < r_end; first += 64) {
         __syncthreads();
         if (tid < 64) {
@@ -261,6 +264,15 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
         float s[4][4] = {}, dp[4][4] = {};
         tile_dot(s, qs, ks, D, pitch);
         tile_dot(dp, os, vs, D, pitch);
+        const bool ragged = row_q[0] < ragged_end;       // a tile's first row has its lowest query
+        float zero = 0.f;                                // NaN: a score or dP of a ragged tile is not finite
+        if (ragged)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) zero = fmaf(s[i][j], 0.f, zero);
+                zero = fmaf(dp[i][0], 0.f, zero);        // an output gradient shows in every column
+            }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = ty + 16 * i, q = row_q[r];
@@ -273,7 +285,26 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
                 ds[r * kWPitch + tx + 16 * j] = in ? w * (dp[i][j] - row_delta[r]) : 0.f;
             }
         }
-        __syncthreads();
+        bool odd_tile = false;
+        if (ragged) odd_tile = __syncthreads_or(zero != 0.f);
+        else __syncthreads();
+        if (odd_tile) {
+            if (!odd_rows) odd.clear(kF32Threads);
+            odd_rows = true;
+            __syncthreads();
+            for (int x = tid; x < (128 + held) * D; x += kF32Threads) {
+                const int r = x / D, c = x - r * D, i = r < 128 ? row_q[r % 64] : 0;
+                float *at = (r < 64 ? qs + r * pitch : r < 128 ? os + (r - 64) * pitch : ks + (r - 128) * pitch) + c;
+                const float f = *at;
+                if (i < 0 || fabsf(f) < INFINITY) continue;
+                const int vis = max(0, (int)min((int64_t)held, i + 1 - j0));
+                *at = 0.f;
+                if (r >= 128) odd.see_key(r - 128, c);
+                else if (r < 64) odd.see_query(vis, c);
+                else odd.see_grad(f, vis, c);
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int x = tid + u * kF32Threads, rg = x / vecs, col = (x - rg * vecs) * 4;
@@ -282,6 +313,13 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             tile_times(y, ds, ks, keys, rg, col, pitch);
+            if (odd_tile)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int vis = max(0, (int)min((int64_t)held, row_q[4 * rg + i] + 1 - j0));
+                    y[i].x = odd.dq(y[i].x, vis, col); y[i].y = odd.dq(y[i].y, vis, col + 1);
+                    y[i].z = odd.dq(y[i].z, vis, col + 2); y[i].w = odd.dq(y[i].w, vis, col + 3);
+                }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (row_q[4 * rg + i] >= 0) *reinterpret_cast<float4 *>(t.part + ((part0 + row_at[4 * rg + i]) * t.nsub + sub) * D + col) = y[i];
@@ -293,7 +331,13 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
                 fma4(dk[u][0], e.x, q); fma4(dk[u][1], e.y, q); fma4(dk[u][2], e.z, q); fma4(dk[u][3], e.w, q);
             }
         }
+        if (odd_tile) {                                  // the keys as they are
+            __syncthreads();
+            stage_f32(ks, (const float *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, p.Hkv * D, held, 64, D);
+            cp_async_commit();
+        }
     }
+    cp_async_wait<0>();
     float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -301,6 +345,12 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
         if (rg >= 16) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            if (odd_rows) {
+                const int r = 4 * rg + i;
+                float4 &x = dk[u][i], &y = dv[u][i];
+                x.x = odd.dk(x.x, r, col); x.y = odd.dk(x.y, r, col + 1); x.z = odd.dk(x.z, r, col + 2); x.w = odd.dk(x.w, r, col + 3);
+                y.x = odd.dv(y.x, r, col); y.y = odd.dv(y.y, r, col + 1); y.z = odd.dv(y.z, r, col + 2); y.w = odd.dv(y.w, r, col + 3);
+            }
             *reinterpret_cast<float4 *>(out + (4 * rg + i) * D + col) = dk[u][i];
             *reinterpret_cast<float4 *>(out + (64 + 4 * rg + i) * D + col) = dv[u][i];
         }

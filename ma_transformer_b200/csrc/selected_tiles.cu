@@ -65,6 +65,32 @@ __device__ __forceinline__ void stage_keys(T *dst, const T *src, int64_t row_str
     }
 }
 
+// Zero does not silence an infinity or a NaN, so the zero weights of pairs that do not see each other need finite factors.
+// Only tiles whose rows see part of the keys (the queries of a causal block itself) have such pairs, and there a value of
+// that kind shows in the tile's scores or dP.  Such a tile forms its gradients from zeros in those values' place, and this
+// says what the pairs that see them get: rows see the first `vis` keys, so it is enough to know, column by column, the first
+// such key, and how many keys the rows with such a value see.  Looking for them takes 9 of 252 us of the backward tiles at
+// 8192 tokens x 8 heads of 64 x 16 blocks of 64 (2 of 460 at 4096 x 2 x 16 heads of 128).
+template <int DP> struct OddColumns {
+    int key[DP];                         // first key with such a value; 64: none
+    int q[DP];                           // keys that see such a query: NaN in dk (the row's weights are NaN)
+    int nan[DP], up[DP], down[DP];       // keys that see such an output gradient: a NaN, an infinity of either sign, in dv
+    __device__ __forceinline__ void clear(int threads) {
+        for (int x = threadIdx.x; x < DP; x += threads) {
+            key[x] = 64;
+            q[x] = nan[x] = up[x] = down[x] = 0;
+        }
+    }
+    __device__ __forceinline__ void see_key(int row, int col) { atomicMin(&key[col], row); }
+    __device__ __forceinline__ void see_query(int vis, int col) { atomicMax(&q[col], vis); }
+    __device__ __forceinline__ void see_grad(float x, int vis, int col) { atomicMax(x != x ? &nan[col] : x > 0.f ? &up[col] : &down[col], vis); }
+    __device__ __forceinline__ float dq(float x, int vis, int col) const { return vis > key[col] ? NAN : x; }
+    __device__ __forceinline__ float dk(float x, int row, int col) const { return row < q[col] ? NAN : x; }
+    __device__ __forceinline__ float dv(float x, int row, int col) const {
+        return x + (row < nan[col] ? NAN : 0.f) + (row < up[col] ? INFINITY : 0.f) - (row < down[col] ? INFINITY : 0.f);
+    }
+};
+
 }  // namespace
 }  // namespace mat
 #include "selected_f32.cuh"
@@ -360,7 +386,13 @@ template <typename T, int LPR, int AHEAD, bool BWD> __global__ void __launch_bou
         }
     }
     if (!in) return;
-    const float f = BWD ? p.scale : l == 0.f ? 0.f : 1.f / l;
+    float f = BWD ? p.scale : 1.f / l;
+    if (!BWD && l == 0.f) {                            // no keys: zeros; keys that all score -inf: NaN, the softmax of such a row
+        f = 0.f;
+        prev = -1;
+        for (int s = 0; s < T_; ++s)
+            if (sel_entry_counts(list[s], prev, limit)) f = NAN;
+    }
     if (!BWD && lane == 0) p.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     store4((T *)(BWD ? p.dq : p.out) + out * D + col, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }
@@ -398,6 +430,7 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
     int *row_q = (int *)(dr + 64 * WP), *row_at = row_q + kBwdRows;
     int *row_src = row_at + kBwdRows;
     float *row_lse = (float *)(row_src + kBwdRows), *row_delta = row_lse + kBwdRows;
+    OddColumns<DP> &odd = *(OddColumns<DP> *)(row_delta + kBwdRows);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t krow = p.Hkv * D;
     stage_keys<T, DP>(ks, (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D);
@@ -442,7 +475,8 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
 #pragma unroll
             for (int y = 0; y < 4; ++y) dk[c][x][y] = dv[c][x][y] = 0.f;
     const int kg = warp % KW, cg = warp / KW;          // this warp's keys and column half in the key pass
-
+    const int ragged_end = p.causal ? (int)(j0 + held) - 1 : 0;        // queries below it see part of the keys
+    bool odd_rows = false;                             // `odd` is in use
     int cur = 0;
     for (int first = item.y; first < r_end; first += 64, cur ^= NBUF - 1) {
         const T *qt = qs + cur * 128 * PITCH, *ot = qt + 64 * PITCH;
@@ -502,6 +536,15 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
             }
             continue;
         }
+        const bool ragged = row_q[first - item.y] < ragged_end;        // a tile's first row has its lowest query
+        float zero = 0.f;                              // NaN: a score or dP of a ragged tile is not finite
+        if (ragged) {
+#pragma unroll
+            for (int c = 0; c < NF; ++c)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) zero = fmaf(s[c][y], 0.f, zero);
+            zero = fmaf(dp[0][0], 0.f, fmaf(dp[0][2], 0.f, zero));      // an output gradient shows in every column
+        }
         uint32_t df[NF / 2][4], dl[NF / 2][4];
 #pragma unroll
         for (int c = 0; c < NF; ++c) {
@@ -530,7 +573,30 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
             *reinterpret_cast<uint32_t *>(dr + row * WP + col) = dl[c / 2][(c % 2) * 2];
             *reinterpret_cast<uint32_t *>(dr + (row + 8) * WP + col) = dl[c / 2][(c % 2) * 2 + 1];
         }
-        __syncthreads();
+        bool odd_tile = false;
+        if (ragged) odd_tile = __syncthreads_or(zero != 0.f);
+        else __syncthreads();
+        if (odd_tile) {
+            if (!odd_rows) odd.clear(128);
+            odd_rows = true;
+            __syncthreads();
+            T *rows = qs + cur * 128 * PITCH;          // 64 queries, then their output gradients
+            for (int x = threadIdx.x; x < (128 + held) * (DP / 8); x += 128) {
+                const int r = x / (DP / 8), c = x % (DP / 8) * 8, i = r < 128 ? row_q[first - item.y + r % 64] : 0;
+                T *at = (r < 128 ? rows + r * PITCH : ks + (r - 128) * PITCH) + c;
+                if (i < 0) continue;
+                const int vis = max(0, (int)min((int64_t)held, i + 1 - j0));
+                for (int y = 0; y < 8; ++y) {
+                    const float f = Elem<T>::to_f(at[y]);
+                    if (f - f == 0.f) continue;
+                    at[y] = Elem<T>::from_f(0.f);
+                    if (r >= 128) odd.see_key(r - 128, c + y);
+                    else if (r < 64) odd.see_query(vis, c + y);
+                    else odd.see_grad(f, vis, c + y);
+                }
+            }
+            __syncthreads();
+        }
         // dq share of this warp's rows, 16 columns at a time
         const int64_t at0 = (part0 + row_at[x0]) * t.nsub + sub, at1 = (part0 + row_at[x1]) * t.nsub + sub;
 #pragma unroll
@@ -581,12 +647,24 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
                         ptx::Mma<T>::run(dk[c][1], ra, x[2], x[3]);
                     }
             }
+        if (odd_tile) {
+            __syncthreads();                 // also puts the shares above before what follows
+            for (int x = threadIdx.x; x < 64 * D; x += 128) {
+                const int r = first - item.y + x / D, col = x % D, i = row_q[r];
+                if (i < 0 || min((int64_t)held, i + 1 - j0) <= odd.key[col]) continue;
+                t.part[((part0 + row_at[r]) * t.nsub + sub) * D + col] = NAN;       // zero times such a key
+            }
+            // the keys as they are
+            stage_keys<T, DP>(ks, (const T *)p.k + ((b * p.S + j0) * p.Hkv + h) * D, krow, held, NKP, D);
+            cp_async_commit();
+        }
         if (NBUF == 1) {
             __syncthreads();             // every warp is done with the tile
             if (first + 64 < r_end) stage_rows(qs, first + 64 - item.y);
         }
     }
     if (DELTA) return;
+    cp_async_wait<0>();
     float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
     if (kg < n16)
 #pragma unroll
@@ -601,6 +679,14 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
                     *reinterpret_cast<float2 *>(out + (64 + row + 8) * D + col) = make_float2(dv[c][x][2], dv[c][x][3]);
                 }
             }
+    if (odd_rows) {
+        __syncthreads();
+        for (int x = threadIdx.x; x < keys * D; x += 128) {
+            const int row = x / D, col = x - row * D;
+            out[x] = odd.dk(out[x], row, col);
+            out[64 * D + x] = odd.dv(out[64 * D + x], row, col);
+        }
+    }
 }
 
 // dk and dv of a (sub-)block: the sum of its items' shares in order; zeros for a block that nobody chose
@@ -777,7 +863,7 @@ template <typename T, int DP, int NKP, bool EXACT> int fwd(const SelProblem &p, 
 }
 
 template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, const Plan &w, SelTile &t) {
-    const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 3 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20;
+    const size_t smem = ((2 * NKP + (DP == 64 ? 4 : 2) * 64) * (DP + 8) + 3 * 64 * (NKP + 8)) * sizeof(T) + kBwdRows * 20 + sizeof(OddColumns<DP>);
     const auto grads = sel_bwd_mma_kernel<T, DP, NKP, EXACT, false>, shares = sel_bwd_mma_kernel<T, DP, NKP, EXACT, true>;
     const bool few = few_keys(p.block, p.topk);
     if (int rc = ensure_dynamic_smem((const void *)grads, smem, "shared memory of the selected attention's backward")) return rc;
