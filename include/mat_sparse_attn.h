@@ -342,7 +342,8 @@ int mat_pattern_nnz(const mat_pattern_spec *spec, int64_t S_q, int64_t S_kv, int
  * k_head_stride + column, in ELEMENTS, so both [pages, slots, heads, D] and [pages, heads, slots, D] storage are
  * served; the same for v.  Bases and strides are multiples of 16 bytes, D is a multiple of 8 up to 256.
  * key_bounds holds, for every page and head, the smallest and the largest key column by column over the page's filled
- * slots, packed [n_pages, 2, H_kv, D] in the cache's type; NULL when pages are never selected by score.
+ * slots (NaN where one of them is), packed [n_pages, 2, H_kv, D] in the cache's type; NULL when pages are never
+ * selected by score.
  *
  * A page table [B, table_width] (rows table_stride apart) of int32 names the physical page of every logical page of a
  * sequence.  Entries of pages that a call does not touch may hold anything.  A touched entry outside [0, n_pages) is
@@ -413,6 +414,7 @@ size_t mat_paged_select_workspace_bytes(const mat_paged_cache *cache, int64_t B,
  * Block selection over whole sequences, the form for prompts and training: the same score with blocks of `block` keys
  * (a multiple of 16, up to 128; the last block may be short) of k: [B, S, H_kv, D] in the place of pages and every row
  * of q: [B, S, H, D] in the place of the new token.  causal: blocks behind the query's own are not eligible.
+ * A block with a NaN key has a score that is not a number: it ranks last.
  * blocks: [B, S, H_kv, topk] int32, ascending, -1 behind the last; the query's own block is always among them.
  */
 int mat_select_blocks(const void *q, const void *k, int64_t B, int64_t S, int64_t H, int64_t H_kv, int64_t D, int dtype,

@@ -44,7 +44,7 @@ __device__ __forceinline__ float of_key32(uint32_t k) {
 
 // ---- bounds of the blocks of whole sequences ------------------------------------------------------------------------
 // One CTA per block and 64 bytes x 8 of its columns: 32 vectors of columns, 8 threads each taking every 8th token, four
-// tokens in flight.
+// tokens in flight.  A NaN key makes its column's bounds NaN.
 template <typename T>
 __global__ void __launch_bounds__(256) block_bounds_kernel(const T *k, T *bounds, int64_t S, int64_t nb, int block, int64_t HD) {
     pdl_trigger();
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(const T *k, T *bounds
             float x[W];
             Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(k + (b * S + s) * HD + c)), x);
 #pragma unroll
-            for (int j = 0; j < W; ++j) { lo[j] = fminf(lo[j], x[j]); hi[j] = fmaxf(hi[j], x[j]); }
+            for (int j = 0; j < W; ++j) { lo[j] = ptx::min_nan(lo[j], x[j]); hi[j] = ptx::max_nan(hi[j], x[j]); }
         }
 #pragma unroll
     for (int j = 0; j < W; ++j) {
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(const T *k, T *bounds
             m[j] = red[part][0][j * 32 + threadIdx.x % 32];
             for (int x = 1; x < 8; ++x) {
                 const float y = red[part][x][j * 32 + threadIdx.x % 32];
-                m[j] = part ? fmaxf(m[j], y) : fminf(m[j], y);
+                m[j] = part ? ptx::max_nan(m[j], y) : ptx::min_nan(m[j], y);
             }
         }
         *reinterpret_cast<uint4 *>(bounds + ((b * nb + n) * 2 + part) * HD + c) = Vec16<T>::pack(m);
@@ -416,8 +416,10 @@ __global__ void __launch_bounds__(128, PER <= 4 ? 8 : 1) select_rows_kernel(cons
         if (i < n) {
             const float x = row[i], y = block_norms[(b * of.Hkv + h) * of.nb + i];
             key[j] = i == own ? 0xffffffffu : key32_of(x);
-            size = fmaxf(size, y);
-            odd |= !(fabsf(x) < INFINITY && y < INFINITY);
+            if (i != own) {                        // its score decides nothing
+                size = fmaxf(size, y);
+                odd |= !(fabsf(x) < INFINITY && y < INFINITY);
+            }
         }
     }
     int32_t *o = out + ((b * of.S + s) * of.Hkv + h) * topk;

@@ -279,7 +279,8 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) append
     }
 }
 
-// Bounds of one page and head from its first `filled` slots, by one warp: LV lanes of 16 bytes share a token.
+// Bounds of one page and head from its first `filled` slots, by one warp: LV lanes of 16 bytes share a token.  A NaN key
+// makes its column's bounds NaN, so that the page's score says so.
 template <typename T> __device__ void page_bounds(const AppendArgs &a, int64_t phys, int h, int filled) {
     constexpr int W = Vec16<T>::N;
     const int lane = threadIdx.x % 32, D = (int)a.D, vecs = D / W;
@@ -297,13 +298,13 @@ template <typename T> __device__ void page_bounds(const AppendArgs &a, int64_t p
                 float x[W];
                 Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(rows + s * a.c.k_tok + col), x);
 #pragma unroll
-                for (int j = 0; j < W; ++j) { lo[j] = fminf(lo[j], x[j]); hi[j] = fmaxf(hi[j], x[j]); }
+                for (int j = 0; j < W; ++j) { lo[j] = ptx::min_nan(lo[j], x[j]); hi[j] = ptx::max_nan(hi[j], x[j]); }
             }
         for (int o = lv; o < 32; o <<= 1)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
-                hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
+                lo[j] = ptx::min_nan(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
+                hi[j] = ptx::max_nan(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
             }
         if (lane < lv && col < D) {
             *reinterpret_cast<uint4 *>(out + col) = Vec16<T>::pack(lo);

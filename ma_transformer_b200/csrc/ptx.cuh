@@ -126,6 +126,18 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                  : "r"(addr));
 }
 
+// smaller and larger of two numbers, NaN if either is (fminf and fmaxf give the other one)
+__device__ __forceinline__ float min_nan(float x, float y) {
+    float z;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -246,7 +246,7 @@ def select_pages(query: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     """The ``topk`` logical pages each new token reads, [B, n_kv_heads, topk] int32, ascending, -1 behind the last: the
     page of the token itself and the best others by an upper bound of the group's q . k that the cache's ``key_bounds``
     give (sum over query heads and columns of max(q * lo, q * hi)).  Scores are compared in 64 bits, equal ones go to
-    the lower page."""
+    the lower page, one that is not a number (a NaN key) ranks last."""
     H = _heads(query, cache)
     B, width, t_stride = _table(page_table, cache)
     q_stride = _rows(query, "query", cache, B, H)

@@ -46,7 +46,7 @@ def select_blocks(query: torch.Tensor, key: torch.Tensor, block: int, topk: int,
     A query's own block is always among them; the others are the best by an upper bound of the group's q . k over the
     block's keys (sum over query heads and columns of max(q * lo, q * hi), lo and hi the block's smallest and largest
     key).  ``causal``: blocks behind the query's own are not eligible.  Scores are compared in 64 bits, equal ones go to
-    the lower block.  ``block``: a multiple of 16 up to 128; head widths: multiples of 8 up to 128.
+    the lower block, one that is not a number (a NaN key) ranks last.  ``block``: a multiple of 16 up to 128; head widths: multiples of 8 up to 128.
     """
     B, S, H, Hkv, D, dt = _shapes(query, key, None)
     topk, block = int(topk), int(block)

@@ -1,0 +1,52 @@
+"""Page selection beside the forms that the paged attention's own tests reach: batches that fill the GPU, keys that are not
+numbers."""
+import math
+
+import pytest
+import torch
+
+import ma_transformer_b200 as mt
+from ma_transformer_b200 import _native as nat
+from ma_transformer_b200 import paged_attention as paged
+
+
+def choose(score, own, topk):
+    """The own page and the best others, not-a-number scores last, equal ones by the lower index."""
+    rank = sorted(range(len(score)), key=lambda n: (n != own, math.isnan(score[n]), -score[n] if score[n] == score[n] else 0, n))[:topk]
+    return sorted(rank) + [-1] * (topk - len(rank))
+
+
+def scores(q, kb, pages, h, G):
+    """By the definition, sum over heads and columns of max(q lo, q hi), in 64 bits."""
+    lo, hi = kb[pages, 0, h].double(), kb[pages, 1, h].double()
+    return sum(torch.maximum(r * lo, r * hi) for r in q[h * G:(h + 1) * G].double()).sum(-1).tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, D", [(torch.bfloat16, 64), (torch.float16, 72), (torch.float32, 64), (torch.float32, 256)])
+def test_keys_that_are_not_numbers_make_their_page_the_last_choice(dtype, D):
+    """Appended one by one and as a prompt: a page's bounds are NaN in the columns where a key is."""
+    N, H, Hkv, page, topk = 400, 4, 2, 16, 5
+    g = torch.Generator().manual_seed(31)
+    q, k, v = (torch.randn(N, h, D, generator=g).to(dtype) for h in (H, Hkv, Hkv))
+    k[3, 0, 5], k[47, 1, D - 1], k[111, :, 0], k[200:232] = float("nan"), -float("nan"), float("nan"), float("nan")
+    k[[3, 47, 111]] *= 4
+    table = torch.randperm(25, generator=g).to(torch.int32)
+    at = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")  # noqa: E731
+    caches = [mt.PagedKVCache(25, page, Hkv, D, dtype, key_bounds=True) for _ in range(2)]
+    kd, vd, td = k.cuda(), v.cuda(), table.cuda()[None]
+    paged.append(caches[0], kd, vd, td, at(0), cu_seqlens=torch.tensor([0, N], dtype=torch.int32, device="cuda"))
+    for i in range(N):
+        paged.append(caches[1], kd[i:i + 1], vd[i:i + 1], td, at(i))
+    held = k.view(25, page, Hkv, D)
+    want = torch.full((25, 2, Hkv, D), 7.0, dtype=dtype)
+    want[table.long(), 0], want[table.long(), 1] = held.float().amin(1).to(dtype), held.float().amax(1).to(dtype)
+    for cache in caches:
+        assert torch.equal(cache.key_bounds.cpu().isnan(), want.isnan()) and torch.equal(cache.key_bounds.cpu().nan_to_num(9), want.nan_to_num(9))
+        for n in (130, 215, 400):
+            for topk in (5, 23):
+                pages = paged.select_pages(q[n - 1:n].cuda(), cache, td, at(n), topk).cpu()
+                used = table[:-(-n // page)].long()
+                for h in range(Hkv):
+                    assert pages[0, h].tolist() == choose(scores(q[n - 1], want, used, h, H // Hkv), len(used) - 1, topk), (n, h, topk)
+    assert nat.device_status() == 0

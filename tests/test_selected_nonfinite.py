@@ -81,3 +81,43 @@ def test_pairs_that_do_not_see_each_other_change_nothing(S, H, Hkv, D, block, to
         assert torch.equal(torch.isfinite(g), finite), f"{name}: {int((torch.isfinite(g) != finite).sum())} values"
         err = (g - w).abs().masked_fill(~finite, 0)
         assert (err <= t.masked_fill(~finite, 1)).all(), f"{name}: off by {float(err.max())}"
+
+
+def choose(score, own, last, topk):
+    """The own block and the best others of the first `last`, not-a-number scores last, equal ones by the lower index."""
+    rank = sorted(range(last), key=lambda n: (n != own, math.isnan(score[n]), -score[n] if score[n] == score[n] else 0, n))[:topk]
+    return sorted(rank) + [-1] * (topk - len(rank))
+
+
+def block_scores(q, k, block, row):
+    """Scores [Hkv, blocks] of one row by the definition, sum over heads and columns of max(q lo, q hi), in 64 bits."""
+    S, Hkv = k.shape[1:3]
+    parts = [k[0, n:n + block].double() for n in range(0, S, block)]
+    lo, hi = torch.stack([x.amin(0) for x in parts], 1), torch.stack([x.amax(0) for x in parts], 1)        # [Hkv, blocks, D]
+    heads = q[0, row].double().view(Hkv, -1, 1, q.shape[-1])
+    return torch.maximum(heads * lo[:, None], heads * hi[:, None]).sum((1, 3))
+
+
+def check_choice(q, k, block, topk, causal, rows):
+    got = sel.select_blocks(q.cuda(), k.cuda(), block, topk, causal).cpu()
+    nb = -(-k.shape[1] // block)
+    for s in rows:
+        score, own = block_scores(q, k, block, s).tolist(), s // block
+        for h in range(k.shape[2]):
+            assert got[0, s, h].tolist() == choose(score[h], own, own + 1 if causal else nb, topk), (s, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("S, D, dtype", [(500, 64, torch.bfloat16), (500, 80, torch.float16), (500, 64, torch.float32), (16500, 8, torch.bfloat16)])
+def test_blocks_with_a_key_that_is_not_a_number_are_chosen_last(S, D, dtype, causal):
+    """One NaN in a block of keys makes its score NaN, whichever token, head or column holds it; the own block stays in."""
+    q, k, _, _ = inputs(1, S, 4, 2, D, dtype, seed=22)
+    k[0, 3, 0, 5], k[0, 47, 1, D - 1], k[0, 111, :, 0], k[0, S - 1, 0, 1] = float("nan"), -float("nan"), float("nan"), float("nan")
+    k[0, 200:232] = float("nan")
+    k[0, [3, 47, 111]] *= 4                               # without the NaN these blocks would be high
+    rows = list(range(0, 240, 3)) + [S - 17, S - 2, S - 1]
+    for topk in (4, 15):
+        check_choice(q, k, 16, topk, causal, rows)
+    if S < 1000:
+        check_choice(q, k, 16, 40, causal, rows)          # more places than blocks that are numbers
