@@ -452,8 +452,9 @@ __global__ void __launch_bounds__(128, PER <= 4 ? 8 : 1) select_rows_kernel(cons
             for (int x = 16; x > 0; x >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, x));
             odd = __any_sync(0xffffffffu, odd);
             // A product step adds 16 products to the accumulator; aligned to the largest and cut at 24 bits, each of the
-            // 17 terms may lose 2^-23 of the largest: 2.1e-6 of the terms' size per step.
-            const float eps = (float)(2 * G * ((D + 15) / 16) + 1) * 2.1e-6f * q_norm * size + 1e-42f;
+            // 17 terms may lose 2^-23 of the largest: 2.1e-6 of the terms' size per step.  Squares and terms below the least
+            // normal number, 1.2e-38, may be lost altogether: up to 2e-18 of a norm of 128 columns, 2.1e-37 of a step.
+            const float eps = (float)(2 * G * ((D + 15) / 16) + 1) * (2.1e-6f * (q_norm + (float)G * 2e-18f) * (size + 2e-18f) + 2.1e-37f);
             // the least that is taken and the most that is not
             uint32_t in = 0xffffffffu, not_in = 0;
 #pragma unroll
