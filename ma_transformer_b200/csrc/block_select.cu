@@ -42,6 +42,19 @@ __device__ __forceinline__ float of_key32(uint32_t k) {
     return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
+// The product form above is the definition's sum where all is finite.  Infinite bounds need its terms as they stand: a head
+// that takes a bound with weight zero would make 0 x inf of it.
+template <typename T> __device__ double score_by_terms(const T *q, const T *low, const T *high, int64_t G, int D) {
+    double s = 0;
+    for (int64_t g = 0; g < G; ++g)
+        for (int d = 0; d < D; ++d) {
+            const double w = (double)Elem<T>::to_f(q[g * D + d]), x = w * (double)Elem<T>::to_f(low[d]), y = w * (double)Elem<T>::to_f(high[d]);
+            if (x != x || y != y) return NAN;
+            s += x > y ? x : y;
+        }
+    return s;
+}
+
 // ---- bounds of the blocks of whole sequences ------------------------------------------------------------------------
 // One CTA per block and 64 bytes x 8 of its columns: 32 vectors of columns, 8 threads each taking every 8th token, four
 // tokens in flight.  A NaN key makes its column's bounds NaN.
@@ -130,7 +143,12 @@ __global__ void __launch_bounds__(256) block_scores_kernel(const T *q, const T *
         if (s >= s_hi) continue;
         for (int j = 0; j < 4; ++j) {
             const int64_t n = n0 + tx + 16 * j;
-            if (n < nb) keys[((s - s_lo) * gridDim.z + blockIdx.z) * nb + n] = n == s / block ? kOwnKey : key_of(acc[i][j]);
+            if (n >= nb) continue;
+            if (!(fabs(acc[i][j]) < INFINITY)) {
+                const T *low = bounds + ((b * nb + n) * 2 * Hkv + h) * D;
+                acc[i][j] = score_by_terms(q + ((b * S + s) * H + h * G) * D, low, low + Hkv * D, G, (int)D);
+            }
+            keys[((s - s_lo) * gridDim.z + blockIdx.z) * nb + n] = n == s / block ? kOwnKey : key_of(acc[i][j]);
         }
     }
 }
@@ -490,7 +508,10 @@ __global__ void __launch_bounds__(128, PER <= 4 ? 8 : 1) select_rows_kernel(cons
                         }
 #pragma unroll
                         for (int x2 = 16; x2 > 0; x2 >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x2);
-                        if (lane == who) exact[j] = key_of(t);
+                        if (lane == who) {
+                            if (!(fabs(t) < INFINITY)) t = score_by_terms(q + ((b * of.S + s) * H + h * G) * D, low, high, G, (int)D);
+                            exact[j] = key_of(t);
+                        }
                     }
                 }
                 topk_of_warp<PER>(exact, n, k, topk, o);
@@ -694,6 +715,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1) select_pages_
         }
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        if (!(fabs(s) < INFINITY)) {
+            const T *low = bounds + (phys * 2 * Hkv + h) * D;
+            s = score_by_terms(q + b * q_stride + h * G * D, low, low + Hkv * D, G, (int)D);
+        }
         return key_of(s);
     };
     if (want > 0)

@@ -50,3 +50,25 @@ def test_keys_that_are_not_numbers_make_their_page_the_last_choice(dtype, D):
                 for h in range(Hkv):
                     assert pages[0, h].tolist() == choose(scores(q[n - 1], want, used, h, H // Hkv), len(used) - 1, topk), (n, h, topk)
     assert nat.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, H, D", [(torch.bfloat16, 2, 64), (torch.float32, 6, 64)])
+def test_pages_with_infinite_keys_score_by_the_definition(dtype, H, D):
+    """An infinite bound counts for the heads whose sign takes it, and is not a number for a query of zero."""
+    B, n_pages, page, Hkv = 4, 40, 8, 2
+    g = torch.Generator().manual_seed(32)
+    kb = torch.randn(n_pages, 2, Hkv, D, generator=g).sort(1).values.to(dtype)
+    kb[3, 1, 0, 5], kb[7, 0, 1, 2], kb[9, 0, :, 4], kb[9, 1, :, 4], kb[20, 0, :, 1] = math.inf, -math.inf, -math.inf, math.inf, -math.inf
+    q = torch.randn(B, H, D, generator=g).to(dtype)
+    q[0, :, 5], q[1, 0, 4] = 0, 0
+    k = torch.zeros(n_pages, page, Hkv, D, dtype=dtype, device="cuda")
+    cache = mt.PagedKVCache.from_tensors(k, k.clone(), key_bounds=kb.cuda())
+    table = torch.stack([torch.randperm(n_pages, generator=g) for _ in range(B)])
+    n = torch.full((B,), n_pages * page, dtype=torch.int32)
+    for topk in (2, 6, 38):
+        pages = paged.select_pages(q.cuda(), cache, table.int().cuda(), n.cuda(), topk).cpu()
+        for b in range(B):
+            for h in range(Hkv):
+                assert pages[b, h].tolist() == choose(scores(q[b], kb, table[b], h, H // Hkv), n_pages - 1, topk), (b, h, topk)
+    assert nat.device_status() == 0

@@ -121,3 +121,18 @@ def test_blocks_with_a_key_that_is_not_a_number_are_chosen_last(S, D, dtype, cau
         check_choice(q, k, 16, topk, causal, rows)
     if S < 1000:
         check_choice(q, k, 16, 40, causal, rows)          # more places than blocks that are numbers
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("S, H, D, dtype", [(500, 2, 64, torch.bfloat16), (500, 6, 80, torch.float16), (500, 4, 64, torch.float32), (16500, 2, 8, torch.bfloat16)])
+def test_blocks_with_infinite_keys_score_by_the_definition(S, H, D, dtype, causal):
+    """An infinite bound counts for the heads whose sign takes it, and is not a number for a query of zero."""
+    q, k, _, _ = inputs(1, S, H, 2, D, dtype, seed=23)
+    inf = float("inf")
+    k[0, 3, 0, 5], k[0, 47, 1, D - 1], k[0, 111, :, 0], k[0, 150, 0, 3], k[0, 151, 0, 3], k[0, 200:232, :, 6] = inf, -inf, inf, inf, -inf, -inf
+    q[0, ::7, :, 5] = 0
+    q[0, 1::7, 0, 6] = 0
+    rows = list(range(0, 240, 3)) + [S - 17, S - 2, S - 1]
+    for topk in (3, 14):
+        check_choice(q, k, 16, topk, causal, rows)
