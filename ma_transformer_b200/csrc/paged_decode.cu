@@ -739,7 +739,7 @@ struct DecodePlan { int nsplit, min_chunk, cluster; };
 DecodePlan plan(const mat_paged_cache *c, int64_t B, int64_t width, int64_t left, int64_t n_sel) {
     int64_t most = width * c->page_size;
     if (n_sel > 0) most = n_sel * c->page_size;
-    else if (left >= 0 && left + 16 < most) most = left + 16;   // up to 15 tokens before the window's first
+    else if (left >= 0 && left < most - 16) most = left + 16;   // up to 15 tokens before the window's first
     const int64_t rows = B * c->H_kv;
     DecodePlan p;
     if (rows * 8 <= kSms && most <= 8192) {       // one cluster of at most eight chunks per row, all of them resident
