@@ -763,7 +763,7 @@ DecodePlan plan(const mat_paged_cache *c, int64_t B, int64_t width, int64_t left
 int check_decode(const mat_paged_cache *c, int64_t B, int64_t H, int64_t left, int64_t n_sel) {
     if (H < c->H_kv || H % c->H_kv) return fail(MAT_ERR_INVALID, "H = %lld query heads do not divide over H_kv = %lld key heads", (long long)H, (long long)c->H_kv);
     if (H > 65535) return fail(MAT_ERR_UNSUPPORTED, "at most 65535 query heads");
-    if (n_sel < 0 || n_sel * c->page_size > INT_MAX) return fail(MAT_ERR_INVALID, "the list of pages is too long");
+    if (n_sel < 0 || n_sel > INT_MAX / c->page_size) return fail(MAT_ERR_INVALID, "the list of pages is too long");
     (void)B; (void)left;
     return MAT_OK;
 }
