@@ -834,8 +834,8 @@ int check_select(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dt
     if (D % 8 || D > 128) return fail(MAT_ERR_UNSUPPORTED, "block selection takes head widths that are multiples of 8 up to 128, got %lld", (long long)D);
     if (block < 16 || block > 128 || block % 16) return fail(MAT_ERR_UNSUPPORTED, "block must be a multiple of 16 from 16 to 128, got %lld", (long long)block);
     if (topk < 1 || topk > 1024) return fail(MAT_ERR_UNSUPPORTED, "topk must be in [1, 1024], got %lld", (long long)topk);
-    if (B * Hkv > 65535 || B > 65535) return fail(MAT_ERR_UNSUPPORTED, "B * H_kv must be at most 65535");
-    if (S > (1ll << 30) / block * block) return fail(MAT_ERR_UNSUPPORTED, "the sequence is too long");
+    if (B > 65535 || Hkv > 65535 || B * Hkv > 65535) return fail(MAT_ERR_UNSUPPORTED, "B * H_kv must be at most 65535");
+    if (H > INT_MAX || S > (1ll << 30) / block * block) return fail(MAT_ERR_UNSUPPORTED, "the sequence is too long");
     return MAT_OK;
 }
 

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ma_transformer_b200 import _native as nat
 from ma_transformer_b200 import selected_attention as sel
 
 
@@ -23,3 +24,18 @@ def test_more_rows_than_lanes_count_in_32_bits():
     grads_l = sel.backward_selected(ql, kl, vl, out_l, lse_l, ql, own, block)
     for name, whole, last in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads), (out_l, lse_l, *grads_l)):
         assert torch.equal(whole[:, -block:], last), name
+
+
+@pytest.mark.parametrize("change", [dict(S=2 ** 60), dict(S=2 ** 62 + 64), dict(B=2 ** 48, H=2 ** 16, Hkv=2 ** 16), dict(B=2 ** 15, H=2 ** 49, Hkv=2 ** 49),
+                                    dict(H=2 ** 60), dict(H=2 ** 62), dict(S=2 ** 30, H=2 ** 4, topk=1)])
+def test_sizes_whose_products_wrap_are_refused(change):
+    a = dict(B=1, S=64, H=4, Hkv=2, D=64, dtype=nat.MAT_BF16, block=16, topk=16)
+    a.update(change)
+    shape, rest, p = (a["B"], a["S"], a["H"], a["Hkv"], a["D"], a["dtype"]), (a["block"], a["topk"]), 256
+    assert nat.lib.mat_selected_attn_fwd_workspace_bytes(*shape, *rest) == 0
+    assert nat.lib.mat_selected_attn_bwd_workspace_bytes(*shape, *rest) == 0
+    assert nat.lib.mat_selected_attn_fwd(p, p, p, p, p, *shape, p, *rest, 1, 0.0, None, 0, None) in (1, 2)
+    assert nat.lib.mat_selected_attn_bwd(p, p, p, p, p, p, p, p, p, *shape, p, *rest, 1, 0.0, None, 0, None) in (1, 2)
+    if a["topk"] != 1:                       # the selection itself takes longer sequences
+        assert nat.lib.mat_select_blocks_workspace_bytes(*shape, *rest) == 0
+        assert nat.lib.mat_select_blocks(p, p, *shape, *rest, 1, p, None, 0, None) in (1, 2)
