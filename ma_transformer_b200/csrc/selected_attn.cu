@@ -64,19 +64,19 @@ __device__ __forceinline__ TileLists tile_lists(const SelProblem &p, int64_t til
     return TileLists{p, p.blocks + ((b * p.S + i0) * p.Hkv + h) * p.topk, (int)min((int64_t)kTile, p.S - i0), stage};
 }
 
-__global__ void __launch_bounds__(kTile) lists_count_kernel(const SelProblem p, const SelLists l) {
+__global__ void __launch_bounds__(kTile) lists_count_kernel(const SelProblem p, const SelLists l, int64_t bh0) {
     __shared__ int hist[kRange], stage[kTile][kStage + 1];
     const int64_t tile = blockIdx.x, bh = blockIdx.z;
     const int n0 = blockIdx.y * kRange, n1 = min(n0 + kRange, (int)p.nb), tid = threadIdx.x;
     pdl_trigger();
     for (int i = tid; i < n1 - n0; i += kTile) hist[i] = 0;
     pdl_wait();
-    tile_lists(p, tile, bh, stage).each(own_limit(p, tile * kTile + tid), n0, n1, [&](int n, int) { atomicAdd(&hist[n - n0], 1); });
+    tile_lists(p, tile, bh0 + bh, stage).each(own_limit(p, tile * kTile + tid), n0, n1, [&](int n, int) { atomicAdd(&hist[n - n0], 1); });
     __syncthreads();
     for (int n = n0 + tid; n < n1; n += kTile) l.counts[(bh * l.tiles + tile) * p.nb + n] = hist[n - n0];
 }
 
-__global__ void __launch_bounds__(kTile) lists_fill_kernel(const SelProblem p, const SelLists l) {
+__global__ void __launch_bounds__(kTile) lists_fill_kernel(const SelProblem p, const SelLists l, int64_t bh0) {
     extern __shared__ int fill_smem[];
     uint32_t (*mask)[kTile / 32] = (uint32_t (*)[kTile / 32])fill_smem;            // [kRange][kTile / 32]
     int *start = fill_smem + kRange * (kTile / 32);                                // [kRange]
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kTile) lists_fill_kernel(const SelProblem p, c
     pdl_wait();
     for (int i = tid; i < n1 - n0; i += kTile) start[i] = l.base[bh * (p.nb + 1) + n0 + i] + l.counts[(bh * l.tiles + tile) * p.nb + n0 + i];
     const int limit = own_limit(p, tile * kTile + tid);
-    TileLists lists = tile_lists(p, tile, bh, stage);
+    TileLists lists = tile_lists(p, tile, bh0 + bh, stage);
     lists.each(limit, n0, n1, [&](int n, int) { atomicOr(&mask[n - n0][tid / 32], 1u << (tid % 32)); });
     __syncthreads();
     int32_t *entries = l.entry + bh * p.S * p.topk;
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb
         if (n < nb) l.base[bh * (nb + 1) + n] = entries + sum - x;
         const int mine = (int)(((int64_t)x * G + rows_per_item - 1) / rows_per_item);
         const int isum = block_scan(mine, of_warp);
-        if (items && n < nb) {
+        if (n < nb) {
             const int at = before + isum - mine;
             item_base[bh * (nb + 1) + n] = at;
             for (int i = 0; i < mine; ++i) items[bh * max_items + at + i] = make_int2((int)n, i * rows_per_item);
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(1024) lists_base_kernel(SelLists l, int64_t nb
     }
     if (threadIdx.x == 0) {
         l.base[bh * (nb + 1) + nb] = entries;
-        if (items) item_base[bh * (nb + 1) + nb] = before;
+        item_base[bh * (nb + 1) + nb] = before;
     }
 }
 
@@ -181,31 +181,29 @@ int check_selected(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int 
 
 }  // namespace
 
-size_t sel_lists_bytes(int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk) {
-    const int64_t tiles = (S + kTile - 1) / kTile, bh = B * Hkv;
-    return sel_align((size_t)bh * nb * tiles * 4) + sel_align((size_t)bh * (nb + 1) * 4) +
-           sel_align((size_t)bh * S * topk * 4);
+size_t sel_lists_bytes(int64_t pairs, int64_t S, int64_t nb, int64_t topk) {
+    const int64_t tiles = (S + kTile - 1) / kTile;
+    return sel_align((size_t)pairs * nb * tiles * 4) + sel_align((size_t)pairs * (nb + 1) * 4) + sel_align((size_t)pairs * S * topk * 4);
 }
 
-SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk) {
+SelLists sel_lists_at(void *ws, int64_t pairs, int64_t S, int64_t nb, int64_t topk) {
     SelLists l;
     l.tiles = (S + kTile - 1) / kTile;
-    const int64_t bh = B * Hkv;
     char *at = (char *)ws;
-    l.counts = (int32_t *)at; at += sel_align((size_t)bh * nb * l.tiles * 4);
-    l.base = (int32_t *)at;   at += sel_align((size_t)bh * (nb + 1) * 4);
+    l.counts = (int32_t *)at; at += sel_align((size_t)pairs * nb * l.tiles * 4);
+    l.base = (int32_t *)at;   at += sel_align((size_t)pairs * (nb + 1) * 4);
     l.entry = (int32_t *)at;
     return l;
 }
 
-int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item) {
-    const unsigned bh = (unsigned)(p.B * p.Hkv);
-    const dim3 grid((unsigned)l.tiles, (unsigned)((p.nb + kRange - 1) / kRange), bh);
-    lists_count_kernel<<<grid, kTile, 0, p.stream>>>(p, l);
-    launch_after(lists_base_kernel, dim3(bh), dim3(1024), 0, p.stream, l, p.nb, (int)(p.H / p.Hkv), items, item_base, max_items, rows_per_item);
+int launch_sel_lists(const SelProblem &p, const SelLists &l, int64_t bh0, int64_t pairs, int2 *items, int32_t *item_base, int64_t max_items,
+                     int rows_per_item) {
+    const dim3 grid((unsigned)l.tiles, (unsigned)((p.nb + kRange - 1) / kRange), (unsigned)pairs);
+    lists_count_kernel<<<grid, kTile, 0, p.stream>>>(p, l, bh0);
+    launch_after(lists_base_kernel, dim3((unsigned)pairs), dim3(1024), 0, p.stream, l, p.nb, (int)(p.H / p.Hkv), items, item_base, max_items, rows_per_item);
     const size_t smem = (kRange * (kTile / 32 + 1) + kTile * (kStage + 1)) * sizeof(int);
     if (int rc = ensure_dynamic_smem((const void *)lists_fill_kernel, smem, "shared memory of the lists of a block selection")) return rc;
-    launch_after(lists_fill_kernel, grid, dim3(kTile), smem, p.stream, p, l);
+    launch_after(lists_fill_kernel, grid, dim3(kTile), smem, p.stream, p, l, bh0);
     return launched("launching the lists of a block selection");
 }
 

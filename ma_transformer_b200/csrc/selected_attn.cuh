@@ -19,7 +19,8 @@ struct SelProblem {
     cudaStream_t stream;
 };
 
-// Which queries chose a block, the selection turned round: for (batch, key head) bh and block n the entries
+// Which queries chose a block, the selection turned round, for a group of (batch, key head) pairs: for pair bh of the group
+// and block n the entries
 // [base[bh * (nb + 1) + n], base[bh * (nb + 1) + n + 1]) of entry[bh * S * topk + ...], ascending, each
 // query * topk + the place of the block in the query's list.
 struct SelLists {
@@ -28,11 +29,12 @@ struct SelLists {
     int32_t *entry;    // [bh][S * topk]
     int64_t tiles;
 };
-size_t sel_lists_bytes(int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk);
-SelLists sel_lists_at(void *ws, int64_t B, int64_t S, int64_t Hkv, int64_t nb, int64_t topk);
-// Fills the lists and, where items is given, cuts each block's rows (entries x query heads of a key head) into items of
+size_t sel_lists_bytes(int64_t pairs, int64_t S, int64_t nb, int64_t topk);
+SelLists sel_lists_at(void *ws, int64_t pairs, int64_t S, int64_t nb, int64_t topk);
+// Fills the lists of pairs [bh0, bh0 + pairs) and cuts each block's rows (entries x query heads of a key head) into items of
 // rows_per_item: items[bh * max_items + x] = (block, first row) for x in [item_base[bh * (nb + 1) + n], ...[n + 1]).
-int launch_sel_lists(const SelProblem &p, const SelLists &l, int2 *items, int32_t *item_base, int64_t max_items, int rows_per_item);
+int launch_sel_lists(const SelProblem &p, const SelLists &l, int64_t bh0, int64_t pairs, int2 *items, int32_t *item_base, int64_t max_items,
+                     int rows_per_item);
 
 // selected_tiles.cu
 size_t sel_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, int64_t block, int64_t topk, bool bwd);

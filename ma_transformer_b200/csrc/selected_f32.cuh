@@ -66,14 +66,15 @@ __device__ __forceinline__ void stage_f32(float *dst, const float *src, int64_t 
 }
 
 __global__ void __launch_bounds__(kF32Threads) sel_fwd_f32_kernel(const SelProblem p, const SelTile t) {
+    const int64_t bhl = blockIdx.y;
     const int bh = (int)t.bh0 + blockIdx.y;
     const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
-    if ((int)blockIdx.x >= t.item_base[(int64_t)bh * (p.nb + 1) + p.nb]) return;
-    const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
-    const int n = item.x, e0 = t.l.base[(int64_t)bh * (p.nb + 1) + n], D = (int)p.D, pitch = D + 4, T_ = (int)p.topk, block = (int)p.block;
-    const int rows_all = (t.l.base[(int64_t)bh * (p.nb + 1) + n + 1] - e0) * t.G, r_end = min(item.y + kF32Rows, rows_all);
+    if ((int)blockIdx.x >= t.item_base[bhl * (p.nb + 1) + p.nb]) return;
+    const int2 item = t.items[bhl * t.max_items + blockIdx.x];
+    const int n = item.x, e0 = t.l.base[bhl * (p.nb + 1) + n], D = (int)p.D, pitch = D + 4, T_ = (int)p.topk, block = (int)p.block;
+    const int rows_all = (t.l.base[bhl * (p.nb + 1) + n + 1] - e0) * t.G, r_end = min(item.y + kF32Rows, rows_all);
     const int64_t j0 = (int64_t)n * block;
     const int held = (int)min((int64_t)block, p.S - j0), key_rows = (block + 63) / 64 * 64;
     extern __shared__ __align__(16) char smem[];
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kF32Threads) sel_fwd_f32_kernel(const SelProbl
             const int r = first + tid;
             int i = -1, at = 0;
             if (r < r_end) {
-                const int e = r / t.G, entry = t.l.entry[(int64_t)bh * p.S * T_ + e0 + e];
+                const int e = r / t.G, entry = t.l.entry[bhl * p.S * T_ + e0 + e];
                 i = entry / T_;
                 at = (i * t.G + r - e * t.G) * T_ + entry - i * T_;
             }
@@ -211,10 +212,10 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
     const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
-    if ((int)blockIdx.x >= t.item_base[(int64_t)bh * (p.nb + 1) + p.nb]) return;
-    const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
-    const int n = item.x, e0 = t.l.base[(int64_t)bh * (p.nb + 1) + n], D = (int)p.D, pitch = D + 4, T_ = (int)p.topk, vecs = D / 4;
-    const int rows_all = (t.l.base[(int64_t)bh * (p.nb + 1) + n + 1] - e0) * t.G, r_end = min(item.y + kF32BwdRows, rows_all);
+    if ((int)blockIdx.x >= t.item_base[bhl * (p.nb + 1) + p.nb]) return;
+    const int2 item = t.items[bhl * t.max_items + blockIdx.x];
+    const int n = item.x, e0 = t.l.base[bhl * (p.nb + 1) + n], D = (int)p.D, pitch = D + 4, T_ = (int)p.topk, vecs = D / 4;
+    const int rows_all = (t.l.base[bhl * (p.nb + 1) + n + 1] - e0) * t.G, r_end = min(item.y + kF32BwdRows, rows_all);
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
     const int keys = min((int)p.block - sub * 64, 64), held = (int)max((int64_t)0, min((int64_t)keys, p.S - j0));
     if (held == 0) return;                                   // the sequence ends before this half
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
             int i = -1, at = 0;
             float lse = 0.f, delta = 0.f;
             if (r < r_end) {
-                const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[(int64_t)bh * p.S * T_ + e0 + e];
+                const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bhl * p.S * T_ + e0 + e];
                 i = entry / T_;
                 at = (i * t.G + g) * T_ + entry - i * T_;
                 const int64_t row = (b * p.S + i) * p.H + h * t.G + g;
@@ -338,21 +339,22 @@ __global__ void __launch_bounds__(kF32Threads) sel_bwd_f32_kernel(const SelProbl
         }
     }
     cp_async_wait<0>();
-    float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
+    float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * t.kv_rows * D;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int x = tid + u * kF32Threads, rg = x / vecs, col = (x - rg * vecs) * 4;
         if (rg >= 16) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            const int r = 4 * rg + i;
+            if (r >= t.kv_rows) break;
             if (odd_rows) {
-                const int r = 4 * rg + i;
                 float4 &x = dk[u][i], &y = dv[u][i];
                 x.x = odd.dk(x.x, r, col); x.y = odd.dk(x.y, r, col + 1); x.z = odd.dk(x.z, r, col + 2); x.w = odd.dk(x.w, r, col + 3);
                 y.x = odd.dv(y.x, r, col); y.y = odd.dv(y.y, r, col + 1); y.z = odd.dv(y.z, r, col + 2); y.w = odd.dv(y.w, r, col + 3);
             }
-            *reinterpret_cast<float4 *>(out + (4 * rg + i) * D + col) = dk[u][i];
-            *reinterpret_cast<float4 *>(out + (64 + 4 * rg + i) * D + col) = dv[u][i];
+            *reinterpret_cast<float4 *>(out + r * D + col) = dk[u][i];
+            *reinterpret_cast<float4 *>(out + (t.kv_rows + r) * D + col) = dv[u][i];
         }
     }
 }

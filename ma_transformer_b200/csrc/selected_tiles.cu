@@ -9,7 +9,8 @@
 // `rows per item` rows and then over the items in order: nothing depends on timing, there are no atomics.
 //
 // The partials are the traffic: 4 D bytes written and read per (row, block) against 2 D for the gathered query, so the
-// (batch, key head) pairs are worked off in groups whose partials take about kPartBudget bytes.  Groups small enough for
+// (batch, key head) pairs are worked off in groups whose partials and lists take at most kPairBudget bytes (one pair where
+// that takes more; beside them the backward holds 4 bytes a row).  Groups small enough for
 // L2 (64 MB) were slower than all pairs at once, for the tails of their launches: 281 + 446 against 247 + 377 us forward
 // and backward at 8192 tokens x 8 heads of 64 x 16 blocks, so the budget only bounds the workspace.
 #include <cmath>
@@ -27,20 +28,20 @@ constexpr int kFwdRows = 256;        // rows per forward item (a multiple of 64)
 // of 64, 75 -> 62 at 2 x 1000 x 4 heads of 32; forward with 64: 241 -> 259.
 constexpr int kF32Rows = 128, kF32BwdRows = 64;
 constexpr int kBwdRows = 512;        // rows per backward item
-constexpr size_t kPartBudget = 1024ull << 20;
+constexpr size_t kPairBudget = 1024ull << 20;
 
 struct SelTile {                     // what the kernels need beside SelProblem
     SelLists l;
-    const int2 *items;               // [bh][max_items] (block, first row)
-    const int32_t *item_base;        // [bh][nb + 1]
+    int2 *items;                     // [group bh][max_items] (block, first row)
+    int32_t *item_base;              // [group bh][nb + 1]
     int64_t max_items;
     float2 *stats;                   // [group rows][slots]
     float *part;                     // [group rows][slots][D]
-    float *kv_part;                  // [group bh][max_items][nsub][2][64][D]
+    float *kv_part;                  // [group bh][max_items][nsub][2][kv_rows][D]
     const float *delta;
     float *delta_part;               // [group rows][slots][nsub]: shares of delta (few keys a row)
     int64_t bh0;                     // first (batch, key head) of the group
-    int G, nsub;
+    int G, nsub, kv_rows;            // kv_rows: keys of a (sub-)block, 64 at most
     float scale_log2;
 };
 
@@ -106,14 +107,15 @@ namespace {
 // EXACT: D == DP and a block is a whole number of NKP keys, known to the compiler.
 template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_bounds__(128, DP == 64 ? 4 : 3) sel_fwd_mma_kernel(const SelProblem p, const SelTile t) {
     constexpr int PITCH = DP + 8, NF = NKP / 8;
+    const int64_t bhl = blockIdx.y;
     const int bh = (int)t.bh0 + blockIdx.y;
     const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
-    if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
-    const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
-    const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n];
-    const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
+    if ((int)blockIdx.x >= t.item_base[bhl * (p.nb + 1) + p.nb]) return;
+    const int2 item = t.items[bhl * t.max_items + blockIdx.x];
+    const int n = item.x, e0 = t.l.base[bhl * (p.nb + 1) + n];
+    const int rows_all = (t.l.base[bhl * (p.nb + 1) + n + 1] - e0) * t.G;
     const int r_end = min(item.y + kFwdRows, rows_all);
     const int D = EXACT ? DP : (int)p.D, d16 = EXACT ? DP / 16 : (D + 15) / 16, block = (int)p.block, T_ = (int)p.topk;
     const int64_t j0 = (int64_t)n * block;
@@ -134,7 +136,7 @@ template <typename T, int DP, int NKP, bool EXACT> __global__ void __launch_boun
         const int r = item.y + x;
         int i = -1, src = 0, at = 0;
         if (r < r_end) {
-            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[(int64_t)bh * p.S * T_ + e0 + e];
+            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bhl * p.S * T_ + e0 + e];
             i = entry / T_;
             src = i * (int)p.H + g;
             at = (i * t.G + g) * T_ + entry - i * T_;
@@ -415,10 +417,10 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
     const int64_t b = bh / (int)p.Hkv, h = bh - b * p.Hkv;
     pdl_trigger();
     pdl_wait();
-    if ((int)blockIdx.x >= t.item_base[bh * (p.nb + 1) + p.nb]) return;
-    const int2 item = t.items[(int64_t)bh * t.max_items + blockIdx.x];
-    const int n = item.x, e0 = t.l.base[bh * (p.nb + 1) + n], sub = blockIdx.y;
-    const int rows_all = (t.l.base[bh * (p.nb + 1) + n + 1] - e0) * t.G;
+    if ((int)blockIdx.x >= t.item_base[bhl * (p.nb + 1) + p.nb]) return;
+    const int2 item = t.items[bhl * t.max_items + blockIdx.x];
+    const int n = item.x, e0 = t.l.base[bhl * (p.nb + 1) + n], sub = blockIdx.y;
+    const int rows_all = (t.l.base[bhl * (p.nb + 1) + n + 1] - e0) * t.G;
     const int r_end = min(item.y + kBwdRows, rows_all);
     const int D = EXACT ? DP : (int)p.D, d16 = EXACT ? DP / 16 : (D + 15) / 16, T_ = (int)p.topk;
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
@@ -441,7 +443,7 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
         int i = -1, at = 0, src = 0;
         float lse = 0.f, delta = 0.f;
         if (r < r_end) {
-            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[(int64_t)bh * p.S * T_ + e0 + e];
+            const int e = r / t.G, g = r - e * t.G, entry = t.l.entry[bhl * p.S * T_ + e0 + e];
             i = entry / T_;
             at = (i * t.G + g) * T_ + entry - i * T_;
             src = i * (int)p.H + g;
@@ -665,7 +667,7 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
     }
     if (DELTA) return;
     cp_async_wait<0>();
-    float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * 64 * D;
+    float *out = t.kv_part + (((bhl * t.max_items + blockIdx.x) * t.nsub + sub) * 2) * t.kv_rows * D, *out_v = out + t.kv_rows * D;
     if (kg < n16)
 #pragma unroll
         for (int c = 0; c < CF; ++c)
@@ -675,8 +677,8 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
                 if ((cg * CF + c) * 16 + x * 8 < D) {
                     *reinterpret_cast<float2 *>(out + row * D + col) = make_float2(dk[c][x][0], dk[c][x][1]);
                     *reinterpret_cast<float2 *>(out + (row + 8) * D + col) = make_float2(dk[c][x][2], dk[c][x][3]);
-                    *reinterpret_cast<float2 *>(out + (64 + row) * D + col) = make_float2(dv[c][x][0], dv[c][x][1]);
-                    *reinterpret_cast<float2 *>(out + (64 + row + 8) * D + col) = make_float2(dv[c][x][2], dv[c][x][3]);
+                    *reinterpret_cast<float2 *>(out_v + row * D + col) = make_float2(dv[c][x][0], dv[c][x][1]);
+                    *reinterpret_cast<float2 *>(out_v + (row + 8) * D + col) = make_float2(dv[c][x][2], dv[c][x][3]);
                 }
             }
     if (odd_rows) {
@@ -684,7 +686,7 @@ template <typename T, int DP, int NKP, bool EXACT, bool DELTA> __global__ void _
         for (int x = threadIdx.x; x < keys * D; x += 128) {
             const int row = x / D, col = x - row * D;
             out[x] = odd.dk(out[x], row, col);
-            out[64 * D + x] = odd.dv(out[64 * D + x], row, col);
+            out_v[x] = odd.dv(out_v[x], row, col);
         }
     }
 }
@@ -699,14 +701,14 @@ template <typename T> __global__ void __launch_bounds__(128) sel_kv_join_kernel(
     const int n = blockIdx.x / t.nsub, sub = blockIdx.x % t.nsub, D = (int)p.D;
     const int64_t j0 = (int64_t)n * p.block + sub * 64;
     const int held = (int)min((int64_t)min((int)p.block - sub * 64, 64), p.S - j0);
-    const int i0 = t.item_base[bh * (p.nb + 1) + n], i1 = t.item_base[bh * (p.nb + 1) + n + 1];
+    const int i0 = t.item_base[bhl * (p.nb + 1) + n], i1 = t.item_base[bhl * (p.nb + 1) + n + 1];
     const int x = blockIdx.z * 128 + threadIdx.x;
     if (x < held * D / 4) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
-            const float *src = t.kv_part + (((bhl * t.max_items + i) * t.nsub + sub) * 2) * 64 * D;
-            const float4 u = *reinterpret_cast<const float4 *>(src + x * 4), w = *reinterpret_cast<const float4 *>(src + 64 * D + x * 4);
+            const float *src = t.kv_part + (((bhl * t.max_items + i) * t.nsub + sub) * 2) * t.kv_rows * D;
+            const float4 u = *reinterpret_cast<const float4 *>(src + x * 4), w = *reinterpret_cast<const float4 *>(src + t.kv_rows * D + x * 4);
             a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
             c.x += w.x; c.y += w.y; c.z += w.z; c.w += w.w;
         }
@@ -793,7 +795,7 @@ int launched(const char *what) {
 // What lies where in the workspace.
 struct Plan {
     int64_t max_items, group;       // items per (batch, key head); pairs worked off together
-    int nsub;
+    int nsub, kv_rows;
     size_t lists, items, base, stats, part, kv, delta, delta_part, total;
 };
 
@@ -808,28 +810,33 @@ Plan plan(int64_t B, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype, in
     w.nsub = bwd ? (int)((block + 63) / 64) : 1;
     const int64_t rows = rows_per_item(dtype, bwd);
     w.max_items = S * topk * G / rows + nb;
-    const size_t per = (size_t)S * G * topk * w.nsub * D * 4;
-    w.group = per >= kPartBudget ? 1 : (int64_t)(kPartBudget / per);
+    w.kv_rows = (int)(block < 64 ? block : 64);
+    const size_t part = (size_t)S * G * topk * w.nsub * D * 4, kv = bwd ? (size_t)w.max_items * w.nsub * 2 * w.kv_rows * D * 4 : 0;
+    const size_t stats = bwd ? 0 : (size_t)S * G * topk * sizeof(float2);
+    const size_t shares = bwd && dtype != MAT_F32 && few_keys(block, topk) ? (size_t)S * G * topk * w.nsub * 4 : 0;
+    const size_t pair = part + kv + stats + shares + (size_t)w.max_items * sizeof(int2) + (size_t)(nb + 1) * 4 + sel_lists_bytes(1, S, nb, topk);
+    w.group = pair >= kPairBudget ? 1 : (int64_t)(kPairBudget / pair);
     if (w.group > bh) w.group = bh;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += sel_align(n); return x; };
-    w.lists = take(sel_lists_bytes(B, S, Hkv, nb, topk));
-    w.items = take((size_t)bh * w.max_items * sizeof(int2));
-    w.base = take((size_t)bh * (nb + 1) * 4);
-    w.stats = take(bwd ? 0 : (size_t)w.group * S * G * topk * sizeof(float2));
-    w.part = take((size_t)w.group * per);
-    w.kv = take(bwd ? (size_t)w.group * w.max_items * w.nsub * 2 * 64 * D * 4 : 0);
+    w.lists = take(sel_lists_bytes(w.group, S, nb, topk));
+    w.items = take((size_t)w.group * w.max_items * sizeof(int2));
+    w.base = take((size_t)w.group * (nb + 1) * 4);
+    w.stats = take(w.group * stats);
+    w.part = take(w.group * part);
+    w.kv = take(w.group * kv);
     w.delta = take(bwd ? (size_t)B * S * H * 4 : 0);
-    w.delta_part = take(bwd && dtype != MAT_F32 && few_keys(block, topk) ? (size_t)w.group * S * G * topk * w.nsub * 4 : 0);
+    w.delta_part = take(w.group * shares);
     w.total = at;
     return w;
 }
 
-int prepare(const SelProblem &p, const Plan &w, void *ws, bool bwd, SelTile &t) {
+SelTile tile_args(const SelProblem &p, const Plan &w, void *ws) {
+    SelTile t{};
     char *at = (char *)ws;
-    t.l = sel_lists_at(at + w.lists, p.B, p.S, p.Hkv, p.nb, p.topk);
-    t.items = (const int2 *)(at + w.items);
-    t.item_base = (const int32_t *)(at + w.base);
+    t.l = sel_lists_at(at + w.lists, w.group, p.S, p.nb, p.topk);
+    t.items = (int2 *)(at + w.items);
+    t.item_base = (int32_t *)(at + w.base);
     t.max_items = w.max_items;
     t.stats = (float2 *)(at + w.stats);
     t.part = (float *)(at + w.part);
@@ -838,15 +845,17 @@ int prepare(const SelProblem &p, const Plan &w, void *ws, bool bwd, SelTile &t) 
     t.delta_part = (float *)(at + w.delta_part);
     t.G = (int)(p.H / p.Hkv);
     t.nsub = w.nsub;
+    t.kv_rows = w.kv_rows;
     t.scale_log2 = p.scale * 1.4426950408889634f;
-    return launch_sel_lists(p, t.l, (int2 *)(at + w.items), (int32_t *)(at + w.base), t.max_items, rows_per_item(p.dtype, bwd));
+    return t;
 }
 
-// The groups of pairs in turn: their tiles, then their joins.
+// The groups of pairs in turn: their lists, their tiles, then their joins.
 template <bool BWD, typename T, typename Launch> int over_groups(const SelProblem &p, const Plan &w, SelTile &t, Launch &&tiles) {
     const int64_t bh = p.B * p.Hkv;
     for (t.bh0 = 0; t.bh0 < bh; t.bh0 += w.group) {
         const int64_t n = bh - t.bh0 < w.group ? bh - t.bh0 : w.group;
+        if (int rc = launch_sel_lists(p, t.l, t.bh0, n, t.items, t.item_base, t.max_items, rows_per_item(p.dtype, BWD))) return rc;
         tiles((unsigned)n);
         launch_join<T, BWD>(p, t, n);
         if (BWD) launch_kv_join<T>(p, t, n);
@@ -869,9 +878,9 @@ template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, 
     if (int rc = ensure_dynamic_smem((const void *)grads, smem, "shared memory of the selected attention's backward")) return rc;
     if (int rc = few ? ensure_dynamic_smem((const void *)shares, smem, "shared memory of the selected attention's backward") : MAT_OK) return rc;
     float *delta = const_cast<float *>(t.delta);
-    if (!few) launch_delta<T>(p, delta);
     return over_groups<true, T>(p, w, t, [&](unsigned n) {
         const dim3 grid((unsigned)w.max_items, (unsigned)w.nsub, n);
+        if (!few && t.bh0 == 0) launch_delta<T>(p, delta);             // of all pairs
         if (few) {
             launch_after(shares, grid, dim3(128), smem, p.stream, p, t);
             launch_after(sel_delta_join_kernel, dim3((unsigned)((p.S * t.G + 127) / 128), n), dim3(128), 0, p.stream, p, t, delta);
@@ -882,8 +891,7 @@ template <typename T, int DP, int NKP, bool EXACT> int bwd(const SelProblem &p, 
 
 int run_f32(const SelProblem &p, void *ws, bool back) {
     const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.dtype, p.block, p.topk, back);
-    SelTile t{};
-    if (int rc = prepare(p, w, ws, back, t)) return rc;
+    SelTile t = tile_args(p, w, ws);
     const size_t pitch = p.D + 4, key_rows = (p.block + 63) / 64 * 64;
     const size_t smem = ((back ? 4 * 64 : 2 * key_rows + 64) * pitch + (back ? 2 : 1) * 64 * kWPitch) * sizeof(float);
     if (int rc = ensure_dynamic_smem(back ? (const void *)sel_bwd_f32_kernel : (const void *)sel_fwd_f32_kernel, smem, "shared memory of the selected attention in fp32")) return rc;
@@ -891,16 +899,15 @@ int run_f32(const SelProblem &p, void *ws, bool back) {
         return over_groups<false, float>(p, w, t, [&](unsigned n) {
             launch_after(sel_fwd_f32_kernel, dim3((unsigned)w.max_items, n), dim3(kF32Threads), smem, p.stream, p, t);
         });
-    launch_delta<float>(p, const_cast<float *>(t.delta));
     return over_groups<true, float>(p, w, t, [&](unsigned n) {
+        if (t.bh0 == 0) launch_delta<float>(p, const_cast<float *>(t.delta));       // of all pairs
         launch_after(sel_bwd_f32_kernel, dim3((unsigned)w.max_items, (unsigned)w.nsub, n), dim3(kF32Threads), smem, p.stream, p, t);
     });
 }
 
 template <typename T> int run(const SelProblem &p, void *ws, bool back) {
     const Plan w = plan(p.B, p.S, p.H, p.Hkv, p.D, p.dtype, p.block, p.topk, back);
-    SelTile t{};
-    if (int rc = prepare(p, w, ws, back, t)) return rc;
+    SelTile t = tile_args(p, w, ws);
     const int dp = p.D <= 64 ? 64 : 128, nkp = p.block <= 32 ? 32 : 64;
     const bool exact = p.D == dp && p.block % nkp == 0;
 #define SEL_CASE(DP, NKP)                                                                        \
