@@ -72,3 +72,75 @@ def test_pages_with_infinite_keys_score_by_the_definition(dtype, H, D):
             for h in range(Hkv):
                 assert pages[b, h].tolist() == choose(scores(q[b], kb, table[b], h, H // Hkv), n_pages - 1, topk), (b, h, topk)
     assert nat.device_status() == 0
+
+
+# Batches of 148 and more (sequence, key head) rows are scored and selected by one CTA a row; fewer rows are scored by all
+# CTAs first.  Both are held to the definition, at every width that has a kernel of its own.
+
+def serving_batch(lengths, H, Hkv, D, page, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    used = [-(-n // page) for n in lengths]
+    n_pages = sum(used) + 1
+    kb = torch.randn(n_pages, 2, Hkv, D, generator=g).sort(1).values.to(dtype)
+    table = torch.full((len(lengths), max(used) + 2), -5, dtype=torch.int32)
+    ids = torch.randperm(n_pages, generator=g).tolist()
+    for b, n in enumerate(used):
+        for w in range(n):
+            table[b, w] = ids.pop()
+    return kb, table, torch.randn(len(lengths), H, D, generator=g).to(dtype)
+
+
+def check_pages(lengths, H, Hkv, page, kb, table, q, topks):
+    k = torch.zeros(kb.shape[0], page, Hkv, kb.shape[3], dtype=kb.dtype, device="cuda")
+    cache = mt.PagedKVCache.from_tensors(k, k, key_bounds=kb.cuda())
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = [[scores(q[b], kb, table[b, :-(-m // page)].long(), h, H // Hkv) for h in range(Hkv)] for b, m in enumerate(lengths)]
+    for topk in topks:
+        pages = paged.select_pages(q.cuda(), cache, table.cuda(), n, topk).cpu()
+        for b, m in enumerate(lengths):
+            for h in range(Hkv):
+                assert pages[b, h].tolist() == choose(want[b][h], (m - 1) // page, topk), (b, h, topk)
+    assert nat.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["many", "few"])
+@pytest.mark.parametrize("D, dtype", [(8, torch.bfloat16), (32, torch.float16), (64, torch.bfloat16), (72, torch.float16), (128, torch.bfloat16), (200, torch.float16),
+                                      (256, torch.bfloat16), (16, torch.float32), (24, torch.float32), (64, torch.float32), (80, torch.float32), (128, torch.float32),
+                                      (256, torch.float32)])
+def test_select_pages_of_batches(D, dtype, rows):
+    """Mixed lengths, idle slots and single tokens among them."""
+    lengths = [0, 1, 8, 9, 1500, 777, 64, 333, 2, 1201] * (4 if rows == "many" else 1)
+    kb, table, q = serving_batch(lengths, 8, 4, D, 8, dtype, D)
+    check_pages(lengths, 8, 4, 8, kb, table, q, (1, 4, 33))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, H, Hkv", [(150, 1, 1), (19, 40, 8)])
+def test_select_pages_of_batches_with_equal_bounds_and_bounds_that_are_not_numbers(B, H, Hkv):
+    lengths, page, D = [40 * 16 + (b % 3) * 16 - b % 5 for b in range(B)], 16, 64
+    kb, table, q = serving_batch(lengths, H, Hkv, D, page, torch.bfloat16, 50)
+    for b in range(B):
+        at = table[b, :38].long()
+        kb[at[5:38]] = kb[at[5]].clone()                  # 33 equal pages
+        kb[at[b % 5], b % 2, b % Hkv, b % D] = float("nan")
+        if b % 7 == 0:
+            kb[at[3:30], 0] = float("nan")
+    check_pages(lengths, H, Hkv, page, kb, table, q, (1, 2, 7, 36, 39, 60))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 150])
+def test_select_pages_where_more_pages_are_near_than_are_held(B):
+    """1500 pages whose bounds differ in one column's last bit: fp32 sums cannot tell them apart."""
+    page, D, n_pages = 8, 64, 1500
+    g = torch.Generator().manual_seed(51)
+    kb = (torch.randn(1, 1, 1, D, generator=g).bfloat16() * 8).expand(n_pages, 2, 1, D).contiguous()
+    for p in range(n_pages):
+        x = kb[p, 1, 0, (p * 7) % D].float()
+        kb[p, 1, 0, (p * 7) % D] = (x + x.abs() * torch.finfo(torch.bfloat16).eps).bfloat16()
+    q = torch.randn(B, 2, D, generator=g).bfloat16() * 1e-3
+    q[..., 0] = 30
+    lengths = [n_pages * page - b for b in range(B)]      # the table is shared: the same pages for every sequence
+    table = torch.randperm(n_pages, generator=g).int()[None].expand(B, n_pages).contiguous()
+    check_pages(lengths, 2, 1, page, kb, table, q, (5, 40) if B > 1 else (1, 5, 40, 1200))
