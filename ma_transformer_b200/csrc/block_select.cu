@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(128) block_norms_kernel(const T *bounds, float
 // first, first + step, ... of a row; `threads` threads take part.
 template <typename T, int LP, int NV>
 __device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds, const T *q, int64_t H, int64_t Hkv, int64_t D, int64_t b, int64_t h,
-                                            int n, int first, int step, float2 *scores, int *status) {
+                                            int n, int first, int step, float2 *scores) {
     constexpr int W = Vec16<T>::N, U = NV >= 4 ? 1 : NV == 2 ? 2 : 4;
     const int64_t G = H / Hkv;
     const int part = threadIdx.x % LP, vecs = (int)D / W;
@@ -336,7 +336,7 @@ __device__ __forceinline__ void score_pages(const PagedView &c, const T *bounds,
 
 template <typename T, int LP, int NV>
 __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *bounds, const T *q, int64_t q_stride, int64_t H, int64_t Hkv, int64_t D,
-                                                          const int32_t *lengths, float2 *scores, int *status) {
+                                                          const int32_t *lengths, float2 *scores) {
     constexpr int GROUPS = 256 / LP;
     const int64_t b = blockIdx.z, h = blockIdx.y;
     pdl_trigger();
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256) page_scores_kernel(PagedView c, const T *
     const int64_t held = ((len - 1) >> c.page_shift) + 1;      // pages that hold tokens; the last is the token's own
     const int n = (int)(held < c.width ? held : c.width), first = blockIdx.x * GROUPS;
     if (first < n)
-        score_pages<T, LP, NV>(c, bounds, q + b * q_stride, H, Hkv, D, b, h, n, first, gridDim.x * GROUPS, scores + (b * Hkv + h) * c.width, status);
+        score_pages<T, LP, NV>(c, bounds, q + b * q_stride, H, Hkv, D, b, h, n, first, gridDim.x * GROUPS, scores + (b * Hkv + h) * c.width);
 }
 
 // ---- the topk of a row -----------------------------------------------------------------------------------------------
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1) select_pages_
         up[d] = u; down[d] = w;
     }
     if (LP > 0) {
-        score_pages<T, LP ? LP : 32, NV>(c, bounds, q + b * q_stride, H, Hkv, D, b, h, n, 0, THREADS / (LP ? LP : 32), scores + row * c.width, status);
+        score_pages<T, LP ? LP : 32, NV>(c, bounds, q + b * q_stride, H, Hkv, D, b, h, n, 0, THREADS / (LP ? LP : 32), scores + row * c.width);
         __syncthreads();
     }
     const float2 *mine = scores + row * c.width;
@@ -948,7 +948,7 @@ int run_select_pages(const mat_paged_cache *c, const PagedView &v, const T *q, i
     const int64_t cap = 148 * 8 / (B * c->H_kv) + 1;         // enough CTAs to fill the GPU; each walks several pages
     if (gx > cap) gx = cap;
     const dim3 grid((unsigned)gx, (unsigned)c->H_kv, (unsigned)B);
-#define PAGE_SCORES(LP, NV) page_scores_kernel<T, LP, NV><<<grid, 256, 0, s>>>(v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores, status)
+#define PAGE_SCORES(LP, NV) page_scores_kernel<T, LP, NV><<<grid, 256, 0, s>>>(v, bounds, q, q_stride, H, c->H_kv, c->D, lengths, scores)
     if (lp == 8) PAGE_SCORES(8, 1);
     else if (vecs <= 16) PAGE_SCORES(16, 1);
     else if (vecs <= 32) PAGE_SCORES(16, 2);

@@ -5,7 +5,9 @@
 // kind (t -> first + t * dilation) or a list of pages (t -> slot t mod page of page entry t / page).  The list is cut
 // into chunks of c tokens, one CTA each; a CTA keeps the running maximum and sum of its softmax and one output row per
 // query head, and rows of several chunks leave (maximum, sum, unnormalised output) in the workspace in fp32 for
-// join_kernel, which adds them up in chunk order: the result depends on the lengths alone, not on timing.
+// join_kernel, which adds them up in chunk order: nothing depends on timing.  How a row is cut follows from its length, the
+// number of rows (sequences x key heads) and the width of the page table or the window or list (plan() below), so a
+// sequence may round differently in another batch or under a wider table.
 #include <limits.h>
 
 #include <cmath>
@@ -613,6 +615,8 @@ template <typename T> __global__ void __launch_bounds__(256) join_kernel(const D
     __shared__ float red[8], weight[256];
     const int64_t b = blockIdx.y, head = b * a.H + blockIdx.x, h = blockIdx.x / (unsigned)a.G;
     const int tid = threadIdx.x, D = (int)a.D, v = blockIdx.z * vecs + tid % vecs, k = tid / vecs;
+    // Ahead of the wait: the lengths were complete before the decode kernel began, which is a plain launch, and that kernel
+    // sets the same status bit (1.6 us of 106 for 4 sequences of 32768 tokens).
     const RowTokens row(a, b, h);
     const int64_t chunk = row.chunk(a);
     pdl_wait();

@@ -1,8 +1,9 @@
 // Programmatic dependent launch for chains of short kernels: a kernel launched with launch_after() may start while the
 // one before it in the stream drains, and waits in pdl_wait() until that one is complete and its writes are visible.
 // Every kernel of a chain calls pdl_trigger() as it starts (the next kernel's CTAs come only when all of this one's are
-// running or done), and every thread of a kernel launched this way calls pdl_wait() before it touches memory or returns:
-// so a kernel's completion means that all before it are complete.  Most of the launch gap between two kernels of a chain
+// running or done), and every thread of a kernel launched this way calls pdl_wait() before it touches memory that the chain
+// writes, and before it returns: so a kernel's completion means that all before it are complete.  What was complete before
+// the chain began may be read ahead of the wait.  Most of the launch gap between two kernels of a chain
 // goes that way; outside such a chain both instructions do nothing.
 #pragma once
 
