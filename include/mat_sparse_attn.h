@@ -428,7 +428,9 @@ size_t mat_select_blocks_workspace_bytes(int64_t B, int64_t S, int64_t H, int64_
  * k, v, dk, dv: [B, S, H_kv, D]; lse: [B, S, H] fp32, the natural logarithm of each row's sum of exp(scale * q . k).
  * D is a multiple of 8 up to 128.  An entry of blocks counts when it is a block of the sequence, is above every entry
  * before it in its row and, with causal, not behind the query's own block.  causal also hides the keys behind the
- * query.  A row without keys gives zeros, lse = -inf and no gradient.  The backward is deterministic (no atomics).
+ * query.  A row without keys gives zeros, lse = -inf and no gradient; one whose keys all score -inf gives NaN, as its
+ * softmax.  Infinities and NaN reach only the pairs that see them.  The backward is deterministic (no atomics).  The
+ * workspaces take at most 1 GiB, or what one (batch, key head) pair takes, plus 4 B S H bytes in the backward.
  */
 int mat_selected_attn_fwd(const void *q, const void *k, const void *v, void *o, float *lse, int64_t B, int64_t S,
                           int64_t H, int64_t H_kv, int64_t D, int dtype, const int32_t *blocks, int64_t block,

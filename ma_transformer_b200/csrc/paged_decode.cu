@@ -350,8 +350,9 @@ __global__ void __launch_bounds__(128) decode_simt_kernel(const DecodeArgs a) {
 // (128 KB a SM with two CTAs) and waited for without a CTA barrier.  A tile never crosses a page (pages of 16 tokens and
 // more), so its 16 rows share one table lookup, a warp looks up 32 tiles at a time, and rows are stepped through: forming
 // every copy's address took more issue slots than the mathematics (150 us instead of 140).
-// 64 sequences of up to 8192 tokens, 32 heads on 8 of 128 columns, 861 MB: 140 us = 6.15 TB/s, 95 % of the measured copy
-// rate; a call of 149 us with its join over states that L2 does not hold (5.8 TB/s).  4 of up to 131072: 6.06 TB/s.
+// 64 sequences of up to 8192 tokens, 32 heads on 8 of 128 columns, 861 MB: 140 us = 6.15 TB/s by ncu, 95 % of the measured
+// copy rate; a call of 154 to 158 us with its join over states that L2 does not hold (5.5 TB/s).  4 of up to 131072, 1254 MB:
+// a call of 217 to 220 us (5.7 TB/s).
 __device__ __forceinline__ void cp_async16(void *dst, const void *src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -737,7 +738,8 @@ template <typename T> int launch_decode(DecodeArgs &a, cudaStream_t s) {
 }
 
 // How many chunks a row may have, and their least size.  The lengths are on the device, so both come from the page
-// table's width; the kernels shorten the chunks' number, not their size, for shorter rows.
+// table's width; the kernels shorten the chunks' number, not their size, for shorter rows.  One sequence of 777 tokens x 8
+// heads of 64 takes 9.8 us under a table for up to 8192 tokens and 13.9 under any wider one.
 struct DecodePlan { int nsplit, min_chunk, cluster; };
 
 DecodePlan plan(const mat_paged_cache *c, int64_t B, int64_t width, int64_t left, int64_t n_sel) {

@@ -100,8 +100,8 @@ namespace {
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // One warp per 16 rows, NKP keys at a time; keys and values of the block are shared by the CTA's warps, each warp's
-// queries have two buffers of their own.  125 us at 8192 tokens x 8 heads of 64 x 16 blocks of 64 (ncu: L1 73 % busy,
-// tensor pipe 25 %, DRAM 23 %), where the partials alone are 268 MB written (41 us).  Tried and not faster: 32 rows a
+// queries have two buffers of their own.  120 to 129 us at 8192 tokens x 8 heads of 64 x 16 blocks of 64 (ncu: L1 73 % busy,
+// tensor pipe 25 to 27 %, DRAM 23 %), where the partials alone are 268 MB written (41 us).  Tried and not faster: 32 rows a
 // warp sharing each key fragment (126 us at 168 registers), partials leaving through shared memory as bulk copies of a
 // row each (135 us).  NKP = 32 instead of 64 in the exact kernels: 220 against 226 us for the whole forward.
 // EXACT: D == DP and a block is a whole number of NKP keys, known to the compiler.
@@ -402,8 +402,8 @@ template <typename T, int LPR, int AHEAD, bool BWD> __global__ void __launch_bou
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // A tile is 64 rows against up to NKP keys of one (sub-)block.  Warp w scores rows 16 w .. 16 w + 15 and writes their
 // share of dq; for dk and dv the weights and dS go through shared memory and warp w owns 16 keys (NKP = 64), or 16 keys
-// and half of the columns (NKP = 32).  Seven products of 16 x 64 x 64 per 16 rows (dq and dk count twice): 250 us at 8192 tokens x
-// 8 heads of 64 x 16 blocks of 64, tensor pipe 41 %, L1 70 % busy (fragments, P and dS, gathered rows), two CTAs a SM by
+// and half of the columns (NKP = 32).  Seven products of 16 x 64 x 64 per 16 rows (dq and dk count twice): 252 us at 8192 tokens x
+// 8 heads of 64 x 16 blocks of 64, tensor pipe 44 %, L1 67 % busy (fragments, P and dS, gathered rows), two CTAs a SM by
 // registers.  fp16 gradients want the loss scale that the library's other 16-bit backward kernels want: dS is held in
 // the inputs' type.
 // DELTA: the tile leaves each row's share of delta = sum p dp instead of gradients.  Where a row has few keys its output is

@@ -67,7 +67,7 @@ def forward_selected(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     An entry of ``blocks`` counts when it names a block of the sequence, is above every entry before it in its row and,
     with ``causal``, not behind the query's own block; other entries are skipped.  A row without keys is zero, its lse
-    -inf."""
+    -inf; a row whose keys all score -inf is NaN, as its softmax."""
     B, S, H, Hkv, D, dt = _shapes(query, key, value)
     topk = _check_blocks(blocks, query, Hkv)
     out = torch.empty_like(query)
@@ -85,7 +85,7 @@ def backward_selected(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
                       grad_out: torch.Tensor, blocks: torch.Tensor, block: int, causal: bool = True,
                       scale: Optional[float] = None) -> List[torch.Tensor]:
     """[dQ, dK, dV] of ``forward_selected``, given its results.  Deterministic (no atomics); the gradients of a shared
-    key head sum over its query heads."""
+    key head sum over its query heads.  Infinities and NaN reach the gradients of the pairs that see them only."""
     B, S, H, Hkv, D, dt = _shapes(query, key, value)
     topk = _check_blocks(blocks, query, Hkv)
     _check_inputs(query, out, grad_out)
