@@ -723,6 +723,8 @@ template <typename T> int run_simt(DecodeArgs &a, cudaStream_t s) {
          : vecs <= 32 ? launch_simt_heads<T, 32, 1>(a, gt, s) : launch_simt_heads<T, 32, 2>(a, gt, s);
 }
 
+// Ring places: three at 256 columns leave no less room (one CTA a SM either way) but start later: one sequence of 4000 tokens x
+// 4 heads of 256 takes 20.4 us with three and 18.8 with two, 64 of 8192 x 8 heads 663 and 667.
 template <typename T> int run_mma(DecodeArgs &a, cudaStream_t s) {
     a.tiles = (int)((a.H / a.Hkv + 15) / 16);
     return a.D <= 64 ? launch_mma<T, 64, 3>(a, s) : a.D <= 128 ? launch_mma<T, 128, 3>(a, s) : launch_mma<T, 256, 2>(a, s);
@@ -756,7 +758,10 @@ DecodePlan plan(const mat_paged_cache *c, int64_t B, int64_t width, int64_t left
     }
     // Every CTA pays some 4 us to look up its pages, fill its rings and write its result.  64 sequences of up to 8192
     // tokens x 8 key heads of 128: 172 us with chunks of 512 tokens and more, 163 with 1024, 159 with 2048; 32 x 2048
-    // chosen tokens x 8: 78, 61, 53 us.  Few rows need the shorter chunks to fill the GPU.
+    // chosen tokens x 8: 78, 61, 53 us.  Few rows need the shorter chunks to fill the GPU, and below 16 rows of up to 65536
+    // tokens chunks of 128: 46 us against 56 with 512 for one fp32 sequence of 60000 tokens x 1 head of 128 (16-bit: 24 us
+    // either way; 8 heads of 64: 37 against 33).  Elsewhere 512: 131072 tokens x 1 head 24 against 41 with 128, 16 x 2048 x 8
+    // heads 35 against 56, 4 x 9000 x 4 heads 26 against 31 (fp32, 4 x 16000 x 8 heads: 136 against 128).
     p.min_chunk = rows >= kSms ? 2048 : rows >= 16 || most > 65536 ? 512 : 128;
     int64_t cap = 16 * kSms / rows;
     if (cap < 8) cap = 8;
