@@ -388,7 +388,7 @@ int mat_paged_append(const mat_paged_cache *cache, const void *k_new, const void
  *   `dilation`.
  *   pages: [B, H_kv, n_sel] logical pages to read instead (ascending and distinct, as mat_paged_select leaves them;
  *   negative entries and entries past the length are skipped), or NULL.
- *   scale <= 0 selects 1/sqrt(D).  A row that sees no token is zero.
+ *   scale <= 0 selects 1/sqrt(D).  A row that sees no token, or only such as score -inf, is zero.
  */
 int mat_paged_decode(const mat_paged_cache *cache, const void *q, int64_t q_stride, void *o, int64_t B, int64_t H,
                      const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,

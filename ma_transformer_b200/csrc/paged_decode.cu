@@ -723,7 +723,7 @@ template <typename T> int run_simt(DecodeArgs &a, cudaStream_t s) {
          : vecs <= 32 ? launch_simt_heads<T, 32, 1>(a, gt, s) : launch_simt_heads<T, 32, 2>(a, gt, s);
 }
 
-// Ring places: three at 256 columns leave no less room (one CTA a SM either way) but start later: one sequence of 4000 tokens x
+// Ring places: at 256 columns three fit as well (one CTA a SM either way) but start later: one sequence of 4000 tokens x
 // 4 heads of 256 takes 20.4 us with three and 18.8 with two, 64 of 8192 x 8 heads 663 and 667.
 template <typename T> int run_mma(DecodeArgs &a, cudaStream_t s) {
     a.tiles = (int)((a.H / a.Hkv + 15) / 16);

@@ -205,7 +205,7 @@ def decode(query: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, l
     """Attention of one new token per sequence over the cached ones: [B, H, head_dim].
 
     query: [B, H, head_dim], H a multiple of the cache's heads (query head h reads key head h // (H / n_kv_heads)).
-    lengths: [B] int32 cached tokens, the new one included; 0 gives a zero row.
+    lengths: [B] int32 cached tokens, the new one included; 0 gives a zero row, as do scores that are all -inf.
     spec: a window ``PatternSpec`` (its ``right`` taps lie in the future and select nothing); pages: the
     [B, n_kv_heads, n] int32 result of ``select_pages``.  With neither, every cached token is read.
     """
